@@ -17,12 +17,17 @@ F32, BF16 = 0, 1
 PAIR_HALF, PAIR_INTERLEAVED = 0, 1
 GEMM_STORE, GEMM_ADD_RESIDUAL = 0, 1
 
-ERR_TOKEN_RANGE, ERR_NONFINITE_LOGIT, ERR_PAGE_RANGE, ERR_WAIT_EXPIRED = 1, 2, 4, 8
+LEVEL_INT8, LEVEL_E4M3 = 0, 1
+BLOCK_TOKENS = 16                # positions of a block of the 8-bit cache
+
+ERR_TOKEN_RANGE, ERR_NONFINITE_LOGIT, ERR_PAGE_RANGE, ERR_WAIT_EXPIRED, ERR_NOTHING_ALLOWED, ERR_HISTORY = 1, 2, 4, 8, 16, 32
 _ERR_TEXT = {
     ERR_TOKEN_RANGE: "a token id outside [0, vocab) reached the embedding kernel",
     ERR_NONFINITE_LOGIT: "sampling saw a NaN or infinite logit",
     ERR_PAGE_RANGE: "a page-table entry outside the page pool was read",
     ERR_WAIT_EXPIRED: "a bounded wait inside a kernel expired",
+    ERR_NOTHING_ALLOWED: "a row's mask and biases left no token to choose",
+    ERR_HISTORY: "a token history that does not exist, or has no room for another token",
 }
 
 
@@ -36,6 +41,14 @@ class KvView(Structure):
                 ("table_width", c_int), ("ring_pages", c_int), ("page_tokens", c_int),
                 ("n_pages", c_int), ("kv_heads", c_int), ("head_dim", c_int),
                 ("dtype", c_int), ("window", c_int), ("chunk", c_int), ("keep", c_int), ("keep_pages", c_int)]
+
+
+class BlockView(Structure):
+    """Mirror of `IertBlockView` (block_cache.cuh); `block_view` makes one."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p), ("weight", c_void_p),
+                ("tail_k", c_void_p), ("tail_v", c_void_p), ("page_table", c_void_p), ("shift", c_void_p),
+                ("n_slots", c_int), ("table_width", c_int), ("ring_pages", c_int), ("n_pages", c_int), ("kv_heads", c_int),
+                ("head_dim", c_int), ("page_tokens", c_int), ("window", c_int), ("format", c_int), ("tail_dtype", c_int)]
 
 
 class BatchView(Structure):
@@ -143,7 +156,14 @@ def _declare(lib) -> None:
         "iert_attention_plain": [P, P, c_int, POINTER(BatchView), POINTER(KvView), c_int, c_float, c_int, c_float, P, P, S],
         "iert_sample_greedy": [P, c_int, c_int, c_longlong, P, P, S],
         "iert_sample_temperature": [P, c_int, c_int, c_longlong, c_float, c_ulonglong, P, P, P, P, S],
+        "iert_sample_temperature_masked": [P, c_int, c_int, c_longlong, c_float, c_ulonglong, P, P, P, P, S],
         "iert_uniform_draws": [c_ulonglong, P, P, P, c_int, S],
+        "iert_logit_rules": [P, c_int, c_int, c_longlong, P, c_longlong, P, c_int, c_int, P, P, P, P, P, c_longlong, P, c_longlong, P, P, P, S],
+        "iert_history_append": [P, c_int, c_int, P, P, P, c_int, P, S],
+        "iert_block_store": [P, c_int, POINTER(BatchView), POINTER(BlockView), P, S],
+        "iert_block_attention_plain": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, P, S],
+        "iert_block_evict": [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int,
+                             P, P, P, S],
         "iert_gemm_tc": [P, c_longlong, P, c_longlong, P, c_int, c_longlong, c_int, c_int, c_int, c_int,
                          P, c_longlong, P, c_int, c_int, c_int, c_int, POINTER(Epilogue), P, S],
         "iert_epilogue_rows": [P, c_int, c_longlong, c_int, c_int, POINTER(Epilogue), S],
@@ -394,6 +414,94 @@ def sample_temperature(logits, temperature: float, seed: int, request_ids, step_
                                          temperature, seed & 0xFFFFFFFFFFFFFFFF,
                                          request_ids.data_ptr(), step_ids.data_ptr(), out.data_ptr(),
                                          err.data_ptr(), stream), "sample_temperature")
+
+
+def sample_temperature_masked(logits, temperature: float, seed: int, request_ids, step_ids, out, err, stream) -> None:
+    """`sample_temperature` with ids whose logit is -infinity ruled out."""
+    rows, vocab = logits.shape
+    check(core().iert_sample_temperature_masked(logits.data_ptr(), rows, vocab, logits.stride(0), temperature, seed & 0xFFFFFFFFFFFFFFFF,
+                                                request_ids.data_ptr(), step_ids.data_ptr(), out.data_ptr(), err.data_ptr(), stream),
+          "sample_temperature_masked")
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise KernelError(what)
+
+
+def _on_current_device(*tensors) -> None:
+    """A kernel is launched on the current device and stream: memory of another device, or of the host, is not its to read."""
+    here = -1
+    for t in tensors:
+        if t is None:
+            continue
+        d = t.get_device()
+        if d < 0 or (here >= 0 and d != here):
+            raise KernelError("the tensors must be on one CUDA device")
+        here = d
+    if here >= 0 and here != torch.cuda.current_device():
+        raise KernelError(f"the tensors are on cuda:{here}, which is not the current device")
+
+
+def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, penalties=None, bias=None, mask=None, chosen=None,
+                lens_out=None) -> None:
+    """Penalties for repeated tokens, biases and a mask on logits fp32 [R, vocab] (any row stride), and the best token left.
+
+    out          fp32 [R, vocab]: the logits after the rules (may be `logits` itself), or None
+    history      int32 [H, width]: row h holds the tokens of a request, prompt first; lens, prompt_lens int32 [H]: how many in all
+                 and how many of them are the prompt's; rows int32 [R]: the history of each logits row, all different (None: row r has
+                 history r).  Tokens outside the vocabulary count for nothing.  history None: no row has one
+    penalties    fp32 [H, 3]: repetition r > 0 (a seen id: x / r if x > 0 else x * r), presence a, frequency f (an id with c > 0
+                 occurrences in the answer: x - f c - a)
+    bias         fp32 [vocab] or [R, vocab], added after the penalties; -infinity rules an id out
+    mask         int32 [R, ceil(vocab / 32)] or [1, ...]: bit i % 32 of word i // 32 set = id i is allowed
+    chosen       int32 [R]: the id of the largest result, the lowest of equal ones; 0 and an error bit where nothing is left
+    lens_out     int32 [H] (may be `lens`): the choice is appended to its history and the length plus one is written here
+    """
+    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1, "logits must be float32 [rows, vocab] with contiguous rows")
+    R, vocab = logits.shape
+    if out is not None:
+        _need(out.shape == logits.shape and out.dtype == torch.float32 and out.stride(1) == 1, "out must be float32 like logits")
+    H = width = 0
+    if history is not None:
+        _need(history.dim() == 2 and history.dtype == torch.int32 and history.is_contiguous(), "history must be contiguous int32 [histories, width]")
+        H, width = history.shape
+        for t, name in ((lens, "lens"), (prompt_lens, "prompt_lens")):
+            _need(t is not None and t.dtype == torch.int32 and t.shape == (H,) and t.is_contiguous(), f"{name} must be int32 [{H}]")
+        _need(rows is None or (rows.dtype == torch.int32 and rows.shape == (R,) and rows.is_contiguous()), f"rows must be int32 [{R}]")
+        _need(lens_out is None or (lens_out.dtype == torch.int32 and lens_out.shape == (H,) and lens_out.is_contiguous()), f"lens_out must be int32 [{H}]")
+        _need(lens_out is None or chosen is not None, "lens_out needs chosen")
+    else:
+        _need(penalties is None and lens_out is None, "penalties and lens_out need a history")
+    _need(penalties is None or (penalties.dtype == torch.float32 and penalties.shape == (H, 3) and penalties.is_contiguous()),
+          f"penalties must be float32 [{H}, 3]")
+    ld_bias = ld_mask = 0
+    if bias is not None:
+        _need(bias.dtype == torch.float32 and bias.stride(-1) == 1 and (bias.shape == (vocab,) or bias.shape == (R, vocab)),
+              "bias must be float32 [vocab] or [rows, vocab]")
+        ld_bias = bias.stride(0) if bias.dim() == 2 else 0
+    if mask is not None:
+        words = -(-vocab // 32)
+        _need(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[1] == words and mask.shape[0] in (1, R) and mask.stride(1) == 1,
+              f"mask must be int32 [rows or 1, {words}]")
+        ld_mask = mask.stride(0) if mask.shape[0] == R and R > 1 else 0
+    _need(chosen is None or (chosen.dtype == torch.int32 and chosen.shape == (R,) and chosen.is_contiguous()), f"chosen must be int32 [{R}]")
+    _on_current_device(logits, out, history, lens, prompt_lens, rows, penalties, bias, mask, chosen, lens_out, err)
+    check(core().iert_logit_rules(logits.data_ptr(), R, vocab, logits.stride(0), _ptr(out), out.stride(0) if out is not None else 0,
+                                  _ptr(history), width, H, _ptr(lens) if H else None, _ptr(prompt_lens) if H else None, _ptr(rows) if H else None,
+                                  _ptr(penalties), _ptr(bias), ld_bias, _ptr(mask), ld_mask, _ptr(chosen), _ptr(lens_out), err.data_ptr(), stream),
+          "logit_rules")
+
+
+def history_append(history, lens, rows, tokens, err, stream) -> None:
+    """tokens[r] (int32 [R]) joins the history of row rows[r] (all different)."""
+    _need(history.dim() == 2 and history.dtype == torch.int32 and history.is_contiguous(), "history must be contiguous int32 [histories, width]")
+    _need(lens.dtype == torch.int32 and lens.shape == (history.shape[0],) and lens.is_contiguous(), "lens must be int32, one per history")
+    _need(tokens.dtype == torch.int32 and tokens.dim() == 1 and tokens.is_contiguous(), "tokens must be int32 [rows]")
+    _need(rows is None or (rows.dtype == torch.int32 and rows.shape == tokens.shape and rows.is_contiguous()), "rows must be int32, one per token")
+    _on_current_device(history, lens, rows, tokens, err)
+    check(core().iert_history_append(history.data_ptr(), history.shape[1], history.shape[0], lens.data_ptr(), _ptr(rows), tokens.data_ptr(),
+                                     tokens.shape[0], err.data_ptr(), stream), "history_append")
 
 
 def uniform_draws(seed: int, request_ids, step_ids, out, stream) -> None:
@@ -1114,3 +1222,132 @@ def selective_scan(u, dt, dt_bias, bc, z, A2, D, state, s_off: int, out, C: int,
     check(core().iert_selective_scan(u.data_ptr(), dtype_code(u.dtype), dt.data_ptr(), dt_bias.data_ptr(), bc.data_ptr(), bc.stride(0), z.data_ptr(),
                                      z.stride(0), A2.data_ptr(), D.data_ptr(), state.data_ptr(), state.stride(0), s_off,
                                      out.data_ptr(), C, N, 1 if one_token else 0, byref(batch), stream), "selective_scan")
+
+
+# ---------------------------------------------------------------------------------------
+# the cache in 8 bits
+
+LEVEL_TYPES = {torch.int8: LEVEL_INT8, torch.float8_e4m3fn: LEVEL_E4M3}
+
+
+def block_view(k, v, k_scale, v_scale, tail_k, tail_v, page_table, *, window: int = 0, ring_pages: Optional[int] = None, weight=None,
+               shift=None) -> BlockView:
+    """One layer's keys and values in 8 bits, as the block kernels receive them (csrc/block_cache.cuh).
+
+    k, v               int8 or float8_e4m3fn [n_pages, kv_heads, page_tokens, head_dim], page_tokens a multiple of 16
+    k_scale, v_scale   fp32 [n_pages, kv_heads, page_tokens / 16]: a level stands for level * scale
+    tail_k, tail_v     bf16 or fp32 [n_slots, kv_heads, 16, head_dim]: the positions behind a sequence's last finished block
+    page_table         int32 [n_slots, width]
+    weight             fp32 like k_scale, or None: accumulated attention weight of each block (not together with a window)
+    shift              int32 [n_slots] or None: positions a sequence has lost to eviction
+    """
+    _need(k.dim() == 4 and k.dtype in LEVEL_TYPES and v.dtype == k.dtype and v.shape == k.shape, "k and v must be int8 or float8_e4m3fn of one shape "
+          "[pages, kv_heads, page_tokens, head_dim]")
+    n_pages, kv_heads, page_tokens, head_dim = k.shape
+    _need(page_tokens % BLOCK_TOKENS == 0 and page_tokens > 0, f"a page must be a multiple of {BLOCK_TOKENS} positions, got {page_tokens}")
+    scales = (n_pages, kv_heads, page_tokens // BLOCK_TOKENS)
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale"), (weight, "weight")):
+        _need((t is None and name == "weight") or (t.dtype == torch.float32 and t.shape == scales and t.is_contiguous()),
+              f"{name} must be contiguous float32 {list(scales)}")
+    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous(), "the page table must be contiguous int32 [slots, width]")
+    n_slots, width = page_table.shape
+    tail = (n_slots, kv_heads, BLOCK_TOKENS, head_dim)
+    _need(tail_k.shape == tail and tail_v.shape == tail and tail_k.dtype == tail_v.dtype, f"tail_k and tail_v must be {list(tail)} of one type")
+    for t, name in ((k, "k"), (v, "v"), (tail_k, "tail_k"), (tail_v, "tail_v")):
+        _need(t.is_contiguous(), f"{name} must be contiguous")
+    _need(weight is None or not window, "block weights are kept for caches without a window")
+    _need(shift is None or (shift.dtype == torch.int32 and shift.shape == (n_slots,) and shift.is_contiguous()), f"shift must be int32 [{n_slots}]")
+    ring = width if ring_pages is None else ring_pages
+    _need(0 < ring <= width and (ring == width or window), "a ring is part of a table row, and needs a window")
+    _need(not window or ring * page_tokens >= min(window, width * page_tokens), "a ring must hold the window")
+    view = BlockView(k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), weight=_ptr(weight),
+                     tail_k=tail_k.data_ptr(), tail_v=tail_v.data_ptr(), page_table=page_table.data_ptr(), shift=_ptr(shift), n_slots=n_slots,
+                     table_width=width, ring_pages=ring, n_pages=n_pages, kv_heads=kv_heads, head_dim=head_dim, page_tokens=page_tokens,
+                     window=window or 0, format=LEVEL_TYPES[k.dtype], tail_dtype=dtype_code(tail_k.dtype))
+    view.tensors = (k, v, k_scale, v_scale, tail_k, tail_v, page_table, weight, shift)      # they live as long as the view
+    return view
+
+
+def _packed_rows(qkv, heads: int, view: BlockView) -> None:
+    _need(qkv.dim() == 2 and qkv.is_contiguous() and dtype_code(qkv.dtype) == view.tail_dtype
+          and qkv.shape[1] == (heads + 2 * view.kv_heads) * view.head_dim,
+          "the projection must be contiguous [tokens, (heads + 2 kv_heads) * head_dim] of the tails' type")
+
+
+def block_store(qkv, batch: BatchView, view: BlockView, heads: int, err, stream) -> None:
+    """Write the keys and values of the step's tokens (packed [T, heads | kv_heads | kv_heads] x head_dim, as they stand) into the
+    cache: finished blocks as levels and scales, the rest of a sequence as it is; the weights of blocks that begin here are set to 0."""
+    _packed_rows(qkv, heads, view)
+    _need(qkv.shape[0] >= batch.n_tokens, "fewer rows than tokens")
+    _on_current_device(qkv, view.tensors[0], err)
+    check(core().iert_block_store(qkv.data_ptr(), heads, byref(batch), byref(view), err.data_ptr(), stream), "block_store")
+
+
+def block_attention_scratch_floats(n_seqs: int, heads: int, view: BlockView) -> int:
+    """Floats of scratch that `block_attention` needs for steps of up to `n_seqs` sequences."""
+    return n_seqs * heads * view.table_width * (view.page_tokens // BLOCK_TOKENS) if view.weight else 1
+
+
+def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,
+                    weight_out=None, plain: bool = False) -> None:
+    """One-token attention over the 8-bit cache, which the step's own key and value join; `out` [n_seqs, heads * head_dim] of the
+    projection's type (rows of padding sequences: 0).
+
+    rope         (inv_freq, rotary_dim, pairing, factor): the kernel rotates queries and the new key by the position, evicted ones included
+    weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
+                 sequences' own blocks are written
+    plain        the kernel that computes as the equations say
+    """
+    _packed_rows(qkv, heads, view)
+    _need(batch.n_tokens == batch.n_seqs and qkv.shape[0] >= batch.n_seqs, "a one-token step has one row per sequence")
+    _need(heads % view.kv_heads == 0, f"heads {heads} is not a multiple of kv_heads {view.kv_heads}")
+    _need(out.dtype == qkv.dtype and out.is_contiguous() and out.numel() >= batch.n_seqs * heads * view.head_dim, "out must be [sequences, heads * head_dim]")
+    weights = weight_out.data_ptr() if weight_out is not None else view.weight
+    _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
+    _need(weight_out is None or (view.weight is not None and weight_out.dtype == torch.float32 and weight_out.is_contiguous()
+                                 and weight_out.shape == view.tensors[7].shape), "weight_out must be laid out as the view's weight")
+    if view.weight:
+        _need(scratch is not None and scratch.dtype == torch.float32 and
+              scratch.numel() >= block_attention_scratch_floats(batch.n_seqs, heads, view), "scratch is too small")
+    inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
+    check(core().iert_block_attention_plain(qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq),
+                                            rotary_dim, pairing, factor, err.data_ptr(), stream), "block_attention")
+
+
+def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, keep: int, recent: int, kept, err, stream, *, slots=None,
+                shift=None) -> None:
+    """Of each sequence's finished blocks keep `keep`: the last `recent` and, among the others, those with the largest weight (of
+    equal ones the lower index), in their order, copied with scales and weights to `new_pages`; the weight of an unfinished block goes along.
+
+    k, v, k_scale, v_scale, weight   the pools of all layers, as `block_view` takes them with an axis of layers in front
+    page_table     int32 [rows, width]; sequence i is row slots[i] (slots int32 [n], None: row i)
+    lengths        int32 [n]: positions that each sequence holds; one with at most `keep` finished blocks keeps them all
+    new_pages      int32 [n, >= keep * 16 / page_tokens, and room for the unfinished block]: pages that no sequence uses, all different
+    kept           int32 [layers, n, kv_heads, keep]: the numbers of the kept blocks (-1 behind the last of a sequence with fewer)
+    shift          int32 [rows] or None: grows by the positions that a sequence loses
+    """
+    _need(k.dim() == 5 and k.dtype in LEVEL_TYPES and v.dtype == k.dtype and v.shape == k.shape and k.is_contiguous() and v.is_contiguous(),
+          "k and v must be contiguous int8 or float8_e4m3fn [layers, pages, kv_heads, page_tokens, head_dim]")
+    layers, n_pages, kv_heads, page_tokens, head_dim = k.shape
+    _need(page_tokens % BLOCK_TOKENS == 0, f"a page must be a multiple of {BLOCK_TOKENS} positions")
+    scales = (layers, n_pages, kv_heads, page_tokens // BLOCK_TOKENS)
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale"), (weight, "weight")):
+        _need(t is not None and t.dtype == torch.float32 and t.shape == scales and t.is_contiguous(), f"{name} must be contiguous float32 {list(scales)}")
+    n = lengths.shape[0]
+    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous(), "the page table must be contiguous int32")
+    rows, width = page_table.shape
+    _need(lengths.dtype == torch.int32 and lengths.is_contiguous() and (slots is not None or n <= rows), "lengths must be int32, one per sequence")
+    _need(slots is None or (slots.dtype == torch.int32 and slots.shape == (n,) and slots.is_contiguous()), f"slots must be int32 [{n}]")
+    _need(0 < keep and 0 <= recent <= keep, f"keep {keep} must be positive and recent {recent} between 0 and keep")
+    _need(new_pages.dtype == torch.int32 and new_pages.dim() == 2 and new_pages.shape[0] == n and new_pages.is_contiguous()
+          and new_pages.shape[1] * page_tokens >= keep * BLOCK_TOKENS, "new_pages must be int32 [sequences, pages] with room for the kept blocks")
+    _need(kept.dtype == torch.int32 and kept.shape == (layers, n, kv_heads, keep) and kept.is_contiguous(),
+          f"kept must be int32 {[layers, n, kv_heads, keep]}")
+    _need(shift is None or (shift.dtype == torch.int32 and shift.shape == (rows,) and shift.is_contiguous()), f"shift must be int32 [{rows}]")
+    _on_current_device(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, kept, slots, shift, err)
+    check(core().iert_block_evict(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), weight.data_ptr(), layers, n_pages, kv_heads,
+                                  page_tokens, head_dim, page_table.data_ptr(), width, rows, _ptr(slots), lengths.data_ptr(), n,
+                                  new_pages.data_ptr(), new_pages.shape[1], keep, recent, width * (page_tokens // BLOCK_TOKENS),
+                                  kept.data_ptr(), _ptr(shift), err.data_ptr(), stream), "block_evict")
+    global launch_count
+    launch_count += 1                # (two kernels)

@@ -24,6 +24,8 @@ enum : int {
   IERT_ERR_NONFINITE_LOGIT = 2, // sampling saw NaN or Inf
   IERT_ERR_PAGE_RANGE = 4,      // a page-table entry outside the pool
   IERT_ERR_WAIT_EXPIRED = 8,    // a bounded wait inside a kernel ran out
+  IERT_ERR_NOTHING_ALLOWED = 16, // a row's mask and biases left no token to choose
+  IERT_ERR_HISTORY = 32,        // a token history that does not exist, or has no room for another token
 };
 
 // Rotary pairings: partner of element k.

@@ -1,0 +1,208 @@
+// Penalties for repeated tokens, biases and a mask on a step's logits, and the best token that is left, in one pass:
+//   x = logits[r, i];  i seen in row r's history: x / rep if x > 0 else x * rep
+//   i among the history's answer, c > 0 times: x - freq * c - pres       (products and differences rounded one by one, in this order)
+//   x + bias[i];  -infinity where the mask has no bit for i
+// A cluster of eight CTAs shares a row: each owns an eighth of the vocabulary, counts the history's tokens that fall into it in
+// shared memory, applies the rules to its logits as they stream by and keeps the best; the eight bests meet in the first CTA's
+// shared memory, which appends the choice to the row's history.  One launch, and nothing but the logits crosses the memory.
+#include <cooperative_groups.h>
+
+#include <utility>
+
+#include "common.cuh"
+
+namespace cg = cooperative_groups;
+using namespace iert;
+
+namespace {
+
+constexpr int THREADS = 512, CLUSTER = 8;
+constexpr int WINDOW = 24576;                 // ids whose counts stand in shared memory at a time (96 KB)
+constexpr uint32_t SEEN = 0x80000000u;
+
+struct RulesParams {
+  const float* logits; long long ld;
+  float* out; long long ld_out;               // null: the rules' results are not written
+  int vocab;
+  int* history; int width, hist_rows;         // [hist_rows][width]
+  const int *lens, *prompt_lens;              // [hist_rows]
+  const int* rows;                            // history row of each logits row (null: its own number)
+  const float* penalties;                     // [hist_rows][3]: repetition, presence, frequency; null: none
+  const float* bias; long long ld_bias;       // 0: one row for all
+  const uint32_t* mask; long long ld_mask;    // words of 32 ids, bit i % 32 of word i / 32; ld 0: one row for all
+  int* chosen;                                // null: no choice is made
+  int* lens_out;                              // null: nothing is appended
+  int chunk, vec;
+  int* err;
+};
+
+__device__ __forceinline__ bool better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
+
+__global__ void __launch_bounds__(THREADS) logit_rules_kernel(RulesParams p) {
+  extern __shared__ uint32_t counts[];
+  __shared__ float vs[THREADS / 32];
+  __shared__ int is[THREADS / 32];
+  __shared__ float best_v[CLUSTER];
+  __shared__ int best_i[CLUSTER];
+  cg::cluster_group cluster = cg::this_cluster();
+  cg::cluster_group::arrival_token started;
+  if (p.chosen) started = cluster.barrier_arrive();
+  pdl_launch_dependents();
+  pdl_wait();
+  const int rank = cluster.block_rank(), r = blockIdx.x / CLUSTER, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int h = p.rows ? p.rows[r] : r;
+  if (h < 0 || h >= p.hist_rows) {            // no such history: the row is treated as one without
+    if (p.hist_rows > 0 && rank == 0 && tid == 0) atomicOr(p.err, IERT_ERR_HISTORY);
+    h = -1;
+  }
+  const int len = h >= 0 ? min(max(p.lens[h], 0), p.width) : 0;
+  const int prompt = h >= 0 ? p.prompt_lens[h] : 0;
+  const bool counted = p.penalties && h >= 0;
+  const float rep = counted ? p.penalties[3 * h] : 1.f, pres = counted ? p.penalties[3 * h + 1] : 0.f, freq = counted ? p.penalties[3 * h + 2] : 0.f;
+  const float* row = p.logits + (long long)r * p.ld;
+  float* out = p.out ? p.out + (long long)r * p.ld_out : nullptr;
+  const float* bias = p.bias ? p.bias + (long long)r * p.ld_bias : nullptr;
+  const uint32_t* mask = p.mask ? p.mask + (long long)r * p.ld_mask : nullptr;
+  const int* hist = p.history + (long long)max(h, 0) * p.width;
+  const int lo = min(p.vocab, rank * p.chunk), hi = min(p.vocab, lo + p.chunk);
+
+  float bv = -INFINITY;
+  int bi = 0x7fffffff;
+  bool bad = false;
+  auto rule = [&](float x, uint32_t c, int i, float b, bool allowed) {
+    if (allowed && !isfinite(x)) bad = true;  // the model's logits are finite, as for the samplers
+    if (c) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+    c &= ~SEEN;
+    if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)c)), pres);
+    if (bias) x = __fadd_rn(x, b);
+    if (!allowed) x = -INFINITY;
+    else if (!(x < INFINITY)) bad = true;     // a bias of -infinity rules an id out; one of +infinity or NaN is a mistake
+    if (x > -INFINITY && better(x, i, bv, bi)) { bv = x; bi = i; }
+    return x;
+  };
+  for (int w0 = lo; w0 < hi; w0 += WINDOW) {
+    const int w1 = min(hi, w0 + WINDOW);
+    if (counted) {
+      __syncthreads();                        // the counts of the window before are read
+      for (int i = tid; i < w1 - w0; i += THREADS) counts[i] = 0;
+      __syncthreads();
+      for (int j = tid; j < len; j += THREADS) {
+        const int id = hist[j] - w0;
+        if (id >= 0 && id < w1 - w0) {
+          if (j >= prompt) atomicAdd(&counts[id], 1u); else atomicOr(&counts[id], SEEN);
+        }
+      }
+      __syncthreads();
+    }
+    if (p.vec) {
+      for (int i = w0 + 4 * tid; i < w1; i += 4 * THREADS) {      // chunks, windows and rows are whole runs of four here
+        const float4 x = *reinterpret_cast<const float4*>(row + i);
+        const uint4 c = counted ? *reinterpret_cast<const uint4*>(counts + (i - w0)) : make_uint4(0, 0, 0, 0);
+        const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const uint32_t m = mask ? mask[i >> 5] >> (i & 31) : 0xfu;
+        float4 y;
+        y.x = rule(x.x, c.x, i, b.x, m & 1);
+        y.y = rule(x.y, c.y, i + 1, b.y, m & 2);
+        y.z = rule(x.z, c.z, i + 2, b.z, m & 4);
+        y.w = rule(x.w, c.w, i + 3, b.w, m & 8);
+        if (out) *reinterpret_cast<float4*>(out + i) = y;
+      }
+    } else {
+      for (int i = w0 + tid; i < w1; i += THREADS) {
+        const float y = rule(row[i], counted ? counts[i - w0] : 0u, i, bias ? bias[i] : 0.f, !mask || ((mask[i >> 5] >> (i & 31)) & 1));
+        if (out) out[i] = y;
+      }
+    }
+  }
+  if (bad) atomicOr(p.err, IERT_ERR_NONFINITE_LOGIT);
+  if (!p.chosen) return;                      // (the same for the whole cluster)
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
+    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
+    if (better(ov, oi, bv, bi)) { bv = ov; bi = oi; }
+  }
+  if (lane == 0) { vs[warp] = bv; is[warp] = bi; }
+  __syncthreads();
+  cluster.barrier_wait(std::move(started));   // the first CTA runs: its shared memory may be written
+  if (tid == 0) {
+    for (int w = 1; w < THREADS / 32; ++w)
+      if (better(vs[w], is[w], bv, bi)) { bv = vs[w]; bi = is[w]; }
+    *cluster.map_shared_rank(&best_v[rank], 0) = bv;
+    *cluster.map_shared_rank(&best_i[rank], 0) = bi;
+  }
+  cluster.sync();                             // every CTA has read the history's length by now
+  if (rank != 0 || tid != 0) return;
+  for (int c = 0; c < CLUSTER; ++c)
+    if (better(best_v[c], best_i[c], bv, bi)) { bv = best_v[c]; bi = best_i[c]; }
+  if (bi == 0x7fffffff) {
+    atomicOr(p.err, IERT_ERR_NOTHING_ALLOWED);
+    bi = 0;
+  }
+  p.chosen[r] = bi;
+  if (p.lens_out && h >= 0) {
+    if (len < p.width) p.history[(long long)h * p.width + len] = bi;
+    else atomicOr(p.err, IERT_ERR_HISTORY);
+    p.lens_out[h] = min(len + 1, p.width);
+  }
+}
+
+__global__ void history_append_kernel(int* history, int width, int hist_rows, int* lens, const int* rows, const int* tokens, int n, int* err) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int r = blockIdx.x * blockDim.x + threadIdx.x;
+  if (r >= n) return;
+  const int h = rows ? rows[r] : r;
+  if (h < 0 || h >= hist_rows || lens[h] < 0 || lens[h] >= width) {
+    atomicOr(err, IERT_ERR_HISTORY);
+    return;
+  }
+  history[(long long)h * width + lens[h]] = tokens[r];
+  lens[h] += 1;
+}
+
+}  // namespace
+
+IERT_API int iert_logit_rules(const float* logits, int rows_n, int vocab, long long ld, float* out, long long ld_out, int* history, int width,
+                              int hist_rows, const int* lens, const int* prompt_lens, const int* rows, const float* penalties, const float* bias,
+                              long long ld_bias, const void* mask, long long ld_mask, int* chosen, int* lens_out, int* err, cudaStream_t stream) {
+  if (rows_n <= 0) return IERT_OK;
+  if (vocab <= 0 || (long long)rows_n * CLUSTER > 0x7fffffffLL || (hist_rows > 0 && (!history || !lens || !prompt_lens || width <= 0)) ||
+      (hist_rows <= 0 && (penalties || lens_out)))
+    return IERT_BAD_ARGUMENT;
+  RulesParams p = {};
+  p.logits = logits; p.ld = ld; p.out = out; p.ld_out = ld_out; p.vocab = vocab; p.history = history; p.width = width; p.hist_rows = hist_rows;
+  p.lens = lens; p.prompt_lens = prompt_lens; p.rows = rows; p.penalties = penalties; p.bias = bias; p.ld_bias = ld_bias;
+  p.mask = (const uint32_t*)mask; p.ld_mask = ld_mask; p.chosen = chosen; p.lens_out = lens_out; p.err = err;
+  // each CTA's share: whole runs of 128 ids (four words of the mask, 16-byte runs)
+  const long long chunk = (((long long)vocab + CLUSTER - 1) / CLUSTER + 127) / 128 * 128;
+  p.chunk = (int)(chunk < 0x7fffff80LL / CLUSTER ? chunk : 0x7fffff80LL / CLUSTER / 128 * 128);
+  if ((long long)p.chunk * CLUSTER < vocab) return IERT_BAD_ARGUMENT;
+  p.vec = vocab % 4 == 0 && ld % 4 == 0 && (uintptr_t)logits % 16 == 0 && (!out || (ld_out % 4 == 0 && (uintptr_t)out % 16 == 0)) &&
+          (!bias || (ld_bias % 4 == 0 && (uintptr_t)bias % 16 == 0));
+  const size_t smem = penalties ? sizeof(uint32_t) * (size_t)(p.chunk < WINDOW ? p.chunk : WINDOW) : 0;
+  if (smem > 40 * 1024) cudaFuncSetAttribute(logit_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows_n * CLUSTER));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CLUSTER; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = iert_pdl_enabled ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, logit_rules_kernel, p);
+  return iert_check_launch("logit_rules");
+}
+
+// tokens[r] joins the history of row rows[r] (null: r); the rows are distinct.
+IERT_API int iert_history_append(int* history, int width, int hist_rows, int* lens, const int* rows, const int* tokens, int n, int* err,
+                                 cudaStream_t stream) {
+  if (n <= 0) return IERT_OK;
+  if (width <= 0 || hist_rows <= 0) return IERT_BAD_ARGUMENT;
+  launch_dep(history_append_kernel, dim3((n + 127) / 128), dim3(128), 0, stream, history, width, hist_rows, lens, rows, tokens, n, err);
+  return iert_check_launch("history_append");
+}

@@ -77,6 +77,9 @@ argmax_kernel(const float* __restrict__ logits, int vocab, long long ld, int* __
 // Thread t owns the contiguous ids [t*chunk, (t+1)*chunk).  Sums: each thread adds its
 // chunk in id order; thread totals are scanned in thread order.  The chosen id is the
 // first one whose running sum exceeds r * total.
+// MASKED: an id whose logit is -infinity is ruled out: it weighs nothing and is never chosen, not even where rounding leaves the
+// draw behind the last running sum.
+template <bool MASKED>
 __global__ void __launch_bounds__(THREADS)
 temperature_kernel(const float* __restrict__ logits, int vocab, long long ld, float temperature,
                    uint64_t seed, const int* __restrict__ request_ids,
@@ -95,14 +98,15 @@ temperature_kernel(const float* __restrict__ logits, int vocab, long long ld, fl
   bool bad = false;
   for (int i = lo; i < hi; ++i) {
     const float v = row[i];
-    if (!isfinite(v)) bad = true;
+    if (!isfinite(v) && !(MASKED && v == -INFINITY)) bad = true;
     mx = fmaxf(mx, v / temperature);
   }
   if (bad) atomicOr(err, IERT_ERR_NONFINITE_LOGIT);
   mx = block_max(mx, scratch);
 
   float local = 0.f;
-  for (int i = lo; i < hi; ++i) local += expf(row[i] / temperature - mx);
+  for (int i = lo; i < hi; ++i)
+    if (!MASKED || row[i] > -INFINITY) local += expf(row[i] / temperature - mx);
 
   // Boundaries: lower[t] = sum of the totals of threads before t (warp scan, then a scan
   // of the warp totals).  The owner of the draw is the LAST thread with a non-empty chunk
@@ -135,18 +139,23 @@ temperature_kernel(const float* __restrict__ logits, int vocab, long long ld, fl
 
   const float r = uniform_draw(seed, (uint32_t)request_ids[blockIdx.x], (uint32_t)step_ids[blockIdx.x]);
   const float target = r * total;
-  if (hi > lo && lower <= target) atomicMax(&owner, (int)threadIdx.x);
+  if (hi > lo && lower <= target && (!MASKED || local > 0.f)) atomicMax(&owner, (int)threadIdx.x);
   __syncthreads();
   if ((int)threadIdx.x == owner) {
     float cum = lower;
     int pick = hi - 1;
     for (int i = lo; i < hi; ++i) {
-      cum += expf(row[i] / temperature - mx);
+      const float e = MASKED && !(row[i] > -INFINITY) ? 0.f : expf(row[i] / temperature - mx);
+      if (MASKED && e > 0.f) pick = i;
+      cum += e;
       if (target < cum) { pick = i; break; }
     }
     out[blockIdx.x] = pick;
   }
-  if (threadIdx.x == 0 && owner < 0) out[blockIdx.x] = vocab - 1;
+  if (threadIdx.x == 0 && owner < 0) {
+    out[blockIdx.x] = MASKED ? 0 : vocab - 1;
+    if (MASKED) atomicOr(err, IERT_ERR_NOTHING_ALLOWED);
+  }
 }
 
 __global__ void uniform_kernel(uint64_t seed, const int* request_ids, const int* step_ids,
@@ -172,9 +181,18 @@ IERT_API int iert_sample_temperature(const float* logits, int rows, int vocab, l
                                      int* err, cudaStream_t stream) {
   if (rows <= 0) return IERT_OK;
   if (vocab <= 0 || !(temperature > 0.f) || !isfinite(temperature)) return IERT_BAD_ARGUMENT;
-  launch_dep(temperature_kernel, rows, THREADS, 0, stream, logits, vocab, ld, temperature, seed,
+  launch_dep(temperature_kernel<false>, rows, THREADS, 0, stream, logits, vocab, ld, temperature, seed,
                                                    request_ids, step_ids, out, err);
   return iert_check_launch("sample_temperature");
+}
+
+// The same with ids whose logit is -infinity ruled out.
+IERT_API int iert_sample_temperature_masked(const float* logits, int rows, int vocab, long long ld, float temperature, unsigned long long seed,
+                                            const int* request_ids, const int* step_ids, int* out, int* err, cudaStream_t stream) {
+  if (rows <= 0) return IERT_OK;
+  if (vocab <= 0 || !(temperature > 0.f) || !isfinite(temperature)) return IERT_BAD_ARGUMENT;
+  launch_dep(temperature_kernel<true>, rows, THREADS, 0, stream, logits, vocab, ld, temperature, seed, request_ids, step_ids, out, err);
+  return iert_check_launch("sample_temperature_masked");
 }
 
 // The draws themselves, for tests and for callers that want to sample elsewhere.
