@@ -162,6 +162,7 @@ def _declare(lib) -> None:
         "iert_history_append": [P, c_int, c_int, P, P, P, c_int, P, S],
         "iert_block_store": [P, c_int, POINTER(BatchView), POINTER(BlockView), P, S],
         "iert_block_attention_plain": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, P, S],
+        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, P, S],
         "iert_block_evict": [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int,
                              P, P, P, S],
         "iert_gemm_tc": [P, c_longlong, P, c_longlong, P, c_int, c_longlong, c_int, c_int, c_int, c_int,
@@ -1289,14 +1290,15 @@ def block_attention_scratch_floats(n_seqs: int, heads: int, view: BlockView) -> 
 
 
 def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,
-                    weight_out=None, plain: bool = False) -> None:
+                    weight_out=None, plain: bool = False, splits: int = 0) -> None:
     """One-token attention over the 8-bit cache, which the step's own key and value join; `out` [n_seqs, heads * head_dim] of the
     projection's type (rows of padding sequences: 0).
 
     rope         (inv_freq, rotary_dim, pairing, factor): the kernel rotates queries and the new key by the position, evicted ones included
     weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
                  sequences' own blocks are written
-    plain        the kernel that computes as the equations say
+    plain        the kernel that computes as the equations say (head sizes other than 64 and 128 always run it)
+    splits       CTAs that share a sequence's kv head: 1, 2, 4, 8, 16; 0: by the kernel's own rule
     """
     _packed_rows(qkv, heads, view)
     _need(batch.n_tokens == batch.n_seqs and qkv.shape[0] >= batch.n_seqs, "a one-token step has one row per sequence")
@@ -1310,8 +1312,12 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
         _need(scratch is not None and scratch.dtype == torch.float32 and
               scratch.numel() >= block_attention_scratch_floats(batch.n_seqs, heads, view), "scratch is too small")
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
-    check(core().iert_block_attention_plain(qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq),
-                                            rotary_dim, pairing, factor, err.data_ptr(), stream), "block_attention")
+    args = (qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq), rotary_dim, pairing, factor)
+    if not plain:
+        status = core().iert_block_attention_tc(*args, splits, err.data_ptr(), stream)
+        if status != 1:
+            return check(status, "block_attention")
+    check(core().iert_block_attention_plain(*args, err.data_ptr(), stream), "block_attention")
 
 
 def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, keep: int, recent: int, kept, err, stream, *, slots=None,

@@ -95,7 +95,7 @@ class Rig:
                 assert torch.equal(t[s, :, :n - done * BLOCK].double().cpu(), want.double()), (s, i)
         assert self.err.item() == 0
 
-    def step(self, slots, pad=0, weight_out=None, plain=True, scale=None, spread=1.0, check=True, scratch=None):
+    def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, scale=None, spread=1.0, check=True, scratch=None):
         """One token for each of `slots`; compares with 64 bits and returns the outputs."""
         b = B()
         scale = self.D ** -0.5 if scale is None else scale
@@ -108,7 +108,8 @@ class Rig:
         out = torch.full((len(slots) + pad + 1, self.H * self.D), 7.0, dtype=self.dtype, device=DEV)
         if scratch is None:
             scratch = torch.full((b.block_attention_scratch_floats(len(slots) + pad, self.H, self.view),), float("nan"), device=DEV)
-        b.block_attention(full, out, view, self.view, self.H, scale, scratch, self.err, b.stream_ptr(), weight_out=weight_out, plain=plain)
+        b.block_attention(full, out, view, self.view, self.H, scale, scratch, self.err, b.stream_ptr(), weight_out=weight_out, plain=plain,
+                          splits=splits)
         torch.cuda.synchronize()
         assert (out[-1] == 7).all(), "a row behind the last sequence was written"
         assert (out[len(slots):-1] == 0).all(), "padding sequences"
@@ -197,7 +198,7 @@ def test_blocks_of_zeros_and_of_extremes(fmt):
 LENS = [0, 1, 14, 15, 16, 17, 63, 64, 65, 127, 128, 200, 255]
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("G, H, D", [(1, 1, 64), (2, 8, 128), (8, 32, 128), (2, 24, 64), (1, 20, 128), (1, 5, 24), (3, 6, 48), (1, 2, 256)])
@@ -217,7 +218,24 @@ def test_one_token_steps(plain, fmt, dtype, G, H, D):
     assert torch.isnan(r.tail_k[other].float()).all()
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_key_head_shared_by_ctas(fmt, splits, D):
+    """Long and short sequences, more CTAs than blocks among them, more than 32 blocks for a warp."""
+    lens = [0, 5, 16, 40, 100, 1023, 2500, 16 * 32 * 4 * 2 + 17]
+    r = Rig(1, 5, D, fmt, torch.bfloat16, n_slots=8, width=66, weights=True, seed=splits)
+    slots = [3, 1, 0, 7, 2, 5, 6, 4]
+    live = [(s, x) for s, x in zip(slots, lens) if x]
+    r.store([s for s, _ in live], [x for _, x in live])
+    for s, x in live:
+        r.blocks_weight[s] = [torch.zeros(1, dtype=torch.float64) for _ in range(-(-x // BLOCK))]
+    for _ in range(2):
+        r.step(slots, plain=False, splits=splits)
+    r.check_content(slots)
+
+
+@pytest.mark.parametrize("plain", [True, False])
 @pytest.mark.parametrize("window, ring", [(1, 1), (16, 1), (17, 1), (64, 1), (65, 2), (100, 2), (128, 2), (1000, None)])
 @pytest.mark.parametrize("D", [64, 128, 40])
 def test_windows_and_rings(plain, window, ring, D):
@@ -230,7 +248,7 @@ def test_windows_and_rings(plain, window, ring, D):
     r.check_content([0, 1, 2, 3])
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_pages_of_other_sizes(plain):
     for pt in (16, 48, 128):
         r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=2, width=9, weights=True, page_tokens=pt, seed=pt)
@@ -241,7 +259,7 @@ def test_pages_of_other_sizes(plain):
         r.check_content([0, 1])
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_weights_elsewhere(plain):
     """Weights into another array: the view's own stay, and of the other only the sequences' blocks are written."""
     r = Rig(2, 4, 128, torch.int8, torch.bfloat16, n_slots=2, width=3, weights=True, seed=5)
@@ -259,7 +277,7 @@ def test_weights_elsewhere(plain):
                 assert (out[page, :, part] == 5).all()
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 @pytest.mark.parametrize("D", [128, 24])
 @pytest.mark.parametrize("pairing", [0, 1])
 def test_rotation_inside_the_kernel(plain, D, pairing):
@@ -291,7 +309,7 @@ def test_rotation_inside_the_kernel(plain, D, pairing):
     assert rs[0].err.item() == 0 and rs[1].err.item() == 0
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_bad_pages_and_slots_set_the_error_word(plain):
     b = B()
     r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=3, width=2, weights=True, seed=11)
@@ -322,7 +340,7 @@ def test_bad_pages_and_slots_set_the_error_word(plain):
     assert r.err.item() == b.ERR_PAGE_RANGE
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_what_is_not_a_number_stays_where_it_is_seen(plain):
     """A NaN among one sequence's values reaches that sequence's heads alone; positions outside a window reach nobody."""
     r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=3, width=3, window=30, seed=13)
@@ -339,7 +357,7 @@ def test_what_is_not_a_number_stays_where_it_is_seen(plain):
     assert clean is r.view
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_large_scores(plain):
     """Scores of several hundred: one position takes nearly all the weight; nothing overflows."""
     r = Rig(2, 8, 128, torch.int8, torch.float32, n_slots=2, width=4, weights=True, seed=14)
@@ -349,7 +367,7 @@ def test_large_scores(plain):
         r.step([0, 1], plain=plain, spread=spread)
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_on_another_stream_and_captured(plain):
     b = B()
     outs = []
@@ -382,7 +400,7 @@ def test_on_another_stream_and_captured(plain):
             assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(c.float()))
 
 
-@pytest.mark.parametrize("plain", [True])
+@pytest.mark.parametrize("plain", [True, False])
 def test_equal_calls_give_equal_bits(plain):
     """No sum depends on what runs when."""
     got = []
