@@ -7,6 +7,7 @@ to its next token for the Mistral / Llama-style dense decoder.
     ids = session.generate([[1, 5, 9], [1, 7]], max_new_tokens=16)
 """
 from .api import InferenceSession, LoadedModel, parse_dtype, write_random_model
+from .cache import EvictionPolicy
 from .config import (ConfigError, MistralConfig, ModelSpec, config_from_dict, known_architectures,
                      load_config, register_architecture, spec_of)
 from .engine import Engine, GenerationResult, Model, StepError
@@ -15,5 +16,5 @@ from .weights import WeightError
 
 __all__ = ["InferenceSession", "LoadedModel", "parse_dtype", "write_random_model", "ConfigError",
            "MistralConfig", "ModelSpec", "config_from_dict", "known_architectures", "load_config",
-           "register_architecture", "spec_of", "Engine", "GenerationResult", "Model", "StepError",
+           "register_architecture", "spec_of", "Engine", "EvictionPolicy", "GenerationResult", "Model", "StepError",
            "Sampler", "SamplingError", "SamplingParams", "WeightError"]

@@ -7,10 +7,11 @@ line (src/main.rs:97-116).
 from __future__ import annotations
 
 import os
-from typing import Iterable, List, Optional, Sequence, Union
+from typing import Callable, Iterable, List, Mapping, Optional, Sequence, Union
 
 import torch
 
+from .cache import EvictionPolicy
 from .config import ConfigError, config_from_dict, load_config, spec_of
 from .engine import Engine, GenerationResult, Model, generate as _generate
 from .parts.base import Runtime
@@ -90,14 +91,25 @@ class InferenceSession:
     max_tokens     positions the cache holds over all live sequences (each rounded up to 64)
     max_sequences  slots; default: as many as there are pages, at most 1024
     use_graphs     replay captured CUDA graphs for one-token steps and short prompts (default)
+    cache_dtype    None: keys and values in the run's type; "int8" or "float8_e4m3": in 8 bits with a scale per 16 positions and
+                   head (models whose mixers take it: the dense decoders), about half of bfloat16's bytes
+    evict_to       positions that a sequence goes back to when it has grown `evict_every` beyond (a multiple of 16, needs `cache_dtype`
+                   and layers without a window): of its finished blocks of 16 every layer and head keeps the last `evict_recent`
+                   positions' (default: a quarter) and those that the one-token steps gave the most attention.  A conversation may
+                   then grow to `max_seq_len` (default: the model's longest) in a cache that holds far fewer positions
     """
 
     def __init__(self, model: LoadedModel, max_tokens: int = 8192,
                  max_sequences: Optional[int] = None, max_seq_len: Optional[int] = None,
-                 poison_cache: bool = False, use_graphs: bool = True):
+                 poison_cache: bool = False, use_graphs: bool = True, cache_dtype=None,
+                 evict_to: Optional[int] = None, evict_recent: Optional[int] = None, evict_every: int = 64):
         self.loaded = model
+        if evict_to is None and evict_recent is not None:
+            raise ValueError("evict_recent needs evict_to")
+        eviction = None if evict_to is None else EvictionPolicy(evict_to, evict_recent, evict_every)
         self.engine = Engine(model.model, max_tokens=max_tokens, max_sequences=max_sequences,
-                             max_seq_len=max_seq_len, poison_cache=poison_cache, use_graphs=use_graphs)
+                             max_seq_len=max_seq_len, poison_cache=poison_cache, use_graphs=use_graphs,
+                             cache_dtype=cache_dtype, eviction=eviction)
         self.max_tokens = max_tokens
         self._slots: List[int] = []
 
@@ -164,23 +176,31 @@ class InferenceSession:
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 20,
                  temperature: float = 0.0, seed: int = 0, stop_ids: Optional[Iterable[int]] = None,
                  max_batch: Optional[int] = None, request_ids: Optional[Sequence[int]] = None,
-                 on_token=None, full: bool = False,
-                 run_ahead: bool = True) -> Union[List[List[int]], List[GenerationResult]]:
+                 on_token=None, full: bool = False, run_ahead: bool = True, repetition_penalty: float = 1.0,
+                 presence_penalty: float = 0.0, frequency_penalty: float = 0.0, logit_bias: Optional[Mapping[int, float]] = None,
+                 allowed_tokens: Optional[Callable[[int, List[int]], object]] = None) -> Union[List[List[int]], List[GenerationResult]]:
         """Generated token ids for every prompt (host lists in, host lists out).  Stop ids
         default to the configuration's EOS; the stop token is not part of the output.
         `run_ahead` (default): chosen ids feed the next step from device memory and reach the
-        host one step behind, so the device never waits for the host; results are the same."""
+        host one step behind, so the device never waits for the host; results are the same.
+
+        `repetition_penalty`, `presence_penalty`, `frequency_penalty` and `logit_bias` change the logits before each choice
+        (`SamplingParams`).  `allowed_tokens(request id, answer so far)` says which ids may come next: a sequence of ids, a boolean
+        array of the vocabulary, or None for all; it is asked on the host before every token, so nothing runs ahead."""
         if self._slots:
             raise RuntimeError("a batch started with prefill() is running; reset() first")
         spec = self.loaded.spec
         if stop_ids is None:
             stop_ids = [] if spec.eos_token_id is None else [spec.eos_token_id]
-        sampler = Sampler(SamplingParams(temperature=temperature, seed=seed), self.engine.rt.err)
+        sampler = Sampler(SamplingParams(temperature=temperature, seed=seed, repetition_penalty=repetition_penalty,
+                                         presence_penalty=presence_penalty, frequency_penalty=frequency_penalty,
+                                         logit_bias=logit_bias or ()), self.engine.rt.err)
         cache = self.engine.cache
+        evicts = {} if cache.eviction is None else {"most_held": cache.eviction.most_held, "capacity": cache.max_seq_len}
         res = _generate(self.engine, sampler, prompts, max_new_tokens, stop_ids=stop_ids,
                         max_tokens=cache.n_pages * cache.page_tokens, max_sequences=cache.n_slots,
-                        max_seq_len=cache.max_seq_len, page_tokens=cache.page_tokens,
+                        max_seq_len=self.engine.max_positions if evicts else cache.max_seq_len, page_tokens=cache.page_tokens,
                         max_batch=max_batch, request_ids=request_ids, on_token=on_token,
-                        run_ahead=run_ahead)
+                        run_ahead=run_ahead, allowed_tokens=allowed_tokens, **evicts)
         self.engine.check_device()
         return res if full else [r.tokens for r in res]

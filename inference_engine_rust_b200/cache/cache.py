@@ -21,6 +21,7 @@ import numpy as np
 import torch
 
 from .allocators import CacheError, CacheFull, IndexPool
+from .blocks import BLOCK_TOKENS, BlockStore, EvictionPolicy
 from .staging import PinnedRing
 
 PAGE_TOKENS = 64
@@ -56,10 +57,14 @@ CacheRequest = Union[KVRequest, StateRequest, None, Tuple]
 
 
 class KVGroup:
-    """Layers with the same key/value geometry and the same visibility share page tables."""
+    """Layers with the same key/value geometry and the same visibility share page tables.
+
+    `levels` (int8, float8_e4m3fn): keys and values stand in `blocks` (8 bits with scales) and `k`, `v` are None.  With `eviction`
+    the pool has pages of its own for a sequence's kept blocks on their way (`EvictionPolicy`)."""
 
     def __init__(self, req: KVRequest, layers: Sequence[int], n_pages: int, n_slots: int,
-                 max_seq_len: int, dtype: torch.dtype, device, page_tokens: int, poison: bool):
+                 max_seq_len: int, dtype: torch.dtype, device, page_tokens: int, poison: bool,
+                 levels: Optional[torch.dtype] = None, eviction: Optional[EvictionPolicy] = None):
         self.req = req
         self.layers = tuple(layers)
         self.page_tokens = page_tokens
@@ -77,13 +82,32 @@ class KVGroup:
             self.ring_pages = min(self.table_width, keep_pages + max(1, math.ceil(req.reach / page_tokens)))
             if self.ring_pages < self.table_width:
                 self.keep_pages = keep_pages
-        shape = (len(self.layers), n_pages, req.kv_heads, page_tokens, req.head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=device)
-        self.v = torch.empty(shape if req.values else (len(self.layers), 0) + shape[2:], dtype=dtype, device=device)
         self.poison = poison
-        if poison:
-            self.k.fill_(float("nan"))
-            self.v.fill_(float("nan"))
+        self.eviction = eviction
+        self.blocks: Optional[BlockStore] = None
+        if levels is not None:
+            if not req.values or req.chunk or req.keep:
+                raise ValueError("an 8-bit cache takes keys and values, all of a sequence or a window of them")
+            if eviction is not None:
+                if req.reach is not None:
+                    raise ValueError("eviction needs layers that see every earlier position (these have a window)")
+                self.kept_pages = math.ceil((eviction.keep + BLOCK_TOKENS) / page_tokens)
+                n_pages += self.kept_pages
+                self.n_pages = n_pages
+            self.k = self.v = None
+            self.blocks = BlockStore(len(self.layers), n_pages, n_slots, req.kv_heads, req.head_dim, page_tokens, levels, dtype, device,
+                                     weights=eviction is not None)
+            if poison:
+                self.blocks.poison()
+        else:
+            if eviction is not None:
+                raise ValueError("eviction needs an 8-bit cache")
+            shape = (len(self.layers), n_pages, req.kv_heads, page_tokens, req.head_dim)
+            self.k = torch.empty(shape, dtype=dtype, device=device)
+            self.v = torch.empty(shape if req.values else (len(self.layers), 0) + shape[2:], dtype=dtype, device=device)
+            if poison:
+                self.k.fill_(float("nan"))
+                self.v.fill_(float("nan"))
         self.pages = IndexPool(n_pages, "page")
         self.table_host = np.full((n_slots, self.table_width), -1, dtype=np.int32)
         self.table = torch.full((n_slots, self.table_width), -1, dtype=torch.int32, device=device)
@@ -100,6 +124,8 @@ class KVGroup:
 
     def open_slot(self, slot: int) -> None:
         self._pages_of[slot] = []
+        if self.eviction is not None:
+            self.blocks.shift[slot] = 0
 
     def ensure(self, slot: int, length: int) -> None:
         """Pages for positions [0, length) of `slot` (or for the ring, if shorter)."""
@@ -111,6 +137,9 @@ class KVGroup:
             raise CacheFull(f"sequence of {length} tokens exceeds the cache's longest sequence "
                             f"({self.table_width * self.page_tokens})")
         if need > len(have):
+            if self.eviction is not None and need - len(have) > self.pages.free_count - self.kept_pages:
+                raise CacheFull(f"{need - len(have)} pages wanted, {max(0, self.pages.free_count - self.kept_pages)} of "
+                                f"{self.n_pages - self.kept_pages} free")        # the rest is for an eviction's copies
             new = self.pages.alloc_many(need - len(have))
             for p in new:
                 self.table_host[slot, len(have)] = p
@@ -120,13 +149,51 @@ class KVGroup:
     def close_slot(self, slot: int) -> None:
         pages = self._pages_of.pop(slot)
         self.pages.free_many(pages)
-        if self.poison and pages:
-            idx = torch.tensor(pages, dtype=torch.long, device=self.device)
-            self.k[:, idx] = float("nan")
-            if self.req.values:
-                self.v[:, idx] = float("nan")
+        self._poison(pages)
         self.table_host[slot, :] = -1
         self._dirty.add(slot)
+
+    def _poison(self, pages: Sequence[int]) -> None:
+        if not self.poison or not pages:
+            return
+        idx = torch.tensor(list(pages), dtype=torch.long, device=self.device)
+        if self.blocks is not None:
+            self.blocks.poison(idx)
+            return
+        self.k[:, idx] = float("nan")
+        if self.req.values:
+            self.v[:, idx] = float("nan")
+
+    def evict(self, slots: Sequence[int], held: Sequence[int], err) -> List[int]:
+        """These sequences go back to the policy's `keep` positions of finished blocks (and what is unfinished); returns the positions
+        that each loses.  The device's page table must be up to date.  Sequences that share a launch need pages for all their kept
+        blocks at once; where the pool has no more they go one after another."""
+        if self.eviction is None:
+            raise CacheError("the cache was made without an eviction policy")
+        if len(set(slots)) != len(slots):
+            raise CacheError("a slot appears twice in one eviction")
+        keep, recent = self.eviction.keep // BLOCK_TOKENS, self.eviction.recent // BLOCK_TOKENS
+        lost = [max(0, n // BLOCK_TOKENS - keep) * BLOCK_TOKENS for n in held]
+        todo = [i for i, n in enumerate(lost) if n]
+        while todo:
+            at_once = min(len(todo), self.pages.free_count // self.kept_pages)
+            if at_once == 0:
+                raise CacheFull(f"{self.kept_pages} pages wanted for the blocks that a sequence keeps, {self.pages.free_count} free")
+            now, todo = todo[:at_once], todo[at_once:]
+            new = [self.pages.alloc_many(self.kept_pages) for _ in now]
+            self.blocks.evict(self.table, [slots[i] for i in now], [held[i] for i in now], np.asarray(new, dtype=np.int32), keep, recent, err)
+            for i, pages in zip(now, new):
+                slot = slots[i]
+                used = self.pages_needed(held[i] - lost[i])       # the rest of the new pages was room for a block that has not begun
+                old = self._pages_of[slot]
+                self.pages.free_many(old)
+                self.pages.free_many(pages[used:])
+                self._poison(old + pages[used:])
+                self._pages_of[slot] = pages[:used]
+                self.table_host[slot, :] = -1
+                self.table_host[slot, :used] = pages[:used]
+                self._dirty.add(slot)
+        return lost
 
     def upload(self, wait: bool = True) -> None:
         """Bring the device page table up to date (rows of slots that changed).  `wait`: the copies have ended on return; else they
@@ -159,7 +226,9 @@ class KVGroup:
     def pages_of(self, slot: int) -> List[int]:
         return list(self._pages_of[slot])
 
-    def bytes_per_token(self) -> int:
+    def bytes_per_token(self) -> float:
+        if self.blocks is not None:
+            return self.blocks.bytes_per_token()
         return (2 if self.req.values else 1) * len(self.layers) * self.req.kv_heads * self.req.head_dim * self.k.element_size()
 
 
@@ -182,6 +251,7 @@ class KVLayerView:
     group: KVGroup
     index: int                     # position of the layer inside the group
     struct: object                 # csrc.bindings.KvView, or None on a CPU-only cache
+    blocks: object = None          # csrc.bindings.BlockView where the group is held in 8 bits (`struct` then gives the geometry only)
 
     @property
     def k(self) -> torch.Tensor:
@@ -209,11 +279,13 @@ class Cache:
                    rounded up to `page_tokens`
     max_seq_len    the longest single sequence (width of a page table)
     max_sequences  number of slots
+    levels         keys and values in 8 bits: torch.int8 or torch.float8_e4m3fn (None: in `dtype`)
+    eviction       a policy by which long sequences go back to a bounded number of positions (needs `levels`)
     """
 
     def __init__(self, requests: Mapping[int, CacheRequest], *, max_tokens: int, max_seq_len: int,
                  max_sequences: int, dtype: torch.dtype, device, page_tokens: int = PAGE_TOKENS,
-                 poison: bool = False):
+                 poison: bool = False, levels: Optional[torch.dtype] = None, eviction: Optional[EvictionPolicy] = None):
         if max_tokens <= 0 or max_seq_len <= 0 or max_sequences <= 0:
             raise ValueError("cache sizes must be positive")
         self.page_tokens = page_tokens
@@ -224,6 +296,9 @@ class Cache:
         self.device = torch.device(device)
         self.slots = IndexPool(self.n_slots, "slot")
         self.seq_lens = np.zeros(self.n_slots, dtype=np.int64)
+        self.eviction = eviction
+        self.lost = np.zeros(self.n_slots, dtype=np.int64)            # positions each sequence has lost to eviction
+        self.steps_since = np.zeros(self.n_slots, dtype=np.int64)     # one-token steps since it last lost any (or began)
 
         kv_by_key: Dict[KVRequest, List[int]] = {}
         st_by_key: Dict[StateRequest, List[int]] = {}
@@ -246,13 +321,16 @@ class Cache:
                     raise TypeError(f"layer {layer}: unknown cache request {r!r}")
         self.kv_groups: List[KVGroup] = [
             KVGroup(req, layers, self.n_pages, self.n_slots, self.max_seq_len, dtype, self.device,
-                    page_tokens, poison) for req, layers in kv_by_key.items()]
+                    page_tokens, poison, levels=levels, eviction=eviction) for req, layers in kv_by_key.items()]
         self.state_groups: List[StateGroup] = [
             StateGroup(req, layers, self.n_slots, self.device) for req, layers in st_by_key.items()]
         self._views: Dict[int, object] = {}
         for g in self.kv_groups:
             for i, layer in enumerate(g.layers):
-                self._views[layer] = KVLayerView(g, i, self._kv_struct(g, i))
+                blocks = None
+                if g.blocks is not None and self.device.type == "cuda":
+                    blocks = g.blocks.view(i, g.table, g.req.window or 0, g.ring_pages)
+                self._views[layer] = KVLayerView(g, i, self._kv_struct(g, i), blocks)
         for g in self.state_groups:
             for i, layer in enumerate(g.layers):
                 self._views[layer] = StateLayerView(g, i)
@@ -263,7 +341,8 @@ class Cache:
         if self.device.type != "cuda":
             return None
         from ..csrc import bindings as B
-        return B.KvView(k=g.k[i].data_ptr(), v=g.v[i].data_ptr() if g.req.values else None, page_table=g.table.data_ptr(),
+        return B.KvView(k=g.k[i].data_ptr() if g.k is not None else None,
+                        v=g.v[i].data_ptr() if g.req.values and g.v is not None else None, page_table=g.table.data_ptr(),
                         table_width=g.table_width, ring_pages=g.ring_pages, page_tokens=g.page_tokens,
                         n_pages=g.n_pages, kv_heads=g.req.kv_heads, head_dim=g.req.head_dim,
                         dtype=B.dtype_code(g.dtype), window=g.req.window or 0, chunk=g.req.chunk or 0,
@@ -272,7 +351,7 @@ class Cache:
     # ---- slots ------------------------------------------------------------------------
     def open_sequence(self) -> int:
         slot = self.slots.alloc()
-        self.seq_lens[slot] = 0
+        self.seq_lens[slot] = self.lost[slot] = self.steps_since[slot] = 0
         for g in self.kv_groups:
             g.open_slot(slot)
         for g in self.state_groups:
@@ -285,7 +364,7 @@ class Cache:
             g.close_slot(slot)
         for g in self.state_groups:
             g.close_slot(slot)
-        self.seq_lens[slot] = 0
+        self.seq_lens[slot] = self.lost[slot] = 0
 
     def length(self, slot: int) -> int:
         if slot not in self.slots._held:
@@ -304,6 +383,19 @@ class Cache:
 
     def advance(self, slot: int, n_tokens: int) -> None:
         self.seq_lens[slot] += n_tokens
+
+    def evict(self, slots: Sequence[int], err) -> None:
+        """Those of these sequences that the eviction policy says go back to what it keeps, in every layer; in the current stream's order."""
+        due = [s for s in slots if self.eviction.due(int(self.seq_lens[s]), int(self.steps_since[s]))]
+        if not due:
+            return
+        self.upload(wait=False)
+        for g in self.kv_groups:
+            lost = g.evict(due, [int(self.seq_lens[s]) for s in due], err)
+        for s, n in zip(due, lost):
+            self.seq_lens[s] -= n
+            self.lost[s] += n
+            self.steps_since[s] = 0
 
     def upload(self, wait: bool = True) -> None:
         """`KVGroup.upload` of every group."""
@@ -327,7 +419,7 @@ class Cache:
                 n = int(self.seq_lens[s])
                 if g.req.reach is not None:
                     n = min(n, g.req.reach + g.req.keep)
-                total += n * g.bytes_per_token()
+                total += int(n * g.bytes_per_token())
         return total
 
     def check(self) -> None:

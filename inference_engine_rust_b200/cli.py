@@ -161,6 +161,19 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("-n", "--new-tokens", type=int, default=20, help="how many new tokens to append after the prompt")
     ap.add_argument("--temperature", type=float, default=0.0, help="0 = greedy; > 0 = temperature sampling")
     ap.add_argument("--seed", type=int, default=0, help="seed of the sampling draws (and of --random weights)")
+    ap.add_argument("--repetition-penalty", type=float, default=1.0,
+                    help="divides the logits of ids seen in prompt or answer where positive, multiplies them where not (1 = off)")
+    ap.add_argument("--presence-penalty", type=float, default=0.0, help="taken from the logits of ids that the answer has")
+    ap.add_argument("--frequency-penalty", type=float, default=0.0, help="taken from an id's logit for each time that the answer has it")
+    ap.add_argument("--logit-bias", action="append", default=None, metavar="ID:BIAS",
+                    help="added to an id's logit (repeatable; -inf = never choose it)")
+    ap.add_argument("--cache-dtype", choices=["int8", "float8_e4m3"], default=None,
+                    help="keys and values in 8 bits with a scale per 16 positions and head (default: the run's type)")
+    ap.add_argument("--evict-to", type=int, default=None, metavar="N",
+                    help="sequences go back to N positions (a multiple of 16), those that got the most attention; needs --cache-dtype")
+    ap.add_argument("--evict-recent", type=int, default=None, metavar="N",
+                    help="how many of them are the newest (a multiple of 16; default: a quarter)")
+    ap.add_argument("--evict-every", type=int, default=64, metavar="N", help="one-token steps between two evictions of a sequence")
     ap.add_argument("--stop-token", type=int, action="append", default=None,
                     help="stop id (repeatable); default: the configuration's EOS; a negative id = never stop")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "bf16", "float32", "fp32"])
@@ -215,6 +228,24 @@ def main(argv: Optional[List[str]] = None) -> int:
     if a.new_tokens < 0:
         print("error: --new-tokens must be >= 0", file=sys.stderr)
         return 2
+    from .cache import EvictionPolicy
+    from .sampling import SamplingError, SamplingParams
+    try:
+        bias = {}
+        for text in a.logit_bias or []:
+            i, _, b = text.partition(":")
+            bias[int(i)] = float(b)
+        rules = dict(repetition_penalty=a.repetition_penalty, presence_penalty=a.presence_penalty, frequency_penalty=a.frequency_penalty,
+                     logit_bias=bias)
+        SamplingParams(temperature=a.temperature, seed=a.seed, **rules)
+        if a.evict_to is None and a.evict_recent is not None:
+            raise ValueError("--evict-recent needs --evict-to")
+        if a.evict_to is not None and a.cache_dtype is None:
+            raise ValueError("--evict-to needs --cache-dtype")
+        policy = None if a.evict_to is None else EvictionPolicy(a.evict_to, a.evict_recent, a.evict_every)
+    except (SamplingError, ValueError) as e:
+        print(f"error: {e}", file=sys.stderr)
+        return 2
 
     from .api import LoadedModel
     from .weights import WeightError
@@ -238,12 +269,18 @@ def main(argv: Optional[List[str]] = None) -> int:
         return 2
     # room for every request at its longest, each rounded up to a page, unless told otherwise
     from .cache import PAGE_TOKENS
-    need = sum(-(-min(len(r) + a.new_tokens, limit) // PAGE_TOKENS) * PAGE_TOKENS for r in requests)
-    session = model.session(max_tokens=a.max_tokens or need, max_seq_len=limit)
+    holds = [min(len(r) + a.new_tokens, limit) if policy is None else min(len(r) + a.new_tokens, limit, policy.most_held(len(r))) for r in requests]
+    need = sum(-(-n // PAGE_TOKENS) * PAGE_TOKENS for n in holds)
+    try:
+        session = model.session(max_tokens=a.max_tokens or need, max_seq_len=limit, cache_dtype=a.cache_dtype, evict_to=a.evict_to,
+                                evict_recent=a.evict_recent, evict_every=a.evict_every)
+    except ValueError as e:                      # a model that does not run over such a cache
+        print(f"error: {e}", file=sys.stderr)
+        return 1
     stop = None if a.stop_token is None else [s for s in a.stop_token if s >= 0]
     try:
         outs = session.generate(requests, max_new_tokens=a.new_tokens, temperature=a.temperature, seed=a.seed,
-                                stop_ids=stop, max_batch=a.max_batch)
+                                stop_ids=stop, max_batch=a.max_batch, **rules)
     except ValueError as e:                      # a request that cannot fit, an id outside the vocabulary
         print(f"error: {e}", file=sys.stderr)
         return 1

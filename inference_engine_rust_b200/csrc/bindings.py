@@ -162,7 +162,7 @@ def _declare(lib) -> None:
         "iert_history_append": [P, c_int, c_int, P, P, P, c_int, P, S],
         "iert_block_store": [P, c_int, POINTER(BatchView), POINTER(BlockView), P, S],
         "iert_block_attention_plain": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, P, S],
-        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, P, S],
+        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, c_int, P, S],
         "iert_block_evict": [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int,
                              P, P, P, S],
         "iert_gemm_tc": [P, c_longlong, P, c_longlong, P, c_int, c_longlong, c_int, c_int, c_int, c_int,
@@ -219,6 +219,8 @@ def _declare(lib) -> None:
         "iert_rglru_gates": [P, P, P, P, P, c_int, P, c_float, P, P, c_int, c_int, c_int, S],
         "iert_rglru_scan": [P, P, P, LL, P, P, P, LL, P, c_int, c_float, c_int, c_int, c_int, P, POINTER(BatchView), S],
     })
+    lib.iert_block_attention_scratch.argtypes = [c_int, c_int, POINTER(BlockView)]
+    lib.iert_block_attention_scratch.restype = c_longlong
     lib.iert_attention_decode.argtypes = [P, P, POINTER(BatchView), POINTER(KvView), c_int, c_float, c_int, P, P, S]
     lib.iert_attention_decode.restype = c_int
     lib.iert_attention_decode_scratch_floats.argtypes = [c_int, c_int, c_int, c_int]
@@ -1286,11 +1288,11 @@ def block_store(qkv, batch: BatchView, view: BlockView, heads: int, err, stream)
 
 def block_attention_scratch_floats(n_seqs: int, heads: int, view: BlockView) -> int:
     """Floats of scratch that `block_attention` needs for steps of up to `n_seqs` sequences."""
-    return n_seqs * heads * view.table_width * (view.page_tokens // BLOCK_TOKENS) if view.weight else 1
+    return core().iert_block_attention_scratch(n_seqs, heads, byref(view))
 
 
 def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,
-                    weight_out=None, plain: bool = False, splits: int = 0) -> None:
+                    weight_out=None, plain: bool = False, splits: int = 0, warps: int = 0) -> None:
     """One-token attention over the 8-bit cache, which the step's own key and value join; `out` [n_seqs, heads * head_dim] of the
     projection's type (rows of padding sequences: 0).
 
@@ -1298,23 +1300,21 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
                  sequences' own blocks are written
     plain        the kernel that computes as the equations say (head sizes other than 64 and 128 always run it)
-    splits       CTAs that share a sequence's kv head: 1, 2, 4, 8, 16; 0: by the kernel's own rule
+    splits       CTAs that share a sequence's kv head (1, 2, 4, 8, 16), of `warps` (4, 8, 16) each; 0: by the kernel's own rule
     """
     _packed_rows(qkv, heads, view)
     _need(batch.n_tokens == batch.n_seqs and qkv.shape[0] >= batch.n_seqs, "a one-token step has one row per sequence")
     _need(heads % view.kv_heads == 0, f"heads {heads} is not a multiple of kv_heads {view.kv_heads}")
     _need(out.dtype == qkv.dtype and out.is_contiguous() and out.numel() >= batch.n_seqs * heads * view.head_dim, "out must be [sequences, heads * head_dim]")
-    weights = weight_out.data_ptr() if weight_out is not None else view.weight
-    _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
+    _need(scratch.dtype == torch.float32 and scratch.numel() >= block_attention_scratch_floats(batch.n_seqs, heads, view), "scratch is too small")
     _need(weight_out is None or (view.weight is not None and weight_out.dtype == torch.float32 and weight_out.is_contiguous()
                                  and weight_out.shape == view.tensors[7].shape), "weight_out must be laid out as the view's weight")
-    if view.weight:
-        _need(scratch is not None and scratch.dtype == torch.float32 and
-              scratch.numel() >= block_attention_scratch_floats(batch.n_seqs, heads, view), "scratch is too small")
+    _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
+    weights = weight_out.data_ptr() if weight_out is not None else view.weight
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
     args = (qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq), rotary_dim, pairing, factor)
     if not plain:
-        status = core().iert_block_attention_tc(*args, splits, err.data_ptr(), stream)
+        status = core().iert_block_attention_tc(*args, splits, warps, err.data_ptr(), stream)
         if status != 1:
             return check(status, "block_attention")
     check(core().iert_block_attention_plain(*args, err.data_ptr(), stream), "block_attention")

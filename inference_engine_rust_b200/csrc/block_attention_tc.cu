@@ -1,20 +1,23 @@
 // One-token attention over the 8-bit cache (block_cache.cuh) on the tensor cores, head sizes 64 and 128.
 //
 // The sequences' keys and values in 8 bits are all that has to come from memory, so everything is arranged around that stream:
-//   * A cluster of up to 16 CTAs shares one (sequence, kv head): each takes a run of its blocks, and their partial results meet in
-//     one another's shared memory.  One launch, no scratch memory for partial outputs, no second kernel.
+//   * A cluster of up to 16 CTAs shares one (sequence, kv head): each takes a run of its blocks, and each adds up a share of the
+//     outputs from what the others have put into its shared memory.  One launch, no scratch memory for partial outputs.
 //   * A warp owns a block (16 positions) at a time, with a ring of its own that cp.async fills: no barrier inside the loop.
 //   * Levels become fp16 in registers, exactly (int8: 1024 + (q + 128) by a byte permutation, minus 1152; e4m3: a conversion
-//     instruction), and are operands of mma.m16n8k16 with fp32 sums.  The tile's 16 rows are 8 query heads twice: rows 0-7 the upper
-//     11 bits of a query (scaled by a power of two of its row), rows 8-15 the next 11.  Products with a row's both halves are
-//     exact to 2^-22, so float32 runs and bfloat16 runs take the same kernel, and weights (which eviction adds up) are as good as fp32.
-//     Probabilities go into the second product the same way.  A bf16 group of up to 8 heads leaves half a tile empty anyway.
+//     instruction), and are the 16-row operand of mma.m16n8k16: S^T = K Q^T has 16 positions x 8 heads, O^T = V^T P^T 16 dimensions x 8
+//     heads, so that a group of up to 8 query heads fills the narrow side.  Queries are scaled by a power of two of their row; bf16
+//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`), and probabilities likewise.
 //   * The order of dimensions inside a product is free as long as both operands agree: a lane takes 16 neighbouring bytes of a key
-//     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.
-//   * A block's key scale multiplies its scores, its value scale the 16-position partial product: no level is ever multiplied.
-// The unfinished block, fewer than 17 rows in the run's type, is done in fp32 by the last CTA of the cluster, which also stores
+//     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.  P^T gets into operand form by
+//     two 8 x 8 transpositions in registers (movmatrix).
+//   * A block's key scale multiplies its scores, its value scale (relative to the largest met so far) its probabilities: no level is
+//     ever multiplied.  The softmax reference moves only where a score passes it by 2^15, so a block costs no maximum across lanes.
+// The unfinished block, up to 16 rows in the run's type, is done in fp32 by the last CTA of the cluster, which also stores
 // the step's own key and value and turns the block into levels when it is full.
 #include <cooperative_groups.h>
+
+#include <utility>
 
 #include "block_cache.cuh"
 
@@ -23,13 +26,15 @@ using namespace iert;
 
 namespace {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, NSTAGE = 3, GH = 8;
-constexpr float P_SHIFT = 14.f;           // probabilities are at most 2^14 in the second product: fp16 keeps what is 2^-38 of the largest
+constexpr int NSTAGE = 2, GH = 8, MAX_SPLITS = 16, WARPS_PER_SM = 16;
+constexpr float HEADROOM = 15.f;          // probabilities stay below 2^15 (fp16's largest is just under 2^16)
+constexpr float BELOW = 4.f;              // where the reference moves it goes to 2^-4 of the largest: scores may grow 2^11-fold before the next time
+constexpr int TAIL_BLOCKS = 8;            // finished blocks that cost a CTA about as much time as the unfinished one
 
 struct BlockTcParams {
   const void* qkv;
   void* out;
-  float* part;                 // [T][heads][blocks]: base-2 logarithm of a block's unnormalised weight
+  float* part;                 // [T][kv_heads][slices of 8 heads][blocks][8]: base-2 logarithm of a block's unnormalised weight
   float* weight_out;
   int heads, blocks;
   float scale_log2e;
@@ -65,13 +70,24 @@ template <int FMT> __device__ __forceinline__ void levels4(uint32_t w, uint32_t&
   }
 }
 
-// Two numbers as the upper 11 bits of each and what is left of them, in fp16.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+__device__ __forceinline__ uint32_t half2_bits(float x, float y) {
   const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = *reinterpret_cast<const uint32_t*>(&l);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// What is left of two numbers when their fp16 roundings are taken away.
+__device__ __forceinline__ uint32_t rest_bits(float x, float y, uint32_t hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  return half2_bits(x - f.x, y - f.y);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // 16-byte chunk `c` of a block's keys (values) in shared memory, moved inside its 128-byte line so that the loads of a warp, which take
@@ -79,27 +95,43 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 template <int HD> __device__ __forceinline__ int k_chunk(int c) { return HD == 128 ? c ^ (((c >> 3) & 1) << 2) : c; }
 template <int HD> __device__ __forceinline__ int v_chunk(int c) { return HD == 128 ? c ^ (((c >> 4) & 3) << 1) : c ^ (((c >> 3) & 3) << 1); }
 
-template <int HD, typename T> struct Shared {
-  static constexpr int QS = HD + 4;               // row stride of the queries
-  uint8_t ring[WARPS][NSTAGE][2][BLK * HD];        // (later each warp's partial output, [GH][HD] fp32, in its own first stages)
+template <int HD, typename T, int WARPS> struct Shared {
+  uint8_t ring[WARPS][NSTAGE][2][BLK * HD];        // (later each warp's partial output, [GH][HD] fp32, in its own ring)
   T tail[2][BLK][HD];
-  float q[GH][QS];
+  float q[GH][HD + 4];
   float cs[HD];
   float tail_s[BLK][GH];
   float tail_o[GH][HD];
-  float ml[WARPS + 1][GH][2];
-  float o[GH][HD];                                 // the CTA's result: read by the whole cluster
-  float oml[GH][2];
+  float ml[WARPS + 1][GH][2];                      // maximum and sum of each warp, and of the unfinished block
+  float o_in[GH * HD + MAX_SPLITS];                // this CTA's share of the outputs, from every CTA of the cluster
+  float ml_in[MAX_SPLITS][GH][2];
+  float wfac[WARPS + 1][GH];                       // what each warp's sums count for in the CTA's
+  float fac[MAX_SPLITS][GH];                       // what each CTA's sums count for in the outputs
   float lse[GH][2];                                // over the cluster: maximum, 1 / sum
   uint32_t red[WARPS];
 };
 
-template <int HD, int FMT, typename T>
-__global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcParams p, IertBatchView b, IertBlockView c) {
+// Element d of a head in fp32, rotated (and then rounded to the run's type, as rotated numbers are everywhere) if the kernel has to.
+template <typename T>
+__device__ __forceinline__ float head_value(const T* src, int d, const BlockTcParams& p, const float* cs) {
+  const float x = to_f32(src[d]);
+  if (!p.rope || d >= p.rotary_dim) return x;
+  const int half = p.rotary_dim / 2;
+  const bool second = p.pairing == IERT_PAIR_HALF ? d >= half : d & 1;
+  const int k = p.pairing == IERT_PAIR_HALF ? (second ? d - half : d) : d >> 1;
+  const float y = to_f32(src[p.pairing == IERT_PAIR_HALF ? (second ? d - half : d + half) : d ^ 1]);
+  return to_f32(from_f32<T>(second ? y * cs[half + k] + x * cs[k] : x * cs[k] - y * cs[half + k]));
+}
+
+template <int HD, int FMT, typename T, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, WARPS_PER_SM / WARPS) block_attention_tc_kernel(BlockTcParams p, IertBatchView b, IertBlockView c) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  using Sh = Shared<HD, T>;
+  using Sh = Shared<HD, T, WARPS>;
+  constexpr int THREADS = WARPS * 32;
   static_assert(NSTAGE * 2 * BLK >= GH * 4, "a warp's partial output fits in its ring");
+  static_assert(THREADS >= MAX_SPLITS * GH && THREADS >= BLK * GH, "a thread per (CTA, head) and per (row, head)");
   Sh& sm = *reinterpret_cast<Sh*>(smem_raw);
+  constexpr bool LO = sizeof(T) == 4;              // both halves of queries and probabilities
   constexpr int KSTEPS = HD / 16, DPL = HD / 8;    // dimensions of a value row that a lane group takes
   cg::cluster_group cluster = cg::this_cluster();
   const int S = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's first axis
@@ -116,32 +148,33 @@ __global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcP
       for (int i = tid; i < group * HD; i += THREADS) out[i] = from_f32<T>(0.f);
     return;
   }
+  cg::cluster_group::arrival_token started = cluster.barrier_arrive();
   const int pos = b.pos0[s], nb = pos / BLK, base = nb * BLK, per_page = c.page_tokens / BLK;
   const int j_min = iert_first_visible(pos, c.window, 0), b_lo = min(j_min / BLK, nb);
-  const int per = (nb - b_lo + S - 1) / S;
+  const int per = (nb - b_lo + (S > 1 ? TAIL_BLOCKS : 0) + S - 1) / S;
   const int lo = min(nb, b_lo + rank * per), hi = min(nb, lo + per);
   const int n_mine = max(0, (hi - lo - warp + WARPS - 1) / WARPS);        // blocks lo + warp, lo + warp + WARPS, ...
   const bool owner = rank == S - 1;                // of the unfinished block
   const T* row = (const T*)p.qkv + (size_t)t * (size_t)(p.heads + 2 * c.kv_heads) * HD;
 
-  // Page and scales of 32 of the warp's blocks at a time, one per lane.
-  int at = -1, at_next = -1;
-  float ks = 0.f, vs = 0.f, ks_next = 0.f, vs_next = 0.f;
-  auto look_up = [&](int i0, int& a, float& k, float& v) {
+  // Page and scales of 32 of the warp's blocks at a time, one per lane; the groups of even number stand in at[0], the odd ones in at[1].
+  int at[2] = {-1, -1};
+  float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
+  auto look_up = [&](int i0, int w) {
     const int x = lo + warp + WARPS * (i0 + lane);
-    a = -1; k = 0.f; v = 0.f;
+    at[w] = -1; ks[w] = 0.f; vs[w] = 0.f;
     if (i0 + lane < n_mine) {
       const int page = block_page(c, slot, x / per_page, p.err);
       if (page >= 0) {
-        a = (page * c.kv_heads + kvh) * per_page + x % per_page;
-        k = c.k_scale[a];
-        v = c.v_scale[a];
+        at[w] = (page * c.kv_heads + kvh) * per_page + x % per_page;
+        ks[w] = c.k_scale[at[w]];
+        vs[w] = c.v_scale[at[w]];
       }
     }
   };
-  auto issue = [&](int i) {                        // (i & 31 of the group that `at` or `at_next` holds)
+  auto issue = [&](int i) {
     if (i < n_mine) {
-      const int a = __shfl_sync(0xffffffffu, ((i >> 5) & 1) == 0 ? at : at_next, i & 31);
+      const int a = __shfl_sync(0xffffffffu, (i >> 5) & 1 ? at[1] : at[0], i & 31);
       if (a >= 0) {
         uint8_t *kd = sm.ring[warp][i % NSTAGE][0], *vd = sm.ring[warp][i % NSTAGE][1];
         const uint8_t *kq = (const uint8_t*)c.k + (size_t)a * (BLK * HD), *vq = (const uint8_t*)c.v + (size_t)a * (BLK * HD);
@@ -157,12 +190,13 @@ __global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcP
 
   for (int g0 = 0; g0 < group; g0 += GH) {
     const int n_g = min(GH, group - g0), head0 = kvh * group + g0;
-    look_up(0, at, ks, vs);
-    look_up(32, at_next, ks_next, vs_next);
+    float* part = c.weight ? p.part + (((size_t)t * c.kv_heads + kvh) * ((group + GH - 1) / GH) + g0 / GH) * p.blocks * GH : nullptr;
+    look_up(0, 0);
+    look_up(32, 1);
 #pragma unroll
     for (int i = 0; i < NSTAGE - 1; ++i) issue(i);
 
-    // ---- queries (and, with the unfinished block's owner, its rows), rotated if the kernel has to
+    // ---- queries and, with the unfinished block's owner, its rows
     if (g0 == 0) {
       if (p.rope) {
         const float where = (float)(pos + (c.shift ? c.shift[slot] : 0));
@@ -178,20 +212,16 @@ __global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcP
         const size_t off = ((size_t)slot * c.kv_heads + kvh) * BLK * HD;
         T *tk = (T*)c.tail_k + off, *tv = (T*)c.tail_v + off;
         const int old = (pos - base) * HD;
-        for (int i = tid; i < old; i += THREADS) { (&sm.tail[0][0][0])[i] = tk[i]; (&sm.tail[1][0][0])[i] = tv[i]; }
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll 4
+        for (int i = tid * V; i < old; i += THREADS * V) {
+          const uint4 x = *reinterpret_cast<const uint4*>(tk + i), y = *reinterpret_cast<const uint4*>(tv + i);
+          *reinterpret_cast<uint4*>(&sm.tail[0][0][0] + i) = x;
+          *reinterpret_cast<uint4*>(&sm.tail[1][0][0] + i) = y;
+        }
         const T *kn = row + (size_t)(p.heads + kvh) * HD, *vn = row + (size_t)(p.heads + c.kv_heads + kvh) * HD;
         for (int d = tid; d < HD; d += THREADS) {
-          T x = kn[d];
-          if (p.rope) {
-            const int half = p.rotary_dim / 2;
-            const bool second = p.pairing == IERT_PAIR_HALF ? d >= half : d & 1;
-            if (d < p.rotary_dim) {
-              const int k = p.pairing == IERT_PAIR_HALF ? (second ? d - half : d) : d >> 1;
-              const float y = to_f32(kn[p.pairing == IERT_PAIR_HALF ? (second ? d - half : d + half) : d ^ 1]), f = to_f32(x);
-              x = from_f32<T>(second ? y * sm.cs[half + k] + f * sm.cs[k] : f * sm.cs[k] - y * sm.cs[half + k]);
-            }
-          }
-          const T v = vn[d];
+          const T x = from_f32<T>(head_value(kn, d, p, sm.cs)), v = vn[d];
           sm.tail[0][pos - base][d] = x;
           sm.tail[1][pos - base][d] = v;
           tk[old + d] = x;
@@ -199,266 +229,291 @@ __global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcP
         }
       }
     }
-    for (int i = tid; i < GH * HD; i += THREADS) {
-      const int r = i / HD, d = i % HD;
-      float x = 0.f;
-      if (r < n_g) {
-        const T* q = row + (size_t)(head0 + r) * HD;
-        x = to_f32(q[d]);
-        if (p.rope && d < p.rotary_dim) {
-          const int half = p.rotary_dim / 2;
-          const bool second = p.pairing == IERT_PAIR_HALF ? d >= half : d & 1;
-          const int k = p.pairing == IERT_PAIR_HALF ? (second ? d - half : d) : d >> 1;
-          const float y = to_f32(q[p.pairing == IERT_PAIR_HALF ? (second ? d - half : d + half) : d ^ 1]);
-          x = second ? y * sm.cs[half + k] + x * sm.cs[k] : x * sm.cs[k] - y * sm.cs[half + k];
-        }
-      }
-      sm.q[r][d] = x;
+#pragma unroll
+    for (int i = 0; i < GH * HD / THREADS; ++i) {
+      const int r = (tid + i * THREADS) / HD, d = (tid + i * THREADS) % HD;
+      sm.q[r][d] = r < n_g ? head_value(row + (size_t)(head0 + r) * HD, d, p, sm.cs) : 0.f;
     }
     __syncthreads();
 
-    // ---- query fragments: row g (head g), scaled by a power of two to [1, 4), in two halves
-    float row_scale;
-    uint32_t qf[KSTEPS][4];
+    // ---- the narrow operand of the scores: head g, scaled by a power of two so that its largest number lies in [2^13, 2^14)
+    float rs[2];                                   // what makes scores of the products, heads 2 tq and 2 tq + 1
+    uint32_t qh[KSTEPS][2], ql[LO ? KSTEPS : 1][2];
     {
       uint32_t largest = 0;
 #pragma unroll
-      for (int j = 0; j < HD / 64; ++j)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(&sm.q[g][64 * j + 16 * tq + 4 * w]);
-          largest = max(max(largest, max(abs_bits(x.x), abs_bits(x.y))), max(abs_bits(x.z), abs_bits(x.w)));
-        }
+      for (int j = 0; j < KSTEPS; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(&sm.q[g][64 * (j >> 2) + 16 * tq + 4 * (j & 3)]);
+        largest = max(max(largest, max(abs_bits(x.x), abs_bits(x.y))), max(abs_bits(x.z), abs_bits(x.w)));
+      }
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
       largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-      const int e = min(max((int)(largest >> 23), 1), 253);              // exponent of the row's largest number
-      const float f = __uint_as_float((uint32_t)(254 - e) << 23);
-      row_scale = __uint_as_float((uint32_t)e << 23) * p.scale_log2e;
+      const int e = min(max((int)(largest >> 23), 14), 253);
+      const float f = __uint_as_float((uint32_t)(267 - e) << 23), back = __uint_as_float((uint32_t)(e - 13) << 23) * p.scale_log2e;
+      rs[0] = __shfl_sync(0xffffffffu, back, 8 * tq);
+      rs[1] = __shfl_sync(0xffffffffu, back, 8 * tq + 4);
 #pragma unroll
-      for (int j = 0; j < HD / 64; ++j)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float4 x = *reinterpret_cast<const float4*>(&sm.q[g][64 * j + 16 * tq + 4 * w]);
-          split2(x.x * f, x.y * f, qf[4 * j + w][0], qf[4 * j + w][1]);
-          split2(x.z * f, x.w * f, qf[4 * j + w][2], qf[4 * j + w][3]);
+      for (int j = 0; j < KSTEPS; ++j) {
+        const float4 x = *reinterpret_cast<const float4*>(&sm.q[g][64 * (j >> 2) + 16 * tq + 4 * (j & 3)]);
+        qh[j][0] = half2_bits(x.x * f, x.y * f);
+        qh[j][1] = half2_bits(x.z * f, x.w * f);
+        if (LO) {
+          ql[j][0] = rest_bits(x.x * f, x.y * f, qh[j][0]);
+          ql[j][1] = rest_bits(x.z * f, x.w * f, qh[j][1]);
         }
+      }
     }
 
     // ---- the unfinished block, in fp32: a thread per (row, head), then per dimension
     if (owner) {
-      const int r = tid >> 3, h = tid & 7;
-      if (tid < BLK * GH) {
+      const int r = tid >> 3, h = tid & 7;           // (threads beyond the 16 rows have nothing to do)
+      float sc = -INFINITY;
+      if (r < BLK && base + r <= pos && base + r >= j_min) {
         float dot = 0.f;
-        if (base + r <= pos) {
 #pragma unroll 8
-          for (int d = 0; d < HD; d += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][d]);
-            const T* k = &sm.tail[0][r][d];
-            dot = fmaf(x.x, to_f32(k[0]), dot); dot = fmaf(x.y, to_f32(k[1]), dot);
-            dot = fmaf(x.z, to_f32(k[2]), dot); dot = fmaf(x.w, to_f32(k[3]), dot);
-          }
+        for (int d = 0; d < HD; d += 4) {
+          const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][d]);
+          const T* k = &sm.tail[0][r][d];
+          dot = fmaf(x.x, to_f32(k[0]), dot); dot = fmaf(x.y, to_f32(k[1]), dot);
+          dot = fmaf(x.z, to_f32(k[2]), dot); dot = fmaf(x.w, to_f32(k[3]), dot);
         }
-        sm.tail_s[r][h] = base + r <= pos && base + r >= j_min ? dot * p.scale_log2e : -INFINITY;
+        sc = dot * p.scale_log2e;
       }
+      if (r < BLK) sm.tail_s[r][h] = sc;
       __syncthreads();
-      if (tid < GH) {
-        float mx = -INFINITY, l = 0.f;
-        for (int i = 0; i < BLK; ++i) mx = fmaxf(mx, sm.tail_s[i][tid]);
-        for (int i = 0; i < BLK; ++i) {
-          const float x = sm.tail_s[i][tid];
-          const float pr = mx == -INFINITY ? (x == x ? 0.f : x) : exp2f(x - mx);
-          sm.tail_s[i][tid] = pr;
-          l += pr;
-        }
-        sm.ml[WARPS][tid][0] = mx;
-        sm.ml[WARPS][tid][1] = l;
-        if (c.weight && tid < n_g) p.part[((size_t)t * p.heads + head0 + tid) * p.blocks + nb] = mx + log2f(l);
+      float mx = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int i = 0; i < BLK; ++i) mx = fmaxf(mx, sm.tail_s[i][h]);
+      const float pr = mx == -INFINITY ? (sc == sc ? 0.f : sc) : ex2(sc - mx);
+      __syncthreads();
+      if (r < BLK) sm.tail_s[r][h] = pr;
+      __syncthreads();
+      if (r == 0) {
+#pragma unroll
+        for (int i = 0; i < BLK; ++i) l += sm.tail_s[i][h];
+        sm.ml[WARPS][h][0] = mx;
+        sm.ml[WARPS][h][1] = l;
+        if (part) part[(size_t)nb * GH + h] = mx + log2f(l);
       }
-      __syncthreads();
-      for (int d = tid; d < HD; d += THREADS) {
-        float acc[GH] = {};
+      constexpr int PER = GH * HD / THREADS < 1 ? 1 : GH * HD / THREADS;     // heads of a thread
+      for (int e = tid; e < HD * GH / PER; e += THREADS) {
+        const int d = e % HD, k0 = e / HD * PER;
+        float acc[PER] = {};
         for (int i = max(0, j_min - base); i <= pos - base; ++i) {
           const float v = to_f32(sm.tail[1][i][d]);
 #pragma unroll
-          for (int k = 0; k < GH; ++k) acc[k] = fmaf(sm.tail_s[i][k], v, acc[k]);
+          for (int k = 0; k < PER; ++k) acc[k] = fmaf(sm.tail_s[i][k0 + k], v, acc[k]);
         }
 #pragma unroll
-        for (int k = 0; k < GH; ++k) sm.tail_o[k][d] = acc[k];
+        for (int k = 0; k < PER; ++k) sm.tail_o[k0 + k][d] = acc[k];
       }
     }
 
-    // ---- the finished blocks
-    float o[DPL][2];
+    // ---- the finished blocks.  o[i]: dimensions DPL g + 2 i (0, 1) and + 1 (2, 3), heads 2 tq (0, 2) and 2 tq + 1 (1, 3)
+    float o[DPL / 2][4];
 #pragma unroll
-    for (int n = 0; n < DPL; ++n) o[n][0] = o[n][1] = 0.f;
-    float ref = -INFINITY, l_row = 0.f;             // sums are relative to 2^ref; ref = running maximum - P_SHIFT
+    for (int n = 0; n < DPL / 2; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // probabilities are relative to 2^ref
+    float v_top = 0.f, v_inv = INFINITY;                            // the largest value scale so far: o is in its units
     for (int i = 0; i < n_mine; ++i) {
-      if ((i & 31) == 0 && i > 0) {                 // the next 32 blocks; `at` holds the groups of even number, `at_next` the odd ones
-        if ((i >> 5) & 1) look_up(i + 32, at, ks, vs); else look_up(i + 32, at_next, ks_next, vs_next);
+      if ((i & 31) == 0 && i > 0) {                 // the next 32 blocks
+        if ((i >> 5) & 1) look_up(i + 32, 0); else look_up(i + 32, 1);
       }
       issue(i + NSTAGE - 1);
+      const bool odd = (i >> 5) & 1;
+      const int a = __shfl_sync(0xffffffffu, odd ? at[1] : at[0], i & 31);
+      const float k_scale = __shfl_sync(0xffffffffu, odd ? ks[1] : ks[0], i & 31), v_scale = __shfl_sync(0xffffffffu, odd ? vs[1] : vs[0], i & 31);
+      const int x = lo + warp + WARPS * i;
       cp_wait<NSTAGE - 1>();
       __syncwarp();
-      const bool odd = (i >> 5) & 1;
-      const int a = __shfl_sync(0xffffffffu, odd ? at_next : at, i & 31);
-      const float k_scale = __shfl_sync(0xffffffffu, odd ? ks_next : ks, i & 31), v_scale = __shfl_sync(0xffffffffu, odd ? vs_next : vs, i & 31);
-      const int x = lo + warp + WARPS * i;
       if (a < 0) {                                   // a page that the pool does not have: the block counts for nothing
-        if (c.weight && lane < n_g) p.part[((size_t)t * p.heads + head0 + lane) * p.blocks + x] = -INFINITY;
+        if (part && lane < GH) part[(size_t)x * GH + lane] = -INFINITY;
         continue;
       }
       const uint8_t *kt = sm.ring[warp][i % NSTAGE][0], *vt = sm.ring[warp][i % NSTAGE][1];
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float sc[4] = {0.f, 0.f, 0.f, 0.f}, sl[4] = {0.f, 0.f, 0.f, 0.f};      // positions g (0, 1) and g + 8 (2, 3), heads as above
 #pragma unroll
-      for (int j = 0; j < HD / 64; ++j)
+      for (int j = 0; j < HD / 64; ++j) {
+        const uint4 w0 = *reinterpret_cast<const uint4*>(kt + k_chunk<HD>(g * (HD / 16) + 4 * j + tq) * 16);
+        const uint4 w1 = *reinterpret_cast<const uint4*>(kt + k_chunk<HD>((g + 8) * (HD / 16) + 4 * j + tq) * 16);
+        const uint32_t wa[4] = {w0.x, w0.y, w0.z, w0.w}, wb[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const uint4 w4 = *reinterpret_cast<const uint4*>(kt + k_chunk<HD>((n * 8 + g) * (HD / 16) + 4 * j + tq) * 16);
-          const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t b0, b1;
-            levels4<FMT>(w[e], b0, b1);
-            mma_f16(sc[n], qf[4 * j + e], b0, b1);
+        for (int e = 0; e < 4; ++e) {
+          uint32_t f[4];
+          levels4<FMT>(wa[e], f[0], f[2]);
+          levels4<FMT>(wb[e], f[1], f[3]);
+          // two sums of half the dimensions each (float runs: upper and lower halves of the queries), so that products wait for one another less
+          if (LO) {
+            mma_f16(sc, f, qh[4 * j + e][0], qh[4 * j + e][1]);
+            mma_f16(sl, f, ql[4 * j + e][0], ql[4 * j + e][1]);
+          } else {
+            mma_f16(e & 1 ? sl : sc, f, qh[4 * j + e][0], qh[4 * j + e][1]);
           }
         }
-      const float f = k_scale * row_scale;
-      const int first = j_min - x * BLK;             // rows below are outside the window
-      float v[2][2], mx = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          v[n][e] = n * 8 + tq * 2 + e >= first ? (sc[n][e] + sc[n][e + 2]) * f : -INFINITY;
-          mx = fmaxf(mx, v[n][e]);
-        }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float ref_new = fmaxf(ref, mx - P_SHIFT);
-      if (__any_sync(0xffffffffu, ref_new != ref)) {
-        const float alpha = ref_new == ref ? 1.f : exp2f(ref - ref_new);
-        ref = ref_new;
-        l_row *= alpha;
-#pragma unroll
-        for (int n = 0; n < DPL; ++n) { o[n][0] *= alpha; o[n][1] *= alpha; }
       }
-      float sum = 0.f, pr[2][2];
+      float v[4], y[4];
+      bool far = false;
+      const int first = j_min - x * BLK;             // positions below are outside the window
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          pr[n][e] = ref == -INFINITY ? (v[n][e] == v[n][e] ? 0.f : v[n][e]) : exp2f(v[n][e] - ref);
-          sum += pr[n][e];
-        }
-      l_row += sum;
-      if (c.weight) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        if (tq == 0 && g < n_g) p.part[((size_t)t * p.heads + head0 + g) * p.blocks + x] = ref + log2f(sum);
+      for (int e = 0; e < 4; ++e) {
+        v[e] = (sc[e] + sl[e]) * (k_scale * rs[e & 1]);
+        if (first > 0 && g + 8 * (e >> 1) < first) v[e] = -INFINITY;
+        y[e] = v[e] - ref[e & 1];
+        far |= !(y[e] <= HEADROOM);
       }
-      uint32_t pf[4];
-      split2(pr[0][0], pr[0][1], pf[0], pf[1]);
-      split2(pr[1][0], pr[1][1], pf[2], pf[3]);
+      if (__any_sync(0xffffffffu, far)) {            // the first block, a score far above what came before, or something that is not a number
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(v[h], v[h + 2]);
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+          const float to = fmaxf(ref[h], mx - BELOW);
+          const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
+          ref[h] = to;
+          l[h] *= alpha;
+#pragma unroll
+          for (int n = 0; n < DPL / 2; ++n) { o[n][h] *= alpha; o[n][h + 2] *= alpha; }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = v[e] == -INFINITY ? v[e] : v[e] - ref[e & 1];
+      }
+      if (v_scale > v_top) {                         // (the same for the whole warp)
+        const float f = v_top / v_scale;
+        v_top = v_scale;
+        v_inv = 1.f / v_scale;
+#pragma unroll
+        for (int n = 0; n < DPL / 2; ++n) { o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f; }
+      }
+      const float vr = v_scale * v_inv;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
+      const float s0 = y[0] + y[2], s1 = y[1] + y[3];
+      l[0] += s0;
+      l[1] += s1;
+      if (part) {                                    // the block's sums: lanes of g < 4 end with head 2 tq, the others with 2 tq + 1
+        float keep = g & 4 ? s1 : s0;
+        keep += __shfl_xor_sync(0xffffffffu, g & 4 ? s0 : s1, 16);
+        keep += __shfl_xor_sync(0xffffffffu, keep, 8);
+        keep += __shfl_xor_sync(0xffffffffu, keep, 4);
+        if ((g & 3) == 0) part[(size_t)x * GH + 2 * tq + (g >> 2)] = (g & 4 ? ref[1] : ref[0]) + log2f(keep);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] *= vr;
+      const uint32_t p0 = half2_bits(y[0], y[1]), p1 = half2_bits(y[2], y[3]);
+      const uint32_t b0 = transposed(p0), b1 = transposed(p1);
+      uint32_t r0 = 0, r1 = 0;
+      if (LO) { r0 = transposed(rest_bits(y[0], y[1], p0)); r1 = transposed(rest_bits(y[2], y[3], p1)); }
       // values of rows 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions [DPL g, DPL (g + 1))
       uint32_t vw[4][DPL / 4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int vr = 2 * tq + (r & 1) + 8 * (r >> 1);
+        const int vr_ = 2 * tq + (r & 1) + 8 * (r >> 1);
         if (HD == 128) {
-          const uint4 w4 = *reinterpret_cast<const uint4*>(vt + v_chunk<HD>(vr * 8 + g) * 16);
+          const uint4 w4 = *reinterpret_cast<const uint4*>(vt + v_chunk<HD>(vr_ * 8 + g) * 16);
           vw[r][0] = w4.x; vw[r][1] = w4.y; vw[r][DPL / 4 - 2] = w4.z; vw[r][DPL / 4 - 1] = w4.w;
         } else {
-          const uint2 w2 = *reinterpret_cast<const uint2*>(vt + v_chunk<HD>(vr * 4 + (g >> 1)) * 16 + (g & 1) * 8);
+          const uint2 w2 = *reinterpret_cast<const uint2*>(vt + v_chunk<HD>(vr_ * 4 + (g >> 1)) * 16 + (g & 1) * 8);
           vw[r][0] = w2.x; vw[r][1] = w2.y;
         }
       }
 #pragma unroll
       for (int w = 0; w < DPL / 4; ++w)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {                // two dimensions at a time: bytes of two rows side by side
-          const uint32_t sel = y ? 0x7362 : 0x5140;
-          uint32_t b00, b01, b10, b11;
-          levels4<FMT>(__byte_perm(vw[0][w], vw[1][w], sel), b00, b01);
-          levels4<FMT>(__byte_perm(vw[2][w], vw[3][w], sel), b10, b11);
-          float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(c0, pf, b00, b10);
-          mma_f16(c1, pf, b01, b11);
-          const int n = 4 * w + 2 * y;
-          o[n][0] = fmaf(v_scale, c0[0] + c0[2], o[n][0]);
-          o[n][1] = fmaf(v_scale, c0[1] + c0[3], o[n][1]);
-          o[n + 1][0] = fmaf(v_scale, c1[0] + c1[2], o[n + 1][0]);
-          o[n + 1][1] = fmaf(v_scale, c1[1] + c1[3], o[n + 1][1]);
+        for (int z = 0; z < 2; ++z) {                // two dimensions at a time: bytes of two rows side by side
+          const uint32_t sel = z ? 0x7362 : 0x5140;
+          uint32_t f[4];
+          levels4<FMT>(__byte_perm(vw[0][w], vw[1][w], sel), f[0], f[1]);
+          levels4<FMT>(__byte_perm(vw[2][w], vw[3][w], sel), f[2], f[3]);
+          mma_f16(o[2 * w + z], f, b0, b1);
+          if (LO) mma_f16(o[2 * w + z], f, r0, r1);
         }
       __syncwarp();                                  // the stage may be filled again
     }
     cp_wait<0>();
     __syncwarp();
-    l_row += __shfl_xor_sync(0xffffffffu, l_row, 1);
-    l_row += __shfl_xor_sync(0xffffffffu, l_row, 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], w);
     float* mine = reinterpret_cast<float*>(&sm.ring[warp][0][0][0]);       // [GH][HD]
 #pragma unroll
-    for (int n = 0; n < DPL; ++n) {
-      mine[g * HD + DPL * (2 * tq) + n] = o[n][0];
-      mine[g * HD + DPL * (2 * tq + 1) + n] = o[n][1];
+    for (int n = 0; n < DPL / 2; ++n) {
+      *reinterpret_cast<float2*>(mine + (2 * tq) * HD + DPL * g + 2 * n) = make_float2(o[n][0] * v_top, o[n][2] * v_top);
+      *reinterpret_cast<float2*>(mine + (2 * tq + 1) * HD + DPL * g + 2 * n) = make_float2(o[n][1] * v_top, o[n][3] * v_top);
     }
-    if (tq == 0) { sm.ml[warp][g][0] = ref; sm.ml[warp][g][1] = l_row; }
-    __syncthreads();
-
-    // ---- the CTA's partial result: warps in their order, then the unfinished block
-    const int parts = WARPS + (owner ? 1 : 0);
-    for (int i = tid; i < n_g * HD; i += THREADS) {
-      const int h = i / HD, d = i % HD;
-      float mm = -INFINITY, ll = 0.f, acc = 0.f;
-      for (int w = 0; w < parts; ++w) mm = fmaxf(mm, sm.ml[w][h][0]);
+    if (g == 0) {
 #pragma unroll
-      for (int w = 0; w < WARPS + 1; ++w) {
-        if (w == WARPS && !owner) break;
-        const float f = sm.ml[w][h][0] == -INFINITY && mm == -INFINITY ? 1.f : exp2f(sm.ml[w][h][0] - mm);
-        ll += f * sm.ml[w][h][1];
-        acc += f * (w < WARPS ? reinterpret_cast<const float*>(&sm.ring[w][0][0][0])[h * HD + d] : sm.tail_o[h][d]);
-      }
-      sm.o[h][d] = acc;
-      if (d == 0) { sm.oml[h][0] = mm; sm.oml[h][1] = ll; }
-    }
-    if (S > 1) cluster.sync(); else __syncthreads();
-
-    // ---- the cluster's: every CTA an equal share of the outputs
-    if (tid < n_g) {
-      float mm = -INFINITY, ll = 0.f;
-      for (int r = 0; r < S; ++r) mm = fmaxf(mm, S > 1 ? *cluster.map_shared_rank(&sm.oml[tid][0], r) : sm.oml[tid][0]);
-      for (int r = 0; r < S; ++r) {
-        const float m = S > 1 ? *cluster.map_shared_rank(&sm.oml[tid][0], r) : sm.oml[tid][0];
-        const float l = S > 1 ? *cluster.map_shared_rank(&sm.oml[tid][1], r) : sm.oml[tid][1];
-        ll += (m == -INFINITY && mm == -INFINITY ? 1.f : exp2f(m - mm)) * l;
-      }
-      sm.lse[tid][0] = mm;
-      sm.lse[tid][1] = ll == 0.f ? 0.f : 1.f / ll;
+      for (int h = 0; h < 2; ++h) { sm.ml[warp][2 * tq + h][0] = ref[h]; sm.ml[warp][2 * tq + h][1] = l[h]; }
     }
     __syncthreads();
-    for (int i = rank * THREADS + tid; i < n_g * HD; i += S * THREADS) {
-      const int h = i / HD, d = i % HD;
-      const float mm = sm.lse[h][0];
-      float acc = 0.f;
-      for (int r = 0; r < S; ++r) {
-        const float m = S > 1 ? *cluster.map_shared_rank(&sm.oml[h][0], r) : sm.oml[h][0];
-        const float y = S > 1 ? *cluster.map_shared_rank(&sm.o[h][d], r) : sm.o[h][d];
-        acc += (m == -INFINITY && mm == -INFINITY ? 1.f : exp2f(m - mm)) * y;
-      }
-      out[(size_t)g0 * HD + i] = from_f32<T>(acc * sm.lse[h][1]);
+    if (tid < (WARPS + 1) * GH) {                  // warps in their order, then the unfinished block
+      const int w = tid / GH, h = tid % GH;
+      const int n = owner ? WARPS + 1 : WARPS;
+      float mm = -INFINITY;
+      for (int k = 0; k < n; ++k) mm = fmaxf(mm, sm.ml[k][h][0]);
+      sm.wfac[w][h] = w >= n ? 0.f : sm.ml[w][h][0] == mm ? 1.f : ex2(sm.ml[w][h][0] - mm);
     }
-    if (c.weight) {
+    cluster.barrier_wait(std::move(started));      // every CTA runs (and has read what it was sent for the heads before)
+    __syncthreads();
+
+    // ---- the CTA's partial result goes to the CTAs that add up its pieces
+    const int share = (n_g * HD + S - 1) / S;
+#pragma unroll
+    for (int k = 0; k < GH * HD / THREADS; ++k) {
+      const int i = tid + k * THREADS, h = i / HD, d = i % HD;
+      if (i >= n_g * HD) break;
+      float acc = owner ? sm.wfac[WARPS][h] * sm.tail_o[h][d] : 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) acc += sm.wfac[w][h] * reinterpret_cast<const float*>(&sm.ring[w][0][0][0])[h * HD + d];
+      const int to = i / share;
+      cluster.map_shared_rank(&sm.o_in[0], to)[rank * share + i - to * share] = acc;
+    }
+    if (tid < S * GH) {
+      const int to = tid / GH, h = tid % GH, n = owner ? WARPS + 1 : WARPS;
+      float mm = -INFINITY, ll = 0.f;
+      for (int k = 0; k < n; ++k) { mm = fmaxf(mm, sm.ml[k][h][0]); ll += sm.wfac[k][h] * sm.ml[k][h][1]; }
+      *reinterpret_cast<float2*>(cluster.map_shared_rank(&sm.ml_in[rank][h][0], to)) = make_float2(mm, ll);
+    }
+    cluster.sync();
+
+    // ---- this CTA's share of the outputs
+    if (tid < S * GH) {
+      const int r = tid / GH, h = tid % GH;
+      float mm = -INFINITY, ll = 0.f;
+      for (int k = 0; k < S; ++k) mm = fmaxf(mm, sm.ml_in[k][h][0]);
+      for (int k = 0; k < S; ++k) ll += (sm.ml_in[k][h][0] == mm ? 1.f : ex2(sm.ml_in[k][h][0] - mm)) * sm.ml_in[k][h][1];
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      sm.fac[r][h] = (sm.ml_in[r][h][0] == mm ? 1.f : ex2(sm.ml_in[r][h][0] - mm)) * inv;
+      if (r == 0) { sm.lse[h][0] = mm; sm.lse[h][1] = inv; }
+    }
+    __syncthreads();
+    for (int k = tid; k < share; k += THREADS) {
+      const int i = rank * share + k;
+      if (i >= n_g * HD) break;
+      float acc = 0.f;
+      for (int r = 0; r < S; ++r) acc += sm.fac[r][i / HD] * sm.o_in[r * share + k];
+      out[(size_t)g0 * HD + i] = from_f32<T>(acc);
+    }
+    if (part) {
       // weight of block x: the sum over the group's heads, in their order, of 2^(part - maximum) / sum
-      const int end = owner ? nb + 1 : hi, begin = owner && lo >= nb ? nb : lo;
-      for (int x = begin + tid; x < end; x += THREADS) {
+      const int end = owner ? nb + 1 : hi;
+      for (int x = lo + tid; x < end; x += THREADS) {
         const int page = block_page(c, slot, x / per_page, p.err);
         if (page < 0) continue;
         const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + x % per_page;
         float w = g0 > 0 ? p.weight_out[i] : x == nb && pos == base ? 0.f : c.weight[i];
-        for (int h = 0; h < n_g; ++h) w += exp2f(p.part[((size_t)t * p.heads + head0 + h) * p.blocks + x] - sm.lse[h][0]) * sm.lse[h][1];
+        const float4 a = *reinterpret_cast<const float4*>(part + (size_t)x * GH), b4 = *reinterpret_cast<const float4*>(part + (size_t)x * GH + 4);
+        const float e[GH] = {a.x, a.y, a.z, a.w, b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+        for (int h = 0; h < GH; ++h)
+          if (h < n_g) w += ex2(e[h] - sm.lse[h][0]) * sm.lse[h][1];
         p.weight_out[i] = w;
       }
     }
-    if (S > 1) cluster.sync(); else __syncthreads();      // nobody reads this CTA's results any more
+    if (g0 + GH < group) {
+      __syncthreads();
+      started = cluster.barrier_arrive();
+    }
   }
 
   if (owner && pos - base == BLK - 1) {              // the block is full: from the next step on it is read in 8 bits
@@ -471,16 +526,16 @@ __global__ void __launch_bounds__(THREADS, 3) block_attention_tc_kernel(BlockTcP
   }
 }
 
-template <int HD, int FMT, typename T>
+template <int HD, int FMT, typename T, int WARPS>
 int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
-  auto kernel = block_attention_tc_kernel<HD, FMT, T>;
-  const size_t smem = sizeof(Shared<HD, T>);
+  auto kernel = block_attention_tc_kernel<HD, FMT, T, WARPS>;
+  const size_t smem = sizeof(Shared<HD, T, WARPS>);
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
       cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return iert_check_launch("block_attention (attributes)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(WARPS * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -494,25 +549,43 @@ int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& 
   return iert_check_launch("block_attention");
 }
 
+template <int HD, int FMT, typename T>
+int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, int warps, cudaStream_t stream) {
+  if (warps == 4) return launch<HD, FMT, T, 4>(p, b, c, splits, stream);
+  if (warps == 8) return launch<HD, FMT, T, 8>(p, b, c, splits, stream);
+  return launch<HD, FMT, T, 16>(p, b, c, splits, stream);
+}
+
 }  // namespace
 
-// `splits` (1, 2, 4, 8, 16; 0: by the rule below): CTAs that share a sequence's kv head.
+// Floats of scratch: the blocks' weights, if the view keeps them.
+IERT_API long long iert_block_attention_scratch(int n_seqs, int heads, const IertBlockView* view) {
+  const IertBlockView& c = *view;
+  if (!c.weight || n_seqs <= 0 || c.kv_heads <= 0 || heads <= 0) return 1;
+  const long long pairs = (long long)n_seqs * c.kv_heads * ((heads / c.kv_heads + GH - 1) / GH);
+  return pairs * c.table_width * (c.page_tokens / BLK) * GH;
+}
+
+// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head, and `warps` (4, 8, 16) of each; 0: by the rule below.
 IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
                                      float* part, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
-                                     int* err, cudaStream_t stream) {
+                                     int warps, int* err, cudaStream_t stream) {
   if (batch->n_tokens <= 0) return IERT_OK;
   const IertBlockView& c = *view;
   if ((c.head_dim != 64 && c.head_dim != 128) || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || batch->n_tokens != batch->n_seqs ||
       batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 || c.ring_pages <= 0 ||
       c.ring_pages > c.table_width || c.n_pages <= 0 || c.n_slots <= 0 || c.window < 0 ||
-      (c.weight && (c.window || !part || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v) % 16 ||
+      (c.weight && (c.window || !part || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)part) % 16 ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > c.head_dim || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
     return IERT_BAD_ARGUMENT;
+  if (warps != 0 && warps != 4 && warps != 8 && warps != 16) return IERT_BAD_ARGUMENT;
+  const long long pairs = (long long)c.kv_heads * batch->n_seqs;
+  const int sms = iert_sm_count_cached();
+  if (warps == 0) warps = pairs > 2 * sms ? 4 : 8;
   if (splits < 0 || splits > 16 || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
   if (splits == 0) {
-    const long long base = (long long)c.kv_heads * batch->n_seqs;
-    splits = 1;
-    while (splits < 16 && base * splits * 2 <= 3LL * iert_sm_count_cached()) splits *= 2;
+    splits = pairs > 2 * sms ? 2 : 1;
+    while (splits < 16 && pairs * splits * 2 <= 2LL * sms) splits *= 2;
   }
   BlockTcParams p = {};
   p.qkv = qkv; p.out = out; p.part = part; p.weight_out = weight_out;
@@ -521,13 +594,13 @@ IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatch
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
   const int which = (c.head_dim == 128 ? 4 : 0) + (c.format == IERT_LEVEL_E4M3 ? 2 : 0) + (c.tail_dtype == IERT_BF16 ? 1 : 0);
   switch (which) {
-    case 0: return launch<64, IERT_LEVEL_INT8, float>(p, *batch, c, splits, stream);
-    case 1: return launch<64, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, stream);
-    case 2: return launch<64, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, stream);
-    case 3: return launch<64, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, stream);
-    case 4: return launch<128, IERT_LEVEL_INT8, float>(p, *batch, c, splits, stream);
-    case 5: return launch<128, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, stream);
-    case 6: return launch<128, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, stream);
-    default: return launch<128, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, stream);
+    case 0: return launch<64, IERT_LEVEL_INT8, float>(p, *batch, c, splits, warps, stream);
+    case 1: return launch<64, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
+    case 2: return launch<64, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, warps, stream);
+    case 3: return launch<64, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
+    case 4: return launch<128, IERT_LEVEL_INT8, float>(p, *batch, c, splits, warps, stream);
+    case 5: return launch<128, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
+    case 6: return launch<128, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, warps, stream);
+    default: return launch<128, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
   }
 }

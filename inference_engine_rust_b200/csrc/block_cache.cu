@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(256) block_attention_plain_kernel(BlockAttenti
     __syncthreads();
     for (int i = threadIdx.x; i < n_g * hd; i += blockDim.x) {
       const T* q = row + (size_t)(head0 + i / hd) * hd;
-      qs[i] = p.rope ? rotated(q, i % hd, p.rotary_dim, p.pairing, cs) : to_f32(q[i % hd]);
+      qs[i] = p.rope ? to_f32(from_f32<T>(rotated(q, i % hd, p.rotary_dim, p.pairing, cs))) : to_f32(q[i % hd]);
     }
     __syncthreads();
     float o[GH][MAXD], m[GH], l[GH];

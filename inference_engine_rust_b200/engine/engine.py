@@ -18,7 +18,7 @@ from typing import List, Optional, Sequence, Tuple, Union
 import numpy as np
 import torch
 
-from ..cache import PAGE_TOKENS, Cache, CacheError, CacheFull
+from ..cache import PAGE_TOKENS, Cache, CacheError, CacheFull, EvictionPolicy, parse_cache_dtype
 from ..cache.staging import PinnedRing
 from ..csrc import bindings as B
 from ..parts.base import HostCopyUnavailable, StepContext
@@ -134,7 +134,7 @@ class Engine:
 
     def __init__(self, model: Model, *, max_tokens: int, max_sequences: Optional[int] = None,
                  max_seq_len: Optional[int] = None, poison_cache: bool = False, use_graphs: bool = True,
-                 page_tokens: int = PAGE_TOKENS):
+                 page_tokens: int = PAGE_TOKENS, cache_dtype=None, eviction: Optional[EvictionPolicy] = None):
         if not model.loaded:
             raise ValueError("the model has no weights yet (load() or load_random() first)")
         B.require_device()
@@ -146,10 +146,16 @@ class Engine:
             max_sequences = max(1, min(n_pages, 1024))
         if max_seq_len is None:
             max_seq_len = spec.max_position
+        levels = parse_cache_dtype(cache_dtype)
+        if eviction is not None and levels is None:
+            raise ValueError("eviction needs an 8-bit cache (cache_dtype)")
+        if levels is not None:
+            model.check_block_cache(eviction is not None)
+        self.max_positions = min(max_seq_len, spec.max_position)      # of a sequence, those that it has lost to eviction included
         self.cache = Cache(model.cache_requests(), max_tokens=max_tokens,
-                           max_seq_len=min(max_seq_len, spec.max_position),
+                           max_seq_len=self.max_positions,
                            max_sequences=max_sequences, dtype=self.rt.dtype, device=self.rt.device,
-                           page_tokens=page_tokens, poison=poison_cache)
+                           page_tokens=page_tokens, poison=poison_cache, levels=levels, eviction=eviction)
         self._staging = PinnedRing()
         self._meta_dev: Optional[torch.Tensor] = None
         self.steps_run = 0
@@ -169,6 +175,7 @@ class Engine:
         self.cache.close_sequence(slot)
 
     def length(self, slot: int) -> int:
+        """Positions that the sequence holds (those it has lost to eviction apart)."""
         return self.cache.length(slot)
 
     # ---- the step ---------------------------------------------------------------------------
@@ -205,6 +212,9 @@ class Engine:
             if p + q > self.cache.max_seq_len:
                 raise CacheFull(f"slot {slot}: {p + q} tokens exceed the longest sequence the cache "
                                 f"holds ({self.cache.max_seq_len})")
+            if p + int(self.cache.lost[slot]) + q > self.max_positions:
+                raise CacheFull(f"slot {slot}: {p + int(self.cache.lost[slot]) + q} tokens, evicted ones included, exceed the longest "
+                                f"sequence ({self.max_positions})")
         cu = np.zeros(len(entries) + 1, dtype=np.int64)
         np.cumsum(q_lens, out=cu[1:])
         rows: List[int] = []
@@ -239,12 +249,13 @@ class Engine:
         if not entries or not (want == "last" or want == "all" or want is None or want == "none"):
             return None
         held, lens, vocab, limit = self.cache.slots._held, self.cache.seq_lens, self.model.spec.vocab_size, self.cache.max_seq_len
+        lost, reach = self.cache.lost, self.max_positions
         slots, pos0, toks = [], [], []
         for slot, t in entries:
             if len(t) != 1 or slot not in held:
                 return None
             tok, p = t[0], int(lens[slot])
-            if not 0 <= tok < vocab or p + 1 > limit:
+            if not 0 <= tok < vocab or p + 1 > limit or p + lost[slot] + 1 > reach:
                 return None
             slots.append(int(slot)); pos0.append(p); toks.append(tok)
         n = len(slots)
@@ -286,6 +297,9 @@ class Engine:
             logits = self._step_eager(kind, slots, q_lens, pos0, tokens, cu, rows, device_tokens)
         for slot, q in zip(slots, q_lens):
             self.cache.advance(slot, q)
+        if self.cache.eviction is not None and kind == "decode":
+            self.cache.steps_since[slots] += 1
+            self.cache.evict(slots, self.rt.err)
         self.steps_run += 1
         return logits
 

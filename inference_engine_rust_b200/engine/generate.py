@@ -38,9 +38,12 @@ class GenerationResult:
 
 def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, *, max_tokens: int,
                  max_sequences: int, max_seq_len: int, page_tokens: int,
-                 max_batch: Optional[int] = None) -> List[List[int]]:
+                 max_batch: Optional[int] = None, most_held: Optional[Callable[[int], int]] = None,
+                 capacity: Optional[int] = None) -> List[List[int]]:
     """Split requests, in order, into batches that fit the cache: a request may come to hold
-    min(prompt + max_new_tokens, max_seq_len) positions, rounded up to a page."""
+    min(prompt + max_new_tokens, max_seq_len) positions, rounded up to a page.  Where sequences lose positions to eviction,
+    `most_held(prompt length)` bounds what one comes to hold and `capacity` is the longest that the cache holds (`max_seq_len`
+    being the longest that one may grow, lost positions included)."""
     if max_batch is not None and max_batch <= 0:
         raise ValueError("max_batch must be positive")
     limit = min(max_sequences, max_batch) if max_batch else max_sequences
@@ -54,6 +57,11 @@ def plan_batches(prompt_lens: Sequence[int], max_new_tokens: int, *, max_tokens:
             raise ValueError(f"request {i}: a prompt of {n} tokens exceeds the longest sequence "
                              f"the cache holds ({max_seq_len})")
         need = min(n + max_new_tokens, max_seq_len)
+        if most_held is not None:
+            need = min(need, most_held(n))
+            if need > capacity:
+                raise ValueError(f"request {i}: a prompt of {n} tokens comes to hold {need} positions, the longest sequence the cache "
+                                 f"holds is {capacity}")
         need = math.ceil(need / page_tokens) * page_tokens
         if need > max_tokens:
             raise ValueError(f"request {i}: needs room for {need} tokens, the cache holds {max_tokens}")
@@ -141,7 +149,8 @@ def run_batch_ahead(engine, sampler, prompts: Sequence[Sequence[int]], request_i
 
 def run_batch(engine, sampler: Callable, prompts: Sequence[Sequence[int]], request_ids: Sequence[int],
               max_new_tokens: int, stop_ids: Set[int], max_seq_len: int,
-              on_token: Optional[Callable[[int, int], None]] = None) -> List[GenerationResult]:
+              on_token: Optional[Callable[[int, int], None]] = None,
+              allowed_tokens: Optional[Callable] = None) -> List[GenerationResult]:
     """One batch from its prompts to the end of its last sequence."""
     results = [GenerationResult(request=r, prompt_len=len(p)) for r, p in zip(request_ids, prompts)]
     if max_new_tokens <= 0:
@@ -156,7 +165,10 @@ def run_batch(engine, sampler: Callable, prompts: Sequence[Sequence[int]], reque
         logits = engine.step([(slots[i], list(prompts[i])) for i in live], want="last")
         step_no = 0
         while live:
-            chosen = sampler(logits, [request_ids[i] for i in live], [step_no] * len(live))
+            more = {}
+            if allowed_tokens is not None:
+                more["allowed"] = [allowed_tokens(request_ids[i], list(results[i].tokens)) for i in live]
+            chosen = sampler(logits, [request_ids[i] for i in live], [step_no] * len(live), **more)
             going_on, feed = [], []
             for i, tok in zip(live, chosen):
                 res = results[i]
@@ -184,9 +196,12 @@ def generate(engine, sampler: Callable, prompts: Sequence[Sequence[int]], max_ne
              page_tokens: int, max_batch: Optional[int] = None,
              request_ids: Optional[Sequence[int]] = None,
              on_token: Optional[Callable[[int, int], None]] = None,
-             run_ahead: bool = True) -> List[GenerationResult]:
+             run_ahead: bool = True, most_held: Optional[Callable[[int], int]] = None, capacity: Optional[int] = None,
+             allowed_tokens: Optional[Callable] = None) -> List[GenerationResult]:
     """All requests, batch after batch, results in the order of `prompts`.  `run_ahead`: keep the
-    device one step ahead of the host where engine and sampler allow it."""
+    device one step ahead of the host where engine and sampler allow it.  `most_held`, `capacity`: see `plan_batches`.
+    `allowed_tokens(request, tokens)`: which ids may come next in a request's answer so far (see `Sampler.sample_device`); it is asked
+    on the host, token by token, so nothing runs ahead then."""
     if request_ids is None:
         request_ids = list(range(len(prompts)))
     if len(request_ids) != len(prompts):
@@ -194,12 +209,16 @@ def generate(engine, sampler: Callable, prompts: Sequence[Sequence[int]], max_ne
     stop = set(int(s) for s in stop_ids)
     batches = plan_batches([len(p) for p in prompts], max_new_tokens, max_tokens=max_tokens,
                            max_sequences=max_sequences, max_seq_len=max_seq_len,
-                           page_tokens=page_tokens, max_batch=max_batch)
+                           page_tokens=page_tokens, max_batch=max_batch, most_held=most_held, capacity=capacity)
     out: List[Optional[GenerationResult]] = [None] * len(prompts)
     for batch in batches:
-        run = run_batch_ahead if run_ahead and can_run_ahead(engine, sampler) else run_batch
-        res = run(engine, sampler, [prompts[i] for i in batch], [request_ids[i] for i in batch],
-                  max_new_tokens, stop, max_seq_len, on_token)
+        if hasattr(sampler, "begin"):
+            sampler.begin([request_ids[i] for i in batch], [prompts[i] for i in batch], max_new_tokens)
+        args = (engine, sampler, [prompts[i] for i in batch], [request_ids[i] for i in batch], max_new_tokens, stop, max_seq_len, on_token)
+        if allowed_tokens is not None:
+            res = run_batch(*args, allowed_tokens=allowed_tokens)
+        else:
+            res = (run_batch_ahead if run_ahead and can_run_ahead(engine, sampler) else run_batch)(*args)
         for i, r in zip(batch, res):
             r.request = i
             out[i] = r

@@ -184,6 +184,27 @@ class Model:
                 out[self._input_key(i)] = request
         return out
 
+    def check_block_cache(self, eviction: bool) -> None:
+        """ValueError if some execution could not run over a cache in 8 bits (or, with `eviction`, over one that loses positions)."""
+        from ..cache import KVRequest
+
+        def requests(r):
+            return [x for part in r for x in requests(part)] if isinstance(r, (tuple, list)) else [r]
+        for pos, e in enumerate(self.spec.schedule):
+            mixer = self._layer_parts[e.layer][1]
+            kept = [r for r in requests(mixer.cache_request()) if isinstance(r, KVRequest)]
+            what = f"layer {e.layer} ({type(mixer).__name__})"
+            if kept and not getattr(mixer, "block_cache", False):
+                raise ValueError(f"{what} does not run over an 8-bit cache")
+            if kept and not e.writes_cache:
+                raise ValueError(f"{what} reads another execution's cache, which an 8-bit cache does not allow")
+            if eviction and not kept:
+                raise ValueError(f"{what} keeps a state per sequence, from which nothing can be evicted")
+            if eviction and getattr(getattr(mixer, "position", None), "rotary_constants", lambda: None)() is None:
+                raise ValueError(f"{what}: its position encoding cannot follow a sequence that loses positions")
+        if any(getattr(part, "cache_request", lambda: None)() is not None for part, _ in self.inputs):
+            raise ValueError("a step input keeps something per sequence, which an 8-bit cache does not allow")
+
     @staticmethod
     def _input_key(i: int) -> int:
         """Under which key the cache keeps what the i-th step input asked for (the schedule's entries count from 0)."""

@@ -12,6 +12,9 @@ which is the layout the rope-and-store and attention kernels index.
 A prompt (every sequence starts at position 0) attends over the step's own keys and values;
 a one-token step attends over the cache.  An execution that reads another execution's cache
 stores nothing and always attends over that cache.
+
+Over a cache in 8 bits (`cache_view.blocks`) a prompt attends over its keys and values as they come and stores them in blocks;
+a one-token step rotates, stores and attends in one kernel.
 """
 from __future__ import annotations
 
@@ -29,6 +32,7 @@ from .linear import Linear
 class Attention(Mixer):
     graph_safe = True
     takes_lazy_input = True          # its input goes to a projection, which may finish a norm itself
+    block_cache = True
 
     def __init__(self, spec, rt: Runtime):
         self.rt = rt
@@ -77,7 +81,7 @@ class Attention(Mixer):
         return ("attention", self.heads, self.kv_heads, self.head_dim, self.window, self.rt.fast)
 
     def cut_by_length(self, pos0, cache_view) -> bool:
-        if not self.rt.fast or cache_view is None:
+        if not self.rt.fast or cache_view is None or cache_view.blocks is not None:
             return False
         from . import fast_attention
         return fast_attention.wants_length_cut(pos0, self.kv_heads, self.heads // self.kv_heads, self.window,
@@ -89,6 +93,10 @@ class Attention(Mixer):
         qkv = ws.take("attn.qkv", (T, self.q_dim + 2 * self.kv_dim), rt.dtype)
         self.qkv.apply(xn, qkv, T, ctx.stream)
         out = ws.take("attn.out", (T, self.q_dim), rt.dtype)
+        if cache_view.blocks is not None and ctx.kind == "decode":
+            self._decode_blocks(qkv, out, ctx, cache_view.blocks)
+            self.o.apply(out, residual, T, ctx.stream, add_residual=True, ctx=ctx)
+            return
         if rt.fast and ctx.kind == "decode":
             # one token per sequence: rotation, cache write and attention in one kernel, if the
             # position encoding is a plain rotation and the kernel takes the sizes
@@ -99,7 +107,10 @@ class Attention(Mixer):
         # positions for queries and keys, then the cache write (the mixer's own business); a plain
         # rotation is fused with the write in one kernel
         rot = getattr(self.position, "rotary_constants", lambda: None)()      # (optional in the interface)
-        if rot is not None:
+        if cache_view.blocks is not None:
+            self.position.encode(qkv, ctx, self.heads, self.kv_heads)
+            B.block_store(qkv, ctx.batch, cache_view.blocks, self.heads, rt.err, ctx.stream)
+        elif rot is not None:
             inv_freq, rotary_dim, pairing = rot
             B.rope_kv_store(qkv, ctx.batch, kv, inv_freq, self.heads, rotary_dim, pairing, writes_cache,
                             rt.err, ctx.stream)
@@ -122,6 +133,17 @@ class Attention(Mixer):
             B.attention_plain(qkv, out, ctx.batch, kv, self.heads, self.scale, from_cache,
                               rt.err, ctx.stream)
         self.o.apply(out, residual, T, ctx.stream, add_residual=True, ctx=ctx)
+
+    def _decode_blocks(self, qkv, out, ctx: StepContext, blocks) -> None:
+        """A one-token step over a cache in 8 bits, which the step's key and value join."""
+        rt = self.rt
+        rot = getattr(self.position, "rotary_constants", lambda: None)()
+        if rot is None:                      # (a cache with eviction is refused for such an encoding: it knows nothing of lost positions)
+            self.position.encode(qkv, ctx, self.heads, self.kv_heads)
+        n = B.block_attention_scratch_floats(ctx.n_seqs, self.heads, blocks)
+        scratch = rt.workspace.take("attn.block_scratch", (n,), torch.float32)
+        B.block_attention(qkv, out, ctx.batch, blocks, self.heads, self.scale, scratch, rt.err, ctx.stream,
+                          rope=None if rot is None else (*rot, 1.0), plain=rt.plain_only and not rt.split_f32)
 
 
 register_part("mixer", "attention", Attention)

@@ -268,6 +268,8 @@ class Mixer(Part):
     # True: `cut_by_length` takes a third argument, the number of sequences that the step's launches are sized for (a captured
     # step is padded to a power of two), which is what they plan by.
     cut_by_batch = False
+    # True: the mixer also runs over a cache in 8 bits (its view's `blocks`)
+    block_cache = False
 
     def cache_request(self) -> CacheRequest:
         return None

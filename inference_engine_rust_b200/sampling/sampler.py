@@ -10,9 +10,11 @@ the same numbers alone and in any batch.
 from __future__ import annotations
 
 import math
+import operator
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import Dict, List, Mapping, Optional, Sequence, Tuple
 
+import numpy as np
 import torch
 
 from ..csrc import bindings as B
@@ -24,9 +26,14 @@ class SamplingError(ValueError):
 
 @dataclass(frozen=True)
 class SamplingParams:
-    """temperature 0 = greedy; > 0 = temperature sampling with `seed`."""
+    """temperature 0 = greedy; > 0 = temperature sampling with `seed`.  The penalties and biases are the rules above; `logit_bias` maps
+    ids to what is added to their logits (finite, or -infinity)."""
     temperature: float = 0.0
     seed: int = 0
+    repetition_penalty: float = 1.0
+    presence_penalty: float = 0.0
+    frequency_penalty: float = 0.0
+    logit_bias: Tuple[Tuple[int, float], ...] = ()
 
     def __post_init__(self):
         t = self.temperature
@@ -34,10 +41,60 @@ class SamplingParams:
             raise SamplingError(f"temperature must be finite and >= 0 (0 = greedy), got {t!r}")
         if isinstance(self.seed, bool) or not isinstance(self.seed, int) or not 0 <= self.seed < 2 ** 64:
             raise SamplingError(f"seed must be an integer in [0, 2^64), got {self.seed!r}")
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            v = getattr(self, name)
+            if isinstance(v, bool) or not isinstance(v, (int, float)) or not math.isfinite(v) or (name == "repetition_penalty" and v <= 0):
+                raise SamplingError(f"{name} must be finite{' and positive' if name == 'repetition_penalty' else ''}, got {v!r}")
+        bias = self.logit_bias
+        if bias is None:
+            bias = ()
+        pairs = []
+        for pair in bias.items() if isinstance(bias, Mapping) else bias:
+            try:
+                i, b = pair
+                i, b = operator.index(i), float(b)
+            except (TypeError, ValueError):
+                raise SamplingError(f"logit_bias maps token ids to numbers, got {pair!r}") from None
+            if i < 0 or math.isnan(b) or b == math.inf:
+                raise SamplingError(f"logit_bias: id {i} must be >= 0 and its bias finite or -infinity, got {b!r}")
+            pairs.append((i, b))
+        if len({i for i, _ in pairs}) != len(pairs):
+            raise SamplingError("logit_bias: an id appears twice")
+        object.__setattr__(self, "logit_bias", tuple(pairs))
 
     @property
     def greedy(self) -> bool:
         return self.temperature == 0
+
+    @property
+    def penalized(self) -> bool:
+        return self.repetition_penalty != 1 or self.presence_penalty != 0 or self.frequency_penalty != 0
+
+
+def pack_allowed(allowed: Sequence, vocab: int) -> np.ndarray:
+    """One row of bits per entry (int32 [rows, ceil(vocab / 32)], bit i % 32 of word i // 32): None = every id, a sequence of ids, or a
+    boolean array of the vocabulary's length."""
+    words = -(-vocab // 32)
+    out = np.empty((len(allowed), words), dtype=np.uint32)
+    for r, a in enumerate(allowed):
+        if a is None:
+            out[r] = 0xFFFFFFFF
+            continue
+        a = a.cpu().numpy() if isinstance(a, torch.Tensor) else np.asarray(list(a) if not isinstance(a, np.ndarray) else a)
+        full = np.zeros(words * 32, dtype=bool)
+        if a.dtype == bool:
+            if a.shape != (vocab,):
+                raise SamplingError(f"a mask of allowed tokens must have the vocabulary's length ({vocab}), got {a.shape}")
+            full[:vocab] = a
+        else:
+            if a.size and (a.ndim != 1 or a.dtype.kind not in "iu" or a.min() < 0 or a.max() >= vocab):
+                raise SamplingError(f"allowed tokens must be ids in [0, {vocab})")
+            if a.size:
+                full[a] = True
+        if not full.any():
+            raise SamplingError("no token is allowed")
+        out[r] = np.packbits(full.reshape(words, 32), axis=1, bitorder="little").view(np.uint32).reshape(words)
+    return out.view(np.int32)
 
 
 class Sampler:
@@ -54,10 +111,61 @@ class Sampler:
         self._ctr_host: List[Optional[torch.Tensor]] = [None] * 4
         self._ctr_events: list = [None] * 4
         self._ctr_turn = 0
+        self._bias: Optional[torch.Tensor] = None
+        # the running batch's histories, one row per request: ids, lengths, prompt lengths and penalties on the device
+        self._row_of: Dict[int, int] = {}
+        self._history = self._lens = self._prompt_lens = self._penalties = None
+
+    def begin(self, request_ids: Sequence[int], prompts: Sequence[Sequence[int]], max_new_tokens: int) -> None:
+        """Start the histories of a batch (penalties look at the prompt too); those of the batch before are dropped."""
+        if not self.params.penalized:
+            return
+        if len(set(request_ids)) != len(request_ids):
+            raise SamplingError("penalties need a different id for every request of a batch")
+        self._row_of = {r: i for i, r in enumerate(request_ids)}
+        n, width = len(prompts), max((len(p) for p in prompts), default=0) + max(max_new_tokens, 0) + 1
+        p, device = self.params, self.err.device
+        host = np.full((n, width), -1, dtype=np.int32)
+        for i, ids in enumerate(prompts):
+            host[i, :len(ids)] = ids
+        self._history = torch.from_numpy(host).to(device)
+        self._lens = torch.tensor([len(x) for x in prompts], dtype=torch.int32, device=device)
+        self._prompt_lens = self._lens.clone()
+        self._penalties = torch.tensor([[p.repetition_penalty, p.presence_penalty, p.frequency_penalty]] * n, dtype=torch.float32, device=device)
+
+    def _rules(self, logits: torch.Tensor, request_ids: Sequence[int], allowed) -> Optional[dict]:
+        """What `logit_rules` takes for these rows; None where the params ask for nothing."""
+        p, vocab = self.params, logits.shape[1]
+        if not p.penalized and not p.logit_bias and allowed is None:
+            return None
+        kw = {"history": None, "lens": None, "prompt_lens": None, "rows": None}
+        if p.logit_bias:
+            if self._bias is None or self._bias.shape[0] != vocab or self._bias.device != logits.device:
+                if max(i for i, _ in p.logit_bias) >= vocab:
+                    raise SamplingError(f"logit_bias: id {max(i for i, _ in p.logit_bias)} is outside the vocabulary [0, {vocab})")
+                bias = np.zeros(vocab, dtype=np.float32)
+                for i, b in p.logit_bias:
+                    bias[i] = b
+                self._bias = torch.from_numpy(bias).to(logits.device)
+            kw["bias"] = self._bias
+        if allowed is not None:
+            if len(allowed) != logits.shape[0]:
+                raise SamplingError("one entry of allowed tokens per row is needed")
+            kw["mask"] = torch.from_numpy(pack_allowed(allowed, vocab)).to(logits.device)
+        if p.penalized:
+            missing = [r for r in request_ids if r not in self._row_of]
+            if len(request_ids) != logits.shape[0] or missing or len(set(request_ids)) != len(request_ids):
+                raise SamplingError("penalties need the batch's prompts (begin()) and one different request per row"
+                                    + (f"; unknown: {missing}" if missing else ""))
+            rows = self._counters_to_device([self._row_of[r] for r in request_ids], request_ids, logits.device)[0]
+            kw.update(history=self._history, lens=self._lens, prompt_lens=self._prompt_lens, rows=rows, penalties=self._penalties)
+        return kw
 
     def sample_device(self, logits: torch.Tensor, request_ids: Sequence[int],
-                      steps: Sequence[int]) -> torch.Tensor:
-        """int32 [rows] on the device.  `request_ids[i]`, `steps[i]`: the Philox counter of row i."""
+                      steps: Sequence[int], allowed: Optional[Sequence] = None) -> torch.Tensor:
+        """int32 [rows] on the device.  `request_ids[i]`, `steps[i]`: the Philox counter of row i.  With penalties the rows are those
+        of requests that `begin` has been told of, and each choice joins its request's history.  `allowed`: for each row the ids
+        that may be chosen (a sequence of ids, a boolean array of the vocabulary, or None: all)."""
         rows = logits.shape[0]
         if logits.dim() != 2 or rows == 0 or logits.shape[1] == 0:
             raise SamplingError("logits are empty")          # src/engine/sampling.rs:58-60
@@ -65,7 +173,19 @@ class Sampler:
             raise SamplingError(f"logits must be float32, got {logits.dtype}")
         out = torch.empty(rows, dtype=torch.int32, device=logits.device)
         stream = B.stream_ptr()
-        if self.params.greedy:
+        rules = self._rules(logits, request_ids, allowed)
+        if rules is not None and self.params.greedy:
+            B.logit_rules(logits, None, err=self.err, stream=stream, chosen=out, lens_out=rules["lens"], **rules)
+        elif rules is not None:
+            if len(request_ids) != rows or len(steps) != rows:
+                raise SamplingError("one request id and one step per row are needed")
+            ruled = torch.empty((rows, logits.shape[1]), dtype=torch.float32, device=logits.device)
+            B.logit_rules(logits, ruled, err=self.err, stream=stream, **rules)
+            ctr = self._counters_to_device(request_ids, steps, logits.device)
+            B.sample_temperature_masked(ruled, float(self.params.temperature), self.params.seed, ctr[0], ctr[1], out, self.err, stream)
+            if rules["history"] is not None:
+                B.history_append(rules["history"], rules["lens"], rules["rows"], out, self.err, stream)
+        elif self.params.greedy:
             B.sample_greedy(logits, out, self.err, stream)
         else:
             if len(request_ids) != rows or len(steps) != rows:
@@ -116,9 +236,10 @@ class Sampler:
         ev.record()
         return PendingTokens(self, buf, rows, ev)
 
-    def __call__(self, logits: torch.Tensor, request_ids: Sequence[int], steps: Sequence[int]) -> List[int]:
+    def __call__(self, logits: torch.Tensor, request_ids: Sequence[int], steps: Sequence[int],
+                 allowed: Optional[Sequence] = None) -> List[int]:
         """Host token ids (synchronises), after checking the device error word."""
-        return self.read_async(self.sample_device(logits, request_ids, steps)).wait()
+        return self.read_async(self.sample_device(logits, request_ids, steps, allowed)).wait()
 
 
 class PendingTokens:

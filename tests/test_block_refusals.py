@@ -97,8 +97,7 @@ def test_steps_refuse():
     view = B.block_view(**p, weight=weight)
     err = torch.zeros(1, dtype=torch.int32)
     good = torch.zeros(2, (4 + 4) * 16, dtype=torch.bfloat16)
-    out, scratch = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(2 * 4 * 8)
-    assert B.block_attention_scratch_floats(2, 4, view) == 64
+    out, scratch = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(B.block_attention_scratch_floats(2, 4, view))
 
     def step(**kw):
         a = dict(qkv=good, out=out, batch=batch(2, 2), heads=4, scratch=scratch)
@@ -106,7 +105,7 @@ def test_steps_refuse():
         B.block_attention(a["qkv"], a["out"], a["batch"], view, a["heads"], 1.0, a["scratch"], err, 0, weight_out=a.get("weight_out"))
     for kw, says in [(dict(qkv=good.float()), "of the tails' type"), (dict(qkv=good[:, :-1]), "projection must be"), (dict(batch=batch(2, 3)), "one row per"),
                      (dict(batch=batch(3, 3)), "one row per"), (dict(heads=3, qkv=torch.zeros(2, 7 * 16, dtype=torch.bfloat16)), "multiple of kv_heads"),
-                     (dict(out=out[:1]), "out must be"), (dict(out=out.float()), "out must be"), ({}, "on one CUDA device")]:
+                     (dict(out=out[:1]), "out must be"), (dict(out=out.float()), "out must be"), (dict(scratch=scratch[1:]), "scratch is too small"), ({}, "on one CUDA device")]:
         with pytest.raises(B.KernelError, match=says):
             step(**kw)
     with pytest.raises(B.KernelError, match="fewer rows"):

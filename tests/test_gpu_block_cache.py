@@ -95,7 +95,7 @@ class Rig:
                 assert torch.equal(t[s, :, :n - done * BLOCK].double().cpu(), want.double()), (s, i)
         assert self.err.item() == 0
 
-    def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, scale=None, spread=1.0, check=True, scratch=None):
+    def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, warps=0, scale=None, spread=1.0, check=True, scratch=None):
         """One token for each of `slots`; compares with 64 bits and returns the outputs."""
         b = B()
         scale = self.D ** -0.5 if scale is None else scale
@@ -109,7 +109,7 @@ class Rig:
         if scratch is None:
             scratch = torch.full((b.block_attention_scratch_floats(len(slots) + pad, self.H, self.view),), float("nan"), device=DEV)
         b.block_attention(full, out, view, self.view, self.H, scale, scratch, self.err, b.stream_ptr(), weight_out=weight_out, plain=plain,
-                          splits=splits)
+                          splits=splits, warps=warps)
         torch.cuda.synchronize()
         assert (out[-1] == 7).all(), "a row behind the last sequence was written"
         assert (out[len(slots):-1] == 0).all(), "padding sequences"
@@ -220,9 +220,10 @@ def test_one_token_steps(plain, fmt, dtype, G, H, D):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
+@pytest.mark.parametrize("warps", [4, 8, 16])
 @pytest.mark.parametrize("D", [64, 128])
-def test_a_key_head_shared_by_ctas(fmt, splits, D):
-    """Long and short sequences, more CTAs than blocks among them, more than 32 blocks for a warp."""
+def test_a_key_head_shared_by_ctas(fmt, splits, warps, D):
+    """Long and short sequences, more CTAs than blocks among them, more than 64 blocks for a warp."""
     lens = [0, 5, 16, 40, 100, 1023, 2500, 16 * 32 * 4 * 2 + 17]
     r = Rig(1, 5, D, fmt, torch.bfloat16, n_slots=8, width=66, weights=True, seed=splits)
     slots = [3, 1, 0, 7, 2, 5, 6, 4]
@@ -230,8 +231,8 @@ def test_a_key_head_shared_by_ctas(fmt, splits, D):
     r.store([s for s, _ in live], [x for _, x in live])
     for s, x in live:
         r.blocks_weight[s] = [torch.zeros(1, dtype=torch.float64) for _ in range(-(-x // BLOCK))]
-    for _ in range(2):
-        r.step(slots, plain=False, splits=splits)
+    for pad in (0, 8):
+        r.step(slots, plain=False, splits=splits, warps=warps, pad=pad)
     r.check_content(slots)
 
 
@@ -300,7 +301,8 @@ def test_rotation_inside_the_kernel(plain, D, pairing):
             out = torch.empty(3, 4 * D, device=DEV)
             if not fused:
                 b.rotate_qk(x, where, inv, 4, 2, D, rot, pairing, r.err, b.stream_ptr(), rot_mul=1.25)
-            b.block_attention(x, out, view, r.view, 4, D ** -0.5, None, r.err, b.stream_ptr(), rope=(inv, rot, pairing, 1.25) if fused else None, plain=plain)
+            scratch = torch.empty(b.block_attention_scratch_floats(3, 4, r.view), device=DEV)
+            b.block_attention(x, out, view, r.view, 4, D ** -0.5, scratch, r.err, b.stream_ptr(), rope=(inv, rot, pairing, 1.25) if fused else None, plain=plain)
             outs.append(out)
         # the same rotation in fp32 (contracted or not: two roundings of a sum of two products) before the same sums
         assert (outs[0] - outs[1]).abs().max().item() <= 1e-4
