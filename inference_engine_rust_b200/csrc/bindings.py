@@ -446,6 +446,10 @@ def _on_current_device(*tensors) -> None:
         raise KernelError(f"the tensors are on cuda:{here}, which is not the current device")
 
 
+def _int_row(t, n: int) -> bool:
+    return t is not None and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)
+
+
 def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, penalties=None, bias=None, mask=None, chosen=None,
                 lens_out=None) -> None:
     """Penalties for repeated tokens, biases and a mask on logits fp32 [R, vocab] (any row stride), and the best token left.
@@ -461,39 +465,47 @@ def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, p
     chosen       int32 [R]: the id of the largest result, the lowest of equal ones; 0 and an error bit where nothing is left
     lens_out     int32 [H] (may be `lens`): the choice is appended to its history and the length plus one is written here
     """
-    _need(logits.dim() == 2 and logits.dtype == torch.float32 and logits.stride(1) == 1, "logits must be float32 [rows, vocab] with contiguous rows")
+    i32, f32 = torch.int32, torch.float32
+    if logits.dim() != 2 or logits.dtype != f32 or logits.stride(1) != 1:
+        raise KernelError("logits must be float32 [rows, vocab] with contiguous rows")
     R, vocab = logits.shape
-    if out is not None:
-        _need(out.shape == logits.shape and out.dtype == torch.float32 and out.stride(1) == 1, "out must be float32 like logits")
+    if out is not None and (out.shape != logits.shape or out.dtype != f32 or out.stride(1) != 1):
+        raise KernelError("out must be float32 like logits")
     H = width = 0
     if history is not None:
-        _need(history.dim() == 2 and history.dtype == torch.int32 and history.is_contiguous(), "history must be contiguous int32 [histories, width]")
+        if history.dim() != 2 or history.dtype != i32 or not history.is_contiguous():
+            raise KernelError("history must be contiguous int32 [histories, width]")
         H, width = history.shape
-        for t, name in ((lens, "lens"), (prompt_lens, "prompt_lens")):
-            _need(t is not None and t.dtype == torch.int32 and t.shape == (H,) and t.is_contiguous(), f"{name} must be int32 [{H}]")
-        _need(rows is None or (rows.dtype == torch.int32 and rows.shape == (R,) and rows.is_contiguous()), f"rows must be int32 [{R}]")
-        _need(lens_out is None or (lens_out.dtype == torch.int32 and lens_out.shape == (H,) and lens_out.is_contiguous()), f"lens_out must be int32 [{H}]")
-        _need(lens_out is None or chosen is not None, "lens_out needs chosen")
+        if not _int_row(lens, H):
+            raise KernelError(f"lens must be int32 [{H}]")
+        if not _int_row(prompt_lens, H):
+            raise KernelError(f"prompt_lens must be int32 [{H}]")
+        if rows is not None and not _int_row(rows, R):
+            raise KernelError(f"rows must be int32 [{R}]")
+        if lens_out is not None and (chosen is None or not _int_row(lens_out, H)):
+            raise KernelError("lens_out needs chosen" if chosen is None else f"lens_out must be int32 [{H}]")
+    elif penalties is not None or lens_out is not None:
+        raise KernelError("penalties and lens_out need a history")
     else:
-        _need(penalties is None and lens_out is None, "penalties and lens_out need a history")
-    _need(penalties is None or (penalties.dtype == torch.float32 and penalties.shape == (H, 3) and penalties.is_contiguous()),
-          f"penalties must be float32 [{H}, 3]")
+        lens = prompt_lens = rows = None
+    if penalties is not None and (penalties.dtype != f32 or penalties.shape != (H, 3) or not penalties.is_contiguous()):
+        raise KernelError(f"penalties must be float32 [{H}, 3]")
     ld_bias = ld_mask = 0
     if bias is not None:
-        _need(bias.dtype == torch.float32 and bias.stride(-1) == 1 and (bias.shape == (vocab,) or bias.shape == (R, vocab)),
-              "bias must be float32 [vocab] or [rows, vocab]")
+        if bias.dtype != f32 or bias.shape[-1] != vocab or bias.stride(-1) != 1 or not (bias.dim() == 1 or bias.shape == (R, vocab)):
+            raise KernelError("bias must be float32 [vocab] or [rows, vocab]")
         ld_bias = bias.stride(0) if bias.dim() == 2 else 0
     if mask is not None:
         words = -(-vocab // 32)
-        _need(mask.dtype == torch.int32 and mask.dim() == 2 and mask.shape[1] == words and mask.shape[0] in (1, R) and mask.stride(1) == 1,
-              f"mask must be int32 [rows or 1, {words}]")
+        if mask.dtype != i32 or mask.dim() != 2 or mask.shape[1] != words or mask.shape[0] not in (1, R) or mask.stride(1) != 1:
+            raise KernelError(f"mask must be int32 [rows or 1, {words}]")
         ld_mask = mask.stride(0) if mask.shape[0] == R and R > 1 else 0
-    _need(chosen is None or (chosen.dtype == torch.int32 and chosen.shape == (R,) and chosen.is_contiguous()), f"chosen must be int32 [{R}]")
+    if chosen is not None and not _int_row(chosen, R):
+        raise KernelError(f"chosen must be int32 [{R}]")
     _on_current_device(logits, out, history, lens, prompt_lens, rows, penalties, bias, mask, chosen, lens_out, err)
     check(core().iert_logit_rules(logits.data_ptr(), R, vocab, logits.stride(0), _ptr(out), out.stride(0) if out is not None else 0,
-                                  _ptr(history), width, H, _ptr(lens) if H else None, _ptr(prompt_lens) if H else None, _ptr(rows) if H else None,
-                                  _ptr(penalties), _ptr(bias), ld_bias, _ptr(mask), ld_mask, _ptr(chosen), _ptr(lens_out), err.data_ptr(), stream),
-          "logit_rules")
+                                  _ptr(history), width, H, _ptr(lens), _ptr(prompt_lens), _ptr(rows), _ptr(penalties), _ptr(bias), ld_bias,
+                                  _ptr(mask), ld_mask, _ptr(chosen), _ptr(lens_out), err.data_ptr(), stream), "logit_rules")
 
 
 def history_append(history, lens, rows, tokens, err, stream) -> None:
@@ -1272,9 +1284,9 @@ def block_view(k, v, k_scale, v_scale, tail_k, tail_v, page_table, *, window: in
 
 
 def _packed_rows(qkv, heads: int, view: BlockView) -> None:
-    _need(qkv.dim() == 2 and qkv.is_contiguous() and dtype_code(qkv.dtype) == view.tail_dtype
-          and qkv.shape[1] == (heads + 2 * view.kv_heads) * view.head_dim,
-          "the projection must be contiguous [tokens, (heads + 2 kv_heads) * head_dim] of the tails' type")
+    if (qkv.dim() != 2 or not qkv.is_contiguous() or qkv.dtype != view.tensors[4].dtype
+            or qkv.shape[1] != (heads + 2 * view.kv_heads) * view.head_dim):
+        raise KernelError("the projection must be contiguous [tokens, (heads + 2 kv_heads) * head_dim] of the tails' type")
 
 
 def block_store(qkv, batch: BatchView, view: BlockView, heads: int, err, stream) -> None:
@@ -1303,12 +1315,19 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     splits       CTAs that share a sequence's kv head (1, 2, 4, 8, 16), of `warps` (4, 8, 16) each; 0: by the kernel's own rule
     """
     _packed_rows(qkv, heads, view)
-    _need(batch.n_tokens == batch.n_seqs and qkv.shape[0] >= batch.n_seqs, "a one-token step has one row per sequence")
-    _need(heads % view.kv_heads == 0, f"heads {heads} is not a multiple of kv_heads {view.kv_heads}")
-    _need(out.dtype == qkv.dtype and out.is_contiguous() and out.numel() >= batch.n_seqs * heads * view.head_dim, "out must be [sequences, heads * head_dim]")
-    _need(scratch.dtype == torch.float32 and scratch.numel() >= block_attention_scratch_floats(batch.n_seqs, heads, view), "scratch is too small")
-    _need(weight_out is None or (view.weight is not None and weight_out.dtype == torch.float32 and weight_out.is_contiguous()
-                                 and weight_out.shape == view.tensors[7].shape), "weight_out must be laid out as the view's weight")
+    n = batch.n_seqs
+    if batch.n_tokens != n or qkv.shape[0] < n:
+        raise KernelError("a one-token step has one row per sequence")
+    if heads % view.kv_heads:
+        raise KernelError(f"heads {heads} is not a multiple of kv_heads {view.kv_heads}")
+    if out.dtype != qkv.dtype or not out.is_contiguous() or out.numel() < n * heads * view.head_dim:
+        raise KernelError("out must be [sequences, heads * head_dim]")
+    if scratch.dtype != torch.float32 or scratch.numel() < block_attention_scratch_floats(n, heads, view):
+        raise KernelError("scratch is too small")
+    weight = view.tensors[7]
+    if weight_out is not None and (weight is None or weight_out.dtype != torch.float32 or not weight_out.is_contiguous()
+                                   or weight_out.shape != weight.shape):
+        raise KernelError("weight_out must be laid out as the view's weight")
     _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
     weights = weight_out.data_ptr() if weight_out is not None else view.weight
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
