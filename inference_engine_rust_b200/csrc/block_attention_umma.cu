@@ -1,0 +1,651 @@
+// One-token attention over the 8-bit cache (block_cache.cuh) on the 5th-generation tensor cores: int8 levels, heads of 128, up to eight
+// query heads to a key head.  (block_attention_tc.cu has the other forms.)
+//
+// tcgen05.mma multiplies 8-bit integers as they stand in shared memory, so no level is ever converted; the other operand is a
+// number written in 8-bit digits, a column of the product per digit, and sums of 32-bit integers are exact:
+//   S [128 positions x 32] = K [128 x 128] Q^T     Q: a head's query as fixed-point numbers, DIG signed digits of 7 bits (base 128)
+//   O [128 dimensions x 32] += V^T [128 x 128] P   P: a head's probabilities as 32-bit fixed-point numbers, four unsigned digits of 8 bits
+// A tile is eight blocks of 16 positions of a (sequence, kv head), keys row by row (K-major), the values' tile read with its columns as
+// rows (MN-major).  Every position is one thread of the softmax, which needs about 210 instructions a warp and tile (mma.sync with
+// its conversions: 3,100 for the same 128 positions): what remains is the stream of levels.
+//   warps 0-3  softmax, a position per thread: a head's score from its digits, times the block's key scale; the probability times the
+//              block's value scale, as digits, into (swizzled) shared memory.  The references (a maximum per head, a largest value scale) move
+//              only where a fixed-point number would pass 2^31; O is then read out, added up in registers and begun again.
+//   warp 4     TMA producer: page numbers and scales of 32 blocks at a time, one per lane; boxes of 16 positions into a ring of two tiles.
+//   warp 5     MMA issuer: the scores of the next tile, then the weighted sum of this one.
+// A cluster of up to 16 CTAs shares a (sequence, kv head): each takes a run of its blocks and adds up a share of the outputs from what
+// the others have put into its shared memory.  The unfinished block, up to 16 rows in the run's type, is done in fp32 by the cluster's
+// last CTA, which also stores the step's own key and value and turns the block into levels when it is full.
+// Queries as fixed-point numbers: bfloat16 runs 20 bits below the row's largest (three digits), float32 runs 27 (four); probabilities 25 bits below
+// the reference, which is at least 2^-6 of the largest.
+// Every wait is bounded; on expiry the kernel records IERT_ERR_WAIT_EXPIRED, waits (bounded) for its copies and MMAs, frees its TMEM
+// and returns.
+#include <cooperative_groups.h>
+
+#include <utility>
+
+#include "block_cache.cuh"
+#include "sm100.cuh"
+#include "tma_host.cuh"
+
+namespace cg = cooperative_groups;
+using namespace iert;
+using namespace sm100;
+
+namespace {
+
+constexpr int HD = 128, TILE = 128, TILE_BLOCKS = TILE / BLK, GH = 8, NSTAGE = 2, SOFT = 128, THREADS = 192, MAX_SPLITS = 16;
+constexpr int TILE_BYTES = TILE * HD, BOX_BYTES = BLK * HD, NCOL = 32;
+constexpr int SLOTS = 2 * NSTAGE;              // of the tiles' scales: the softmax reads a tile's after its stage may be filled again
+constexpr uint32_t TMEM_COLS = 128;            // S twice, O
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+constexpr int P_BITS = 25;                     // a probability of 1 (times the largest value scale) is 2^25; 2^31 is the bound
+constexpr int MAX_RUN = 256;                   // tiles that O adds up at most: 255 * 127 * 128 * 256 < 2^31
+constexpr int TAIL_BLOCKS = 16;                // finished blocks that cost a CTA about as much time as the unfinished one
+
+struct UmmaParams {
+  const void* qkv;
+  void* out;
+  float* part;                 // [T][kv_heads][blocks][8]: base-2 logarithm of a block's unnormalised weight
+  float* weight_out;
+  int heads, blocks;
+  float scale_log2e;
+  const float* inv_freq;
+  int rope, rotary_dim, pairing;
+  float rot_mul;
+  int* err;
+};
+
+template <typename T> struct __align__(1024) Shared {
+  uint8_t ring[NSTAGE][2][TILE_BYTES];          // keys, values: rows of 128 bytes, 128-byte swizzle
+  uint8_t qd[NCOL * HD];                         // digits of the queries: row 8 j + h is digit j of head h
+  uint8_t pd[2][NCOL * TILE];                    // digits of the probabilities, likewise
+  float q[GH][HD + 4];
+  float o[GH][HD];                               // this CTA's finished blocks
+  T tail[2][BLK][HD];
+  float cs[HD];
+  float tail_s[BLK][GH];
+  float tail_o[GH][HD];
+  float o_in[GH * HD + MAX_SPLITS];              // this CTA's share of the outputs, from every CTA of the cluster
+  float ml_in[MAX_SPLITS][GH][2];
+  float fac[MAX_SPLITS][GH];
+  float ml[2][GH][2];                            // maximum and sum: finished blocks, unfinished block
+  float lse[GH][2];
+  float rs[GH];                                  // what makes scores of the integers
+  float top[4][GH];
+  float sum[4][GH];
+  float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there: key scale NaN of its own kind (see NOWHERE)
+  uint32_t red[THREADS / 32];
+  uint64_t k_full[NSTAGE], v_full[NSTAGE], k_empty[NSTAGE], v_empty[NSTAGE], s_full[2], s_empty[2], p_ready[2], pv_done[2], drained;
+  uint32_t tmem;
+  int restart[2];
+  int asked_k, asked_v;
+  int abort_flag;
+};
+constexpr uint32_t NOWHERE = 0x7fc0beefu;        // the key scale of a block that counts for nothing (no division gives this pattern)
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *abort_flag) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ void mma_i8(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
+}
+// s8 x (s8 or u8) -> s32, M x N; A MN-major on request, B K-major.
+__host__ __device__ constexpr uint32_t instr_desc_i8(uint32_t M, uint32_t N, uint32_t b_signed, uint32_t a_mn) {
+  return (2u << 4) | (1u << 7) | (b_signed << 10) | (a_mn << 15) | ((N >> 3) << 17) | ((M >> 4) << 24);
+}
+__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory"); }
+// The same for the softmax and the MMA warp.
+__device__ __forceinline__ void early_sync() { asm volatile("bar.sync 2, %0;" ::"n"(SOFT + 32) : "memory"); }
+__device__ __forceinline__ bool soft_any(bool x) {
+  int y;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+               : "=r"(y) : "r"((int)x), "n"(SOFT) : "memory");
+  return y != 0;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld16_issue(taddr, r);
+  tmem_ld16_issue(taddr + 16, r + 16);
+  tmem_ld_wait();
+}
+
+template <typename T>
+__device__ __forceinline__ float head_value(const T* src, int d, const UmmaParams& p, const float* cs) {
+  const float x = to_f32(src[d]);
+  if (!p.rope || d >= p.rotary_dim) return x;
+  const int half = p.rotary_dim / 2;
+  const bool second = p.pairing == IERT_PAIR_HALF ? d >= half : d & 1;
+  const int k = p.pairing == IERT_PAIR_HALF ? (second ? d - half : d) : d >> 1;
+  const float y = to_f32(src[p.pairing == IERT_PAIR_HALF ? (second ? d - half : d + half) : d ^ 1]);
+  return to_f32(from_f32<T>(second ? y * cs[half + k] + x * cs[k] : x * cs[k] - y * cs[half + k]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 2)
+block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, UmmaParams p, IertBatchView b,
+                            IertBlockView c) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];        // no static shared memory: the window starts 1024-byte aligned
+  Shared<T>& sm = *reinterpret_cast<Shared<T>*>(smem_raw);
+  constexpr int DIG = sizeof(T) == 4 ? 4 : 3;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int S = gridDim.x, rank = blockIdx.x;                  // the cluster is the grid's first axis
+  const int kvh = blockIdx.y, t = blockIdx.z, n_g = p.heads / c.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int s = sequence_of_token(b, t);
+  int slot = block_slot(c, b, s, p.err);
+  if (slot >= 0 && !block_reaches(c, b.pos0[s], p.err)) slot = -1;
+  T* out = (T*)p.out + ((size_t)t * p.heads + (size_t)kvh * n_g) * HD;
+  if (slot < 0) {                                              // (the same for the whole cluster)
+    pdl_launch_dependents();
+    pdl_wait();
+    if (rank == 0)
+      for (int i = tid; i < n_g * HD; i += THREADS) out[i] = from_f32<T>(0.f);
+    return;
+  }
+  if (smem_addr(smem_raw) & 1023u) {                           // never expected; refuse rather than compute garbage
+    if (tid == 0) atomicOr(p.err, IERT_ERR_WAIT_EXPIRED);
+    return;
+  }
+  cg::cluster_group::arrival_token started = cluster.barrier_arrive();
+  const int pos = b.pos0[s], nb = pos / BLK, base = nb * BLK, per_page = c.page_tokens / BLK;
+  const int j_min = iert_first_visible(pos, c.window, 0), b_lo = min(j_min / BLK, nb);
+  const int per = (nb - b_lo + (S > 1 ? TAIL_BLOCKS : 0) + S - 1) / S;
+  const int lo = min(nb, b_lo + rank * per), hi = min(nb, lo + per);
+  const int n_tiles = (hi - lo + TILE_BLOCKS - 1) / TILE_BLOCKS;
+  const bool owner = rank == S - 1;                            // of the unfinished block
+  const T* row = (const T*)p.qkv + (size_t)t * (size_t)(p.heads + 2 * c.kv_heads) * HD;
+  volatile int* abort_flag = &sm.abort_flag;
+  if (tid == 0) {
+    for (int i = 0; i < NSTAGE; ++i) { mbar_init(&sm.k_full[i], 1); mbar_init(&sm.v_full[i], 1); mbar_init(&sm.k_empty[i], 1); mbar_init(&sm.v_empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.s_empty[i], SOFT); mbar_init(&sm.p_ready[i], SOFT); mbar_init(&sm.pv_done[i], 1); }
+    mbar_init(&sm.drained, 1);
+    sm.abort_flag = 0; sm.asked_k = 0; sm.asked_v = 0;
+    mbar_fence_init();
+  }
+  if (warp == 5) tmem_alloc(&sm.tmem, TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();                                     // (a later kernel must not take the TMEM this CTA waits for)
+  const uint32_t tmem = sm.tmem, o_col = 2 * NCOL;
+  bool ok = true;
+  pdl_wait();
+
+  if (warp == 4) {
+    // ---------------- TMA producer ----------------
+    if (lane == 0) { tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v); }
+    for (int i0 = 0; i0 < n_tiles && ok; i0 += 32 / TILE_BLOCKS) {
+      const int x = lo + i0 * TILE_BLOCKS + lane;
+      int at = -1;
+      float ks = __uint_as_float(NOWHERE), vs = 0.f;
+      if (x < hi) {
+        const int page = block_page(c, slot, x / per_page, p.err);
+        if (page >= 0) {
+          at = (page * c.kv_heads + kvh) * per_page + x % per_page;
+          ks = c.k_scale[at];
+          vs = c.v_scale[at];
+        }
+      }
+      for (int k = 0; k < 32 / TILE_BLOCKS && i0 + k < n_tiles && ok; ++k) {
+        const int i = i0 + k, st = i % NSTAGE;
+        const uint32_t again = ((i / NSTAGE) - 1) & 1;
+        const unsigned here = (__ballot_sync(0xffffffffu, at >= 0) >> (k * TILE_BLOCKS)) & 0xffu;
+        if (i >= NSTAGE) ok = wait_bar(&sm.k_empty[st], again, abort_flag);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        if ((lane >> 3) == k) sm.scale[i % SLOTS][lane & 7] = make_float2(ks, vs);
+        __syncwarp();
+        for (int kv = 0; kv < 2; ++kv) {
+          if (kv == 1 && i >= NSTAGE) {
+            ok = wait_bar(&sm.v_empty[st], again, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+          }
+          uint64_t* full = kv ? &sm.v_full[st] : &sm.k_full[st];
+          if (lane == 0) {
+            mbar_expect_tx(full, __popc(here) * BOX_BYTES);
+            if (kv) sm.asked_v = i + 1; else sm.asked_k = i + 1;
+          }
+          __syncwarp();
+          // a lane per block asks for its box: rows 16 (i & 7).. of the tile
+          if ((lane >> 3) == k && at >= 0) tma_load_2d(sm.ring[st][kv] + (lane & 7) * BOX_BYTES, kv ? &map_v : &map_k, full, 0, at * BLK);
+        }
+      }
+    }
+  } else {
+    // ---------------- the queries' digits (softmax and MMA warps) ----------------
+    const int me = warp == 5 ? SOFT + lane : tid;              // 0..159
+    constexpr int N = SOFT + 32;
+    if (p.rope) {
+      const float where = (float)(pos + (c.shift ? c.shift[slot] : 0));
+      for (int k = me; k < p.rotary_dim / 2; k += N) {
+        float sn, co;
+        sincosf(where * p.inv_freq[k], &sn, &co);
+        sm.cs[k] = co * p.rot_mul;
+        sm.cs[p.rotary_dim / 2 + k] = sn * p.rot_mul;
+      }
+      early_sync();
+    }
+    if (owner) {
+      const size_t off = ((size_t)slot * c.kv_heads + kvh) * BLK * HD;
+      T *tk = (T*)c.tail_k + off, *tv = (T*)c.tail_v + off;
+      const int old = (pos - base) * HD;
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll 2
+      for (int i = me * V; i < old; i += N * V) {
+        const uint4 x = *reinterpret_cast<const uint4*>(tk + i), y = *reinterpret_cast<const uint4*>(tv + i);
+        *reinterpret_cast<uint4*>(&sm.tail[0][0][0] + i) = x;
+        *reinterpret_cast<uint4*>(&sm.tail[1][0][0] + i) = y;
+      }
+      const T *kn = row + (size_t)(p.heads + kvh) * HD, *vn = row + (size_t)(p.heads + c.kv_heads + kvh) * HD;
+      for (int d = me; d < HD; d += N) {
+        const T x = from_f32<T>(head_value(kn, d, p, sm.cs)), v = vn[d];
+        sm.tail[0][pos - base][d] = x;
+        sm.tail[1][pos - base][d] = v;
+        tk[old + d] = x;
+        tv[old + d] = v;
+      }
+    }
+#pragma unroll 4
+    for (int i = me; i < GH * HD; i += N) {
+      const int r = i / HD, d = i % HD;
+      sm.q[r][d] = r < n_g ? head_value(row + (size_t)r * HD + (size_t)kvh * n_g * HD, d, p, sm.cs) : 0.f;
+    }
+    early_sync();
+    for (int h = warp == 5 ? 4 : warp; h < GH; h += 5) {       // a warp per head: four numbers a lane
+      const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][4 * lane]);
+      uint32_t largest = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      // scaled by a power of two: the row's largest number lies in [2^TOP, 2^(TOP + 1))
+      constexpr int TOP = DIG == 4 ? 26 : 19;
+      const int e = min(max((int)(largest >> 23), TOP + 1), 253);
+      const float f = __uint_as_float((uint32_t)(254 + TOP - e) << 23);
+      // (what is not a number reaches the scores through the scale that turns integers into them)
+      if (lane == 0) sm.rs[h] = (largest >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __uint_as_float((uint32_t)(e - TOP) << 23)) * p.scale_log2e;
+      const int v[4] = {__float2int_rn(x.x * f), __float2int_rn(x.y * f), __float2int_rn(x.z * f), __float2int_rn(x.w * f)};
+      uint32_t dig[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        int y = v[k];
+#pragma unroll
+        for (int j = DIG - 1; j > 0; --j) {                    // the lowest digit stands last
+          const int d = ((y + 64) & 127) - 64;
+          dig[j] |= (uint32_t)(d & 255) << (8 * k);
+          y = (y - d) >> 7;
+        }
+        dig[0] |= (uint32_t)(y & 255) << (8 * k);
+      }
+#pragma unroll
+      for (int j = 0; j < DIG; ++j)
+        *reinterpret_cast<uint32_t*>(sm.qd + (8 * j + h) * HD + (((lane >> 2) ^ (h & 7)) << 4) + (lane & 3) * 4) = dig[j];
+    }
+    fence_proxy_async_smem();
+    early_sync();
+
+    if (warp == 5) {
+      // ---------------- MMA issuer (the whole warp, one lane of it acting) ----------------
+      constexpr uint32_t IDESC_S = instr_desc_i8(TILE, NCOL, 1, 0), IDESC_O = instr_desc_i8(HD, NCOL, 0, 1);
+      const uint32_t leader = elect_leader();
+      auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag)) != 0; };
+      auto scores = [&](int i) {
+        const int st = i % NSTAGE;
+        if (!warp_wait(&sm.k_full[st], (i / NSTAGE) & 1) || (i >= 2 && !warp_wait(&sm.s_empty[i & 1], ((i >> 1) - 1) & 1))) return false;
+        tc_fence_after();
+        const uint64_t kd = smem_desc_k128(smem_addr(sm.ring[st][0])), qd = smem_desc_k128(smem_addr(sm.qd));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + (i & 1) * NCOL, kd + k * 2, qd + k * 2, IDESC_S, k > 0);
+        mma_commit(leader, &sm.s_full[i & 1]);
+        mma_commit(leader, &sm.k_empty[st]);
+        return true;
+      };
+      ok = n_tiles == 0 || scores(0);
+      for (int i = 0; ok && i < n_tiles; ++i) {
+        const int st = i % NSTAGE;
+        if (i + 1 < n_tiles && !scores(i + 1)) { ok = false; break; }
+        if (!warp_wait(&sm.p_ready[i & 1], (i >> 1) & 1) || !warp_wait(&sm.v_full[st], (i / NSTAGE) & 1)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t more = *(volatile int*)&sm.restart[i & 1] ? 0u : 1u;
+        const uint64_t vd = smem_desc_mn128(smem_addr(sm.ring[st][1]), TILE_BYTES), pd = smem_desc_k128(smem_addr(sm.pd[i & 1]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + o_col, vd + k * (32 * HD >> 4), pd + k * 2, IDESC_O, k > 0 ? 1u : more);
+        mma_commit(leader, &sm.pv_done[i & 1]);
+        mma_commit(leader, &sm.v_empty[st]);
+      }
+      mma_commit(leader, &sm.drained);
+    } else {
+      // ---------------- the unfinished block, in fp32: a thread per (row, head), then per dimension ----------------
+      if (owner) {
+        const int r = tid >> 3, h = tid & 7;
+        float sc = -INFINITY;
+        if (base + r <= pos && base + r >= j_min) {
+          float dot = 0.f;
+#pragma unroll 8
+          for (int d = 0; d < HD; d += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][d]);
+            const T* k = &sm.tail[0][r][d];
+            dot = fmaf(x.x, to_f32(k[0]), dot); dot = fmaf(x.y, to_f32(k[1]), dot);
+            dot = fmaf(x.z, to_f32(k[2]), dot); dot = fmaf(x.w, to_f32(k[3]), dot);
+          }
+          sc = dot * p.scale_log2e;
+        }
+        sm.tail_s[r][h] = sc;
+        soft_sync();
+        float mx = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < BLK; ++i) mx = fmaxf(mx, sm.tail_s[i][h]);
+        const float pr = mx == -INFINITY ? (sc == sc ? 0.f : sc) : ex2(sc - mx);
+        soft_sync();
+        sm.tail_s[r][h] = pr;
+        soft_sync();
+        if (r == 0) {
+#pragma unroll
+          for (int i = 0; i < BLK; ++i) l += sm.tail_s[i][h];
+          sm.ml[1][h][0] = mx;
+          sm.ml[1][h][1] = l;
+          if (c.weight) p.part[(((size_t)t * c.kv_heads + kvh) * p.blocks + nb) * GH + h] = mx + log2f(l);
+        }
+        float acc[GH] = {};
+        for (int i = max(0, j_min - base); i <= pos - base; ++i) {
+          const float v = to_f32(sm.tail[1][i][tid]);
+#pragma unroll
+          for (int k = 0; k < GH; ++k) acc[k] = fmaf(sm.tail_s[i][k], v, acc[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < GH; ++k) sm.tail_o[k][tid] = acc[k];
+      }
+
+      // ---------------- softmax: position tid of a tile; dimension tid of O ----------------
+      const uint32_t lane_bits = (uint32_t)(warp * 32) << 16;
+      const int blk = tid >> 4;
+      float* part = c.weight ? p.part + ((size_t)t * c.kv_heads + kvh) * p.blocks * GH : nullptr;
+      float rs[GH], ref[GH], l[GH], acc[GH];
+#pragma unroll
+      for (int h = 0; h < GH; ++h) { rs[h] = sm.rs[h]; ref[h] = -INFINITY; l[h] = 0.f; acc[h] = 0.f; }
+      float v_ref = 0.f, v_inv = 0.f;              // the value scale that probabilities are relative to, and its inverse
+      int run = 0;                                 // tiles in O
+      // O of the tiles so far, in units of v_ref 2^-P_BITS, joins acc (dimension tid)
+      auto flush = [&](int i) {                    // i: the last tile in O
+        if (!wait_bar(&sm.pv_done[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t r[32];
+        tmem_ld32(tmem + lane_bits + o_col, r);
+        tc_fence_before();
+#pragma unroll
+        for (int h = 0; h < GH; ++h) {
+          const float hi2 = fmaf((float)(int)r[24 + h], 256.f, (float)(int)r[16 + h]), lo2 = fmaf((float)(int)r[8 + h], 256.f, (float)(int)r[h]);
+          acc[h] += fmaf(hi2, 65536.f, lo2);
+        }
+        run = 0;
+      };
+      for (int i = 0; i < n_tiles; ++i) {
+        if (!wait_bar(&sm.s_full[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t r[32];
+        tmem_ld32(tmem + lane_bits + (i & 1) * NCOL, r);
+        const float2 sc = sm.scale[i % SLOTS][blk];
+        tc_fence_before();
+        mbar_arrive(&sm.s_empty[i & 1]);
+        const int x = lo + i * TILE_BLOCKS + blk;
+        const bool there = __float_as_uint(sc.x) != NOWHERE && x * BLK + (tid & 15) >= j_min;
+        float v[GH], y[GH];
+#pragma unroll
+        for (int h = 0; h < GH; ++h) {
+          float f;
+          if (DIG == 4) f = fmaf((float)((int)r[h] * 128 + (int)r[8 + h]), 16384.f, (float)((int)r[16 + h] * 128 + (int)r[24 + h]));
+          else f = fmaf((float)((int)r[h] * 128 + (int)r[8 + h]), 128.f, (float)(int)r[16 + h]);
+          v[h] = there ? f * (sc.x * rs[h]) : -INFINITY;
+          y[h] = ex2(v[h] - ref[h]);
+        }
+        const float vu = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
+        bool far = !ok;
+#pragma unroll
+        for (int h = 0; h < GH; ++h) far |= !(y[h] * vu < 2147483648.f) || !(y[h] < 1e30f);
+        if (soft_any(far || run == MAX_RUN)) {       // (the same for all four warps)
+          if (soft_any(!ok)) { ok = false; break; }
+          // new references: the largest of the tile per head, the largest value scale; what was added up moves to them
+          if (run > 0) flush(i - 1);
+#pragma unroll
+          for (int h = 0; h < GH; ++h) {
+            float mx = v[h];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (lane == 0) sm.top[warp][h] = mx;
+          }
+          soft_sync();
+          float v_new = v_ref;
+#pragma unroll
+          for (int k = 0; k < TILE_BLOCKS; ++k) {
+            const float2 z = sm.scale[i % SLOTS][k];
+            if (__float_as_uint(z.x) != NOWHERE) v_new = fmaxf(v_new, z.y);
+          }
+          const float v_move = v_new > 0.f ? v_ref / v_new : 1.f;
+          v_ref = v_new;
+          v_inv = v_ref > 0.f ? 1.f / v_ref : 0.f;
+#pragma unroll
+          for (int h = 0; h < GH; ++h) {
+            const float to = fmaxf(ref[h], fmaxf(fmaxf(sm.top[0][h], sm.top[1][h]), fmaxf(sm.top[2][h], sm.top[3][h])));
+            const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
+            ref[h] = to;
+            l[h] *= alpha;
+            acc[h] *= alpha * v_move;
+            y[h] = v[h] == -INFINITY ? 0.f : ex2(v[h] - to);
+          }
+          soft_sync();                             // (sm.top may be written again)
+        }
+        const float unit = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
+        if (i >= 2 && !wait_bar(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, abort_flag)) ok = false;      // the buffer is free
+        uint8_t* pd = sm.pd[i & 1] + (tid & 15);
+#pragma unroll
+        for (int h = 0; h < GH; ++h) {
+          const float w = y[h] * unit;
+          l[h] = fmaf(w, 0.f, l[h] + y[h]);        // (a value scale that is no number makes the head's sum none)
+          const uint32_t z = __float2uint_rn(w);
+          uint8_t* at = pd + h * TILE + ((blk ^ h) << 4);
+          at[0] = (uint8_t)z;
+          at[8 * TILE] = (uint8_t)(z >> 8);
+          at[16 * TILE] = (uint8_t)(z >> 16);
+          at[24 * TILE] = (uint8_t)(z >> 24);
+        }
+        if (tid == 0) sm.restart[i & 1] = run == 0;
+        ++run;
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&sm.p_ready[i & 1]);
+        if (part) {
+          // sums over a block's 16 lanes, eight heads: halves of the heads are exchanged until a lane has one
+          float a4[4], a2[2];
+          const bool b8 = lane & 8, b4 = lane & 4, b2 = lane & 2;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) a4[h] = (b8 ? y[4 + h] : y[h]) + __shfl_xor_sync(0xffffffffu, b8 ? y[h] : y[4 + h], 8);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) a2[h] = (b4 ? a4[2 + h] : a4[h]) + __shfl_xor_sync(0xffffffffu, b4 ? a4[h] : a4[2 + h], 4);
+          float one = (b2 ? a2[1] : a2[0]) + __shfl_xor_sync(0xffffffffu, b2 ? a2[0] : a2[1], 2);
+          one += __shfl_xor_sync(0xffffffffu, one, 1);
+          const float r4[4] = {b8 ? ref[4] : ref[0], b8 ? ref[5] : ref[1], b8 ? ref[6] : ref[2], b8 ? ref[7] : ref[3]};
+          const float r2[2] = {b4 ? r4[2] : r4[0], b4 ? r4[3] : r4[1]};
+          if (!(lane & 1) && x < hi) part[(size_t)x * GH + (b8 ? 4 : 0) + (b4 ? 2 : 0) + (b2 ? 1 : 0)] = (b2 ? r2[1] : r2[0]) + log2f(one);
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok) != 0;
+      if (ok && run > 0) flush(n_tiles - 1);
+#pragma unroll
+      for (int h = 0; h < GH; ++h) {
+        sm.o[h][tid] = acc[h] * (v_ref * (1.f / (1 << P_BITS)));
+        float z = l[h];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        if (lane == 0) sm.sum[warp][h] = z;
+      }
+      if (tid == 0)
+#pragma unroll
+        for (int h = 0; h < GH; ++h) sm.ml[0][h][0] = ref[h];
+    }
+  }
+  if (!ok && lane == 0) {
+    atomicOr(p.err, IERT_ERR_WAIT_EXPIRED);
+    *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && tid == 0) {                   // copies and MMAs still on their way end before the memory is let go
+    mbar_wait(&sm.drained, 0, WAIT_LIMIT);
+    for (int st = 0; st < NSTAGE; ++st) {
+      if (sm.asked_k > st) mbar_wait(&sm.k_full[st], (((sm.asked_k - 1 - st) / NSTAGE)) & 1, WAIT_LIMIT);
+      if (sm.asked_v > st) mbar_wait(&sm.v_full[st], (((sm.asked_v - 1 - st) / NSTAGE)) & 1, WAIT_LIMIT);
+    }
+  }
+  if (tid < GH) sm.ml[0][tid][1] = (sm.sum[0][tid] + sm.sum[1][tid]) + (sm.sum[2][tid] + sm.sum[3][tid]);
+  cluster.barrier_wait(std::move(started));        // every CTA runs
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+
+  // ---- the CTA's partial result, finished blocks and the unfinished one, goes to the CTAs that add up its pieces
+  const int share = (n_g * HD + S - 1) / S;
+  auto merged = [&](int h, float& mm, float& f0, float& f1) {
+    const float m0 = sm.ml[0][h][0], m1 = owner ? sm.ml[1][h][0] : -INFINITY;
+    mm = fmaxf(m0, m1);
+    f0 = m0 == mm ? 1.f : ex2(m0 - mm);
+    f1 = !owner ? 0.f : m1 == mm ? 1.f : ex2(m1 - mm);
+  };
+  for (int i = tid; i < n_g * HD; i += THREADS) {
+    const int h = i / HD, d = i % HD, to = i / share;
+    float mm, f0, f1;
+    merged(h, mm, f0, f1);
+    const float x = f0 * sm.o[h][d] + (owner ? f1 * sm.tail_o[h][d] : 0.f);
+    cluster.map_shared_rank(&sm.o_in[0], to)[rank * share + i - to * share] = x;
+  }
+  if (tid < S * GH) {
+    const int to = tid / GH, h = tid % GH;
+    float mm, f0, f1;
+    merged(h, mm, f0, f1);
+    *reinterpret_cast<float2*>(cluster.map_shared_rank(&sm.ml_in[rank][h][0], to)) =
+        make_float2(mm, f0 * sm.ml[0][h][1] + (owner ? f1 * sm.ml[1][h][1] : 0.f));
+  }
+  cluster.sync();
+
+  // ---- this CTA's share of the outputs
+  if (tid < S * GH) {
+    const int r = tid / GH, h = tid % GH;
+    float mm = -INFINITY, ll = 0.f;
+    for (int k = 0; k < S; ++k) mm = fmaxf(mm, sm.ml_in[k][h][0]);
+    for (int k = 0; k < S; ++k) ll += (sm.ml_in[k][h][0] == mm ? 1.f : ex2(sm.ml_in[k][h][0] - mm)) * sm.ml_in[k][h][1];
+    const float inv = ll == 0.f ? 0.f : 1.f / ll;
+    sm.fac[r][h] = (sm.ml_in[r][h][0] == mm ? 1.f : ex2(sm.ml_in[r][h][0] - mm)) * inv;
+    if (r == 0) { sm.lse[h][0] = mm; sm.lse[h][1] = inv; }
+  }
+  __syncthreads();
+  for (int k = tid; k < share; k += THREADS) {
+    const int i = rank * share + k;
+    if (i >= n_g * HD) break;
+    float a = 0.f;
+    for (int r = 0; r < S; ++r) a += sm.fac[r][i / HD] * sm.o_in[r * share + k];
+    out[i] = from_f32<T>(a);
+  }
+  if (c.weight) {
+    // weight of block x: the sum over the group's heads, in their order, of 2^(part - maximum) / sum
+    const float* part = p.part + ((size_t)t * c.kv_heads + kvh) * p.blocks * GH;
+    const int end = owner ? nb + 1 : hi;
+    for (int x = lo + tid; x < end; x += THREADS) {
+      const int page = block_page(c, slot, x / per_page, p.err);
+      if (page < 0) continue;
+      const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + x % per_page;
+      float w = x == nb && pos == base ? 0.f : c.weight[i];
+      const float4 a = *reinterpret_cast<const float4*>(part + (size_t)x * GH), b4 = *reinterpret_cast<const float4*>(part + (size_t)x * GH + 4);
+      const float e[GH] = {a.x, a.y, a.z, a.w, b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int h = 0; h < GH; ++h)
+        if (h < n_g) w += ex2(e[h] - sm.lse[h][0]) * sm.lse[h][1];
+      p.weight_out[i] = w;
+    }
+  }
+  if (owner && pos - base == BLK - 1) {            // the block is full: from the next step on it is read in 8 bits
+    const int page = block_page(c, slot, nb / per_page, p.err);
+    if (page >= 0) {
+      const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + nb % per_page;
+      finish_block<IERT_LEVEL_INT8>(&sm.tail[0][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.k + i * BLK * HD, c.k_scale + i, sm.red);
+      finish_block<IERT_LEVEL_INT8>(&sm.tail[1][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.v + i * BLK * HD, c.v_scale + i, sm.red);
+    }
+  }
+}
+
+// The levels of a pool as rows of 128 bytes, fetched as boxes of a block's 16.
+bool level_map(const void* levels, long long rows, CUtensorMap* out) {
+  tma_host::EncodeTiledFn fn = tma_host::encode_fn();
+  if (!fn || rows <= 0 || rows > 0x7fffffffLL) return false;
+  cuuint64_t dims[2] = {HD, (cuuint64_t)rows}, strides[1] = {HD};
+  cuuint32_t box[2] = {HD, BLK}, estr[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(levels), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
+  auto kernel = block_attention_umma_kernel<T>;
+  const size_t smem = sizeof(Shared<T>);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return iert_check_launch("block_attention (attributes)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = iert_pdl_enabled ? 2 : 1;
+  cudaLaunchKernelEx(&cfg, kernel, mk, mv, p, b, c);
+  return iert_check_launch("block_attention");
+}
+
+}  // namespace
+
+// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule below.
+IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
+                                       float* part, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
+                                       int* err, cudaStream_t stream) {
+  if (batch->n_tokens <= 0) return IERT_OK;
+  const IertBlockView& c = *view;
+  if (c.head_dim != HD || c.format != IERT_LEVEL_INT8 || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || heads / c.kv_heads > GH ||
+      batch->n_tokens != batch->n_seqs || batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 ||
+      c.ring_pages <= 0 || c.ring_pages > c.table_width || c.n_pages <= 0 || c.n_slots <= 0 || c.window < 0 ||
+      (c.weight && (c.window || !part || !weight_out)) ||
+      ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)part) % 16 ||
+      (inv_freq && (rotary_dim < 0 || rotary_dim > HD || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
+    return IERT_BAD_ARGUMENT;
+  if (splits < 0 || splits > 16 || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
+  const long long pairs = (long long)c.kv_heads * batch->n_seqs;
+  if (splits == 0) {
+    splits = 1;
+    while (splits < 16 && pairs * splits * 2 <= 2LL * iert_sm_count_cached()) splits *= 2;
+  }
+  CUtensorMap mk, mv;
+  const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
+  if (!level_map(c.k, rows, &mk) || !level_map(c.v, rows, &mv)) return IERT_BAD_ARGUMENT;
+  UmmaParams p = {};
+  p.qkv = qkv; p.out = out; p.part = part; p.weight_out = weight_out;
+  p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
+  p.scale_log2e = scale * 1.44269504088896340736f;
+  p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
+  return c.tail_dtype == IERT_BF16 ? launch<__nv_bfloat16>(mk, mv, p, *batch, c, splits, stream) : launch<float>(mk, mv, p, *batch, c, splits, stream);
+}

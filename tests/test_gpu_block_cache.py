@@ -220,7 +220,7 @@ def test_one_token_steps(plain, fmt, dtype, G, H, D):
 
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("splits", [1, 2, 4, 8, 16])
-@pytest.mark.parametrize("warps", [4, 8, 16])
+@pytest.mark.parametrize("warps", [0, 4, 8, 16])
 @pytest.mark.parametrize("D", [64, 128])
 def test_a_key_head_shared_by_ctas(fmt, splits, warps, D):
     """Long and short sequences, more CTAs than blocks among them, more than 64 blocks for a warp."""
