@@ -558,12 +558,14 @@ int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& 
 
 }  // namespace
 
-// Floats of scratch: the blocks' weights, if the view keeps them.
+long long block_attention_piece_floats();          // block_attention_umma.cu
+
+// Floats of scratch: what CTAs leave for one another, and the blocks' weights, if the view keeps them.
 IERT_API long long iert_block_attention_scratch(int n_seqs, int heads, const IertBlockView* view) {
   const IertBlockView& c = *view;
-  if (!c.weight || n_seqs <= 0 || c.kv_heads <= 0 || heads <= 0) return 1;
+  if (!c.weight || n_seqs <= 0 || c.kv_heads <= 0 || heads <= 0) return block_attention_piece_floats();
   const long long pairs = (long long)n_seqs * c.kv_heads * ((heads / c.kv_heads + GH - 1) / GH);
-  return pairs * c.table_width * (c.page_tokens / BLK) * GH;
+  return block_attention_piece_floats() + pairs * c.table_width * (c.page_tokens / BLK) * GH;
 }
 
 // `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head, and `warps` (4, 8, 16) of each; 0: by the rule below.

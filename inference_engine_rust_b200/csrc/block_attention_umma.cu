@@ -11,10 +11,13 @@
 //   warps 0-3  softmax, a position per thread: a head's score from its digits, times the block's key scale; the probability times the
 //              block's value scale, as digits, into (swizzled) shared memory.  The references (a maximum per head, a largest value scale) move
 //              only where a fixed-point number would pass 2^31; O is then read out, added up in registers and begun again.
-//   warp 4     TMA producer: page numbers and scales of 32 blocks at a time, one per lane; boxes of 16 positions into a ring of two tiles.
+//   warp 4     TMA producer: page numbers and scales of 32 blocks at a time, one per lane; boxes of up to 128
+//              positions, as a page's size allows, into a ring of tiles.
 //   warp 5     MMA issuer: the scores of the next tile, then the weighted sum of this one.
-// A cluster of up to 16 CTAs shares a (sequence, kv head): each takes a run of its blocks and adds up a share of the outputs from what
-// the others have put into its shared memory.  The unfinished block, up to 16 rows in the run's type, is done in fp32 by the cluster's
+// A cluster of up to 8 CTAs shares a (sequence, kv head): each takes a run of its blocks and adds up a share of the outputs from what
+// the others have put into its shared memory.  Few long sequences need more CTAs than that to fill the device (an SM reads 42 GB/s at most, and
+// clusters of 16 fit only seven of its eight groups of SMs): theirs are not clusters, put their results into scratch memory, and a
+// second kernel, started while the first ends, adds them up (`WIDE`).  The unfinished block, up to 16 rows in the run's type, is done in fp32 by the
 // last CTA, which also stores the step's own key and value and turns the block into levels when it is full.
 // Queries as fixed-point numbers: bfloat16 runs 20 bits below the row's largest (three digits), float32 runs 27 (four); probabilities 25 bits below
 // the reference, which is at least 2^-6 of the largest.
@@ -34,21 +37,24 @@ using namespace sm100;
 
 namespace {
 
-constexpr int HD = 128, TILE = 128, TILE_BLOCKS = TILE / BLK, GH = 8, NSTAGE = 2, SOFT = 128, THREADS = 192, MAX_SPLITS = 16;
-constexpr int TILE_BYTES = TILE * HD, BOX_BYTES = BLK * HD, NCOL = 32;
-constexpr int SLOTS = 2 * NSTAGE;              // of the tiles' scales: the softmax reads a tile's after its stage may be filled again
-constexpr uint32_t TMEM_COLS = 128;            // S twice, O
+constexpr int HD = 128, TILE = 128, TILE_BLOCKS = TILE / BLK, GH = 8, SOFT = 128, MAX_SPLITS = 8, MERGE_THREADS = 128, MAX_PIECES = 160;
+constexpr int TILE_BYTES = TILE * HD, BLOCK_BYTES = BLK * HD, NCOL = 32;
+constexpr uint32_t TMEM_COLS = 128;            // S twice, O once per group
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int P_BITS = 25;                     // a probability of 1 (times the largest value scale) is 2^25; 2^31 is the bound
 constexpr int MAX_RUN = 256;                   // tiles that O adds up at most: 255 * 127 * 128 * 256 < 2^31
+constexpr int WIDE_FROM = 32768;               // positions that a sequence may hold from which few sequences' CTAs are no clusters
 constexpr int TAIL_BLOCKS = 16;                // finished blocks that cost a CTA about as much time as the unfinished one
 
 struct UmmaParams {
   const void* qkv;
   void* out;
   float* part;                 // [T][kv_heads][blocks][8]: base-2 logarithm of a block's unnormalised weight
+  float* piece_o;              // WIDE: [T][kv_heads][CTAs][8][HD], what each CTA has
+  float* piece_ml;             // and [T][kv_heads][CTAs][8][2], maximum and sum
   float* weight_out;
   int heads, blocks;
+  int run;                     // blocks of a box: they stand side by side in a page (1, 2, 4 or 8)
   float scale_log2e;
   const float* inv_freq;
   int rope, rotary_dim, pairing;
@@ -56,12 +62,13 @@ struct UmmaParams {
   int* err;
 };
 
-template <typename T> struct __align__(1024) Shared {
+template <typename T, int GROUPS, int NSTAGE> struct __align__(1024) Shared {
+  static constexpr int SLOTS = 2 * NSTAGE;       // of the tiles' scales: the softmax may read a tile's after its stage is filled again
   uint8_t ring[NSTAGE][2][TILE_BYTES];          // keys, values: rows of 128 bytes, 128-byte swizzle
   uint8_t qd[NCOL * HD];                         // digits of the queries: row 8 j + h is digit j of head h
   uint8_t pd[2][NCOL * TILE];                    // digits of the probabilities, likewise
   float q[GH][HD + 4];
-  float o[GH][HD];                               // this CTA's finished blocks
+  float o[GROUPS][GH][HD];                       // each group's finished blocks
   T tail[2][BLK][HD];
   float cs[HD];
   float tail_s[BLK][GH];
@@ -69,13 +76,14 @@ template <typename T> struct __align__(1024) Shared {
   float o_in[GH * HD + MAX_SPLITS];              // this CTA's share of the outputs, from every CTA of the cluster
   float ml_in[MAX_SPLITS][GH][2];
   float fac[MAX_SPLITS][GH];
-  float ml[2][GH][2];                            // maximum and sum: finished blocks, unfinished block
+  float ml[GROUPS + 1][GH][2];                   // maximum and sum: each group's blocks, the unfinished block
+  float wfac[GROUPS + 1][GH];                    // what each of them counts for in the CTA's result
   float lse[GH][2];
   float rs[GH];                                  // what makes scores of the integers
-  float top[4][GH];
-  float sum[4][GH];
+  float top[GROUPS][4][GH];
+  float sum[GROUPS][4][GH];
   float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there: key scale NaN of its own kind (see NOWHERE)
-  uint32_t red[THREADS / 32];
+  uint32_t red[GROUPS * 4 + 2];
   uint64_t k_full[NSTAGE], v_full[NSTAGE], k_empty[NSTAGE], v_empty[NSTAGE], s_full[2], s_empty[2], p_ready[2], pv_done[2], drained;
   uint32_t tmem;
   int restart[2];
@@ -106,15 +114,16 @@ __device__ __forceinline__ void mma_i8(uint32_t leader, uint32_t d, uint64_t a, 
 __host__ __device__ constexpr uint32_t instr_desc_i8(uint32_t M, uint32_t N, uint32_t b_signed, uint32_t a_mn) {
   return (2u << 4) | (1u << 7) | (b_signed << 10) | (a_mn << 15) | ((N >> 3) << 17) | ((M >> 4) << 24);
 }
-__device__ __forceinline__ void soft_sync() { asm volatile("bar.sync 1, %0;" ::"n"(SOFT) : "memory"); }
-// The same for the softmax and the MMA warp.
-__device__ __forceinline__ void early_sync() { asm volatile("bar.sync 2, %0;" ::"n"(SOFT + 32) : "memory"); }
-__device__ __forceinline__ bool soft_any(bool x) {
+// Barriers of one softmax group.
+__device__ __forceinline__ void soft_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(SOFT) : "memory"); }
+__device__ __forceinline__ bool soft_any(int group, bool x) {
   int y;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-               : "=r"(y) : "r"((int)x), "n"(SOFT) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+               : "=r"(y) : "r"((int)x), "r"(1 + group), "n"(SOFT) : "memory");
   return y != 0;
 }
+// All but the producer.
+template <int N> __device__ __forceinline__ void early_sync() { asm volatile("bar.sync 3, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   tmem_ld16_issue(taddr, r);
   tmem_ld16_issue(taddr + 16, r + 16);
@@ -132,12 +141,18 @@ __device__ __forceinline__ float head_value(const T* src, int d, const UmmaParam
   return to_f32(from_f32<T>(second ? y * cs[half + k] + x * cs[k] : x * cs[k] - y * cs[half + k]));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 2)
+// GROUPS: of four softmax warps each, which take the tiles in turn and keep an O, references and sums of their own.  One group and two CTAs
+// an SM where there are CTAs enough, else two groups and a deeper ring in one CTA an SM: a tile takes a group about 1.1 us, an SM's share of the
+// memory's rate brings one in 0.75 us.
+template <typename T, int GROUPS, int NSTAGE, bool WIDE>
+__global__ void __launch_bounds__(GROUPS * SOFT + 64, 3 - GROUPS)
 block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, UmmaParams p, IertBatchView b,
                             IertBlockView c) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];        // no static shared memory: the window starts 1024-byte aligned
-  Shared<T>& sm = *reinterpret_cast<Shared<T>*>(smem_raw);
+  using Sh = Shared<T, GROUPS, NSTAGE>;
+  Sh& sm = *reinterpret_cast<Sh*>(smem_raw);
+  constexpr int THREADS = GROUPS * SOFT + 64, PRODUCER = 4 * GROUPS, ISSUER = PRODUCER + 1, SLOTS = Sh::SLOTS;
+  static_assert(THREADS >= MAX_SPLITS * GH && SLOTS >= NSTAGE + 2, "a thread per (CTA, head); see sm.scale");
   constexpr int DIG = sizeof(T) == 4 ? 4 : 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int S = gridDim.x, rank = blockIdx.x;                  // the cluster is the grid's first axis
@@ -151,7 +166,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   if (slot < 0) {                                              // (the same for the whole cluster)
     pdl_launch_dependents();
     pdl_wait();
-    if (rank == 0)
+    if (rank == 0 && !WIDE)
       for (int i = tid; i < n_g * HD; i += THREADS) out[i] = from_f32<T>(0.f);
     return;
   }
@@ -159,10 +174,12 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     if (tid == 0) atomicOr(p.err, IERT_ERR_WAIT_EXPIRED);
     return;
   }
-  cg::cluster_group::arrival_token started = cluster.barrier_arrive();
+  cg::cluster_group::arrival_token started;
+  if (!WIDE) started = cluster.barrier_arrive();
   const int pos = b.pos0[s], nb = pos / BLK, base = nb * BLK, per_page = c.page_tokens / BLK;
-  const int j_min = iert_first_visible(pos, c.window, 0), b_lo = min(j_min / BLK, nb);
-  const int per = (nb - b_lo + (S > 1 ? TAIL_BLOCKS : 0) + S - 1) / S;
+  const int j_min = iert_first_visible(pos, c.window, 0), b_lo = min(j_min / BLK, nb) / p.run * p.run;
+  // a run of blocks that begins with a box's first (blocks in front of the window's, or behind the last, count for nothing)
+  const int per = ((nb - b_lo + (S > 1 ? TAIL_BLOCKS : 0) + S - 1) / S + p.run - 1) / p.run * p.run;
   const int lo = min(nb, b_lo + rank * per), hi = min(nb, lo + per);
   const int n_tiles = (hi - lo + TILE_BLOCKS - 1) / TILE_BLOCKS;
   const bool owner = rank == S - 1;                            // of the unfinished block
@@ -175,34 +192,35 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     sm.abort_flag = 0; sm.asked_k = 0; sm.asked_v = 0;
     mbar_fence_init();
   }
-  if (warp == 5) tmem_alloc(&sm.tmem, TMEM_COLS);
+  if (warp == ISSUER) tmem_alloc(&sm.tmem, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_launch_dependents();                                     // (a later kernel must not take the TMEM this CTA waits for)
   const uint32_t tmem = sm.tmem, o_col = 2 * NCOL;
   bool ok = true;
-  pdl_wait();
 
-  if (warp == 4) {
+  if (warp == PRODUCER) {
     // ---------------- TMA producer ----------------
     if (lane == 0) { tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v); }
+    auto page_at = [&](int x) { return x < hi ? block_page(c, slot, x / per_page, p.err) : -1; };
+    int page = page_at(lo + lane);                             // like the step's description, the page table does not depend on the kernel before
+    pdl_wait();
     for (int i0 = 0; i0 < n_tiles && ok; i0 += 32 / TILE_BLOCKS) {
       const int x = lo + i0 * TILE_BLOCKS + lane;
       int at = -1;
       float ks = __uint_as_float(NOWHERE), vs = 0.f;
-      if (x < hi) {
-        const int page = block_page(c, slot, x / per_page, p.err);
-        if (page >= 0) {
-          at = (page * c.kv_heads + kvh) * per_page + x % per_page;
-          ks = c.k_scale[at];
-          vs = c.v_scale[at];
-        }
+      if (page >= 0) {
+        at = (page * c.kv_heads + kvh) * per_page + x % per_page;
+        ks = c.k_scale[at];
+        vs = c.v_scale[at];
       }
+      page = page_at(x + 32);                                  // (of the next 32)
       for (int k = 0; k < 32 / TILE_BLOCKS && i0 + k < n_tiles && ok; ++k) {
         const int i = i0 + k, st = i % NSTAGE;
         const uint32_t again = ((i / NSTAGE) - 1) & 1;
-        const unsigned here = (__ballot_sync(0xffffffffu, at >= 0) >> (k * TILE_BLOCKS)) & 0xffu;
+        const bool asks = (lane >> 3) == k && at >= 0 && lane % p.run == 0;        // a lane per box
+        const unsigned here = __ballot_sync(0xffffffffu, asks);
         if (i >= NSTAGE) ok = wait_bar(&sm.k_empty[st], again, abort_flag);
         if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
         if ((lane >> 3) == k) sm.scale[i % SLOTS][lane & 7] = make_float2(ks, vs);
@@ -214,19 +232,19 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
           }
           uint64_t* full = kv ? &sm.v_full[st] : &sm.k_full[st];
           if (lane == 0) {
-            mbar_expect_tx(full, __popc(here) * BOX_BYTES);
+            mbar_expect_tx(full, __popc(here) * p.run * BLOCK_BYTES);
             if (kv) sm.asked_v = i + 1; else sm.asked_k = i + 1;
           }
           __syncwarp();
-          // a lane per block asks for its box: rows 16 (i & 7).. of the tile
-          if ((lane >> 3) == k && at >= 0) tma_load_2d(sm.ring[st][kv] + (lane & 7) * BOX_BYTES, kv ? &map_v : &map_k, full, 0, at * BLK);
+          if (asks) tma_load_2d(sm.ring[st][kv] + (lane & 7) * BLOCK_BYTES, kv ? &map_v : &map_k, full, 0, at * BLK);
         }
       }
     }
   } else {
     // ---------------- the queries' digits (softmax and MMA warps) ----------------
-    const int me = warp == 5 ? SOFT + lane : tid;              // 0..159
-    constexpr int N = SOFT + 32;
+    pdl_wait();
+    const int me = warp == ISSUER ? GROUPS * SOFT + lane : tid;
+    constexpr int N = GROUPS * SOFT + 32;
     if (p.rope) {
       const float where = (float)(pos + (c.shift ? c.shift[slot] : 0));
       for (int k = me; k < p.rotary_dim / 2; k += N) {
@@ -235,7 +253,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         sm.cs[k] = co * p.rot_mul;
         sm.cs[p.rotary_dim / 2 + k] = sn * p.rot_mul;
       }
-      early_sync();
+      early_sync<N>();
     }
     if (owner) {
       const size_t off = ((size_t)slot * c.kv_heads + kvh) * BLK * HD;
@@ -262,8 +280,8 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       const int r = i / HD, d = i % HD;
       sm.q[r][d] = r < n_g ? head_value(row + (size_t)r * HD + (size_t)kvh * n_g * HD, d, p, sm.cs) : 0.f;
     }
-    early_sync();
-    for (int h = warp == 5 ? 4 : warp; h < GH; h += 5) {       // a warp per head: four numbers a lane
+    early_sync<N>();
+    for (int h = warp == ISSUER ? PRODUCER : warp; h < GH; h += PRODUCER + 1) {       // a warp per head: four numbers a lane
       const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][4 * lane]);
       uint32_t largest = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
 #pragma unroll
@@ -292,9 +310,9 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         *reinterpret_cast<uint32_t*>(sm.qd + (8 * j + h) * HD + (((lane >> 2) ^ (h & 7)) << 4) + (lane & 3) * 4) = dig[j];
     }
     fence_proxy_async_smem();
-    early_sync();
+    early_sync<N>();
 
-    if (warp == 5) {
+    if (warp == ISSUER) {
       // ---------------- MMA issuer (the whole warp, one lane of it acting) ----------------
       constexpr uint32_t IDESC_S = instr_desc_i8(TILE, NCOL, 1, 0), IDESC_O = instr_desc_i8(HD, NCOL, 0, 1);
       const uint32_t leader = elect_leader();
@@ -319,15 +337,16 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         const uint32_t more = *(volatile int*)&sm.restart[i & 1] ? 0u : 1u;
         const uint64_t vd = smem_desc_mn128(smem_addr(sm.ring[st][1]), TILE_BYTES), pd = smem_desc_k128(smem_addr(sm.pd[i & 1]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + o_col, vd + k * (32 * HD >> 4), pd + k * 2, IDESC_O, k > 0 ? 1u : more);
+        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + o_col + (GROUPS == 2 ? (i & 1) * NCOL : 0), vd + k * (32 * HD >> 4), pd + k * 2, IDESC_O, k > 0 ? 1u : more);
         mma_commit(leader, &sm.pv_done[i & 1]);
         mma_commit(leader, &sm.v_empty[st]);
       }
       mma_commit(leader, &sm.drained);
     } else {
       // ---------------- the unfinished block, in fp32: a thread per (row, head), then per dimension ----------------
-      if (owner) {
-        const int r = tid >> 3, h = tid & 7;
+      const int grp = warp >> 2, me = tid & (SOFT - 1);            // position `me` of a tile; dimension `me` of O
+      if (owner && grp == GROUPS - 1) {
+        const int r = me >> 3, h = me & 7;
         float sc = -INFINITY;
         if (base + r <= pos && base + r >= j_min) {
           float dot = 0.f;
@@ -341,47 +360,47 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
           sc = dot * p.scale_log2e;
         }
         sm.tail_s[r][h] = sc;
-        soft_sync();
+        soft_sync(grp);
         float mx = -INFINITY, l = 0.f;
 #pragma unroll
         for (int i = 0; i < BLK; ++i) mx = fmaxf(mx, sm.tail_s[i][h]);
         const float pr = mx == -INFINITY ? (sc == sc ? 0.f : sc) : ex2(sc - mx);
-        soft_sync();
+        soft_sync(grp);
         sm.tail_s[r][h] = pr;
-        soft_sync();
+        soft_sync(grp);
         if (r == 0) {
 #pragma unroll
           for (int i = 0; i < BLK; ++i) l += sm.tail_s[i][h];
-          sm.ml[1][h][0] = mx;
-          sm.ml[1][h][1] = l;
+          sm.ml[GROUPS][h][0] = mx;
+          sm.ml[GROUPS][h][1] = l;
           if (c.weight) p.part[(((size_t)t * c.kv_heads + kvh) * p.blocks + nb) * GH + h] = mx + log2f(l);
         }
         float acc[GH] = {};
         for (int i = max(0, j_min - base); i <= pos - base; ++i) {
-          const float v = to_f32(sm.tail[1][i][tid]);
+          const float v = to_f32(sm.tail[1][i][me]);
 #pragma unroll
           for (int k = 0; k < GH; ++k) acc[k] = fmaf(sm.tail_s[i][k], v, acc[k]);
         }
 #pragma unroll
-        for (int k = 0; k < GH; ++k) sm.tail_o[k][tid] = acc[k];
+        for (int k = 0; k < GH; ++k) sm.tail_o[k][me] = acc[k];
       }
 
-      // ---------------- softmax: position tid of a tile; dimension tid of O ----------------
-      const uint32_t lane_bits = (uint32_t)(warp * 32) << 16;
-      const int blk = tid >> 4;
+      // ---------------- softmax ----------------
+      const uint32_t lane_bits = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem + lane_bits + o_col + (GROUPS == 2 ? grp * NCOL : 0);
+      const int blk = me >> 4;
       float* part = c.weight ? p.part + ((size_t)t * c.kv_heads + kvh) * p.blocks * GH : nullptr;
       float rs[GH], ref[GH], l[GH], acc[GH];
 #pragma unroll
       for (int h = 0; h < GH; ++h) { rs[h] = sm.rs[h]; ref[h] = -INFINITY; l[h] = 0.f; acc[h] = 0.f; }
       float v_ref = 0.f, v_inv = 0.f;              // the value scale that probabilities are relative to, and its inverse
       int run = 0;                                 // tiles in O
-      // O of the tiles so far, in units of v_ref 2^-P_BITS, joins acc (dimension tid)
+      // O of the tiles so far, in units of v_ref 2^-P_BITS, joins acc (dimension `me`)
       auto flush = [&](int i) {                    // i: the last tile in O
         if (!wait_bar(&sm.pv_done[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
         __syncwarp();
         tc_fence_after();
         uint32_t r[32];
-        tmem_ld32(tmem + lane_bits + o_col, r);
+        tmem_ld32(my_o, r);
         tc_fence_before();
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
@@ -390,7 +409,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         }
         run = 0;
       };
-      for (int i = 0; i < n_tiles; ++i) {
+      for (int i = GROUPS == 2 ? grp : 0; i < n_tiles; i += GROUPS) {
         if (!wait_bar(&sm.s_full[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
         __syncwarp();
         tc_fence_after();
@@ -400,7 +419,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         tc_fence_before();
         mbar_arrive(&sm.s_empty[i & 1]);
         const int x = lo + i * TILE_BLOCKS + blk;
-        const bool there = __float_as_uint(sc.x) != NOWHERE && x * BLK + (tid & 15) >= j_min;
+        const bool there = __float_as_uint(sc.x) != NOWHERE && x * BLK + (me & 15) >= j_min;
         float v[GH], y[GH];
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
@@ -414,18 +433,18 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         bool far = !ok;
 #pragma unroll
         for (int h = 0; h < GH; ++h) far |= !(y[h] * vu < 2147483648.f) || !(y[h] < 1e30f);
-        if (soft_any(far || run == MAX_RUN)) {       // (the same for all four warps)
-          if (soft_any(!ok)) { ok = false; break; }
+        if (soft_any(grp, far || run == MAX_RUN)) {       // (the same for all four warps)
+          if (soft_any(grp, !ok)) { ok = false; break; }
           // new references: the largest of the tile per head, the largest value scale; what was added up moves to them
-          if (run > 0) flush(i - 1);
+          if (run > 0) flush(i - GROUPS);
 #pragma unroll
           for (int h = 0; h < GH; ++h) {
             float mx = v[h];
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            if (lane == 0) sm.top[warp][h] = mx;
+            if (lane == 0) sm.top[grp][warp & 3][h] = mx;
           }
-          soft_sync();
+          soft_sync(grp);
           float v_new = v_ref;
 #pragma unroll
           for (int k = 0; k < TILE_BLOCKS; ++k) {
@@ -437,18 +456,18 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
           v_inv = v_ref > 0.f ? 1.f / v_ref : 0.f;
 #pragma unroll
           for (int h = 0; h < GH; ++h) {
-            const float to = fmaxf(ref[h], fmaxf(fmaxf(sm.top[0][h], sm.top[1][h]), fmaxf(sm.top[2][h], sm.top[3][h])));
+            const float to = fmaxf(ref[h], fmaxf(fmaxf(sm.top[grp][0][h], sm.top[grp][1][h]), fmaxf(sm.top[grp][2][h], sm.top[grp][3][h])));
             const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
             ref[h] = to;
             l[h] *= alpha;
             acc[h] *= alpha * v_move;
             y[h] = v[h] == -INFINITY ? 0.f : ex2(v[h] - to);
           }
-          soft_sync();                             // (sm.top may be written again)
+          soft_sync(grp);                             // (sm.top may be written again)
         }
         const float unit = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
         if (i >= 2 && !wait_bar(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, abort_flag)) ok = false;      // the buffer is free
-        uint8_t* pd = sm.pd[i & 1] + (tid & 15);
+        uint8_t* pd = sm.pd[i & 1] + (me & 15);
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
           const float w = y[h] * unit;
@@ -460,7 +479,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
           at[16 * TILE] = (uint8_t)(z >> 16);
           at[24 * TILE] = (uint8_t)(z >> 24);
         }
-        if (tid == 0) sm.restart[i & 1] = run == 0;
+        if (me == 0) sm.restart[i & 1] = run == 0;
         ++run;
         fence_proxy_async_smem();
         tc_fence_before();
@@ -481,18 +500,18 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         }
       }
       ok = __all_sync(0xffffffffu, ok) != 0;
-      if (ok && run > 0) flush(n_tiles - 1);
+      if (ok && run > 0) flush(GROUPS == 2 ? (n_tiles - 1 - grp) / 2 * 2 + grp : n_tiles - 1);       // its last tile
 #pragma unroll
       for (int h = 0; h < GH; ++h) {
-        sm.o[h][tid] = acc[h] * (v_ref * (1.f / (1 << P_BITS)));
+        sm.o[grp][h][me] = acc[h] * (v_ref * (1.f / (1 << P_BITS)));
         float z = l[h];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        if (lane == 0) sm.sum[warp][h] = z;
+        if (lane == 0) sm.sum[grp][warp & 3][h] = z;
       }
-      if (tid == 0)
+      if (me == 0)
 #pragma unroll
-        for (int h = 0; h < GH; ++h) sm.ml[0][h][0] = ref[h];
+        for (int h = 0; h < GH; ++h) sm.ml[grp][h][0] = ref[h];
     }
   }
   if (!ok && lane == 0) {
@@ -508,35 +527,54 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       if (sm.asked_v > st) mbar_wait(&sm.v_full[st], (((sm.asked_v - 1 - st) / NSTAGE)) & 1, WAIT_LIMIT);
     }
   }
-  if (tid < GH) sm.ml[0][tid][1] = (sm.sum[0][tid] + sm.sum[1][tid]) + (sm.sum[2][tid] + sm.sum[3][tid]);
-  cluster.barrier_wait(std::move(started));        // every CTA runs
+  if (tid < GH * GROUPS) {
+    const int w = tid / GH, h = tid % GH;
+    sm.ml[w][h][1] = (sm.sum[w][0][h] + sm.sum[w][1][h]) + (sm.sum[w][2][h] + sm.sum[w][3][h]);
+  }
   __syncthreads();
-  if (warp == 5) {
+  const int parts = GROUPS + (owner ? 1 : 0);
+  if (tid < GH * (GROUPS + 1)) {
+    const int w = tid / GH, h = tid % GH;
+    float mm = -INFINITY;
+    for (int k = 0; k < parts; ++k) mm = fmaxf(mm, sm.ml[k][h][0]);
+    sm.wfac[w][h] = w >= parts ? 0.f : sm.ml[w][h][0] == mm ? 1.f : ex2(sm.ml[w][h][0] - mm);
+  }
+  if (!WIDE) cluster.barrier_wait(std::move(started));        // every CTA runs
+  __syncthreads();
+  if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
 
-  // ---- the CTA's partial result, finished blocks and the unfinished one, goes to the CTAs that add up its pieces
+  if (WIDE) {
+    const size_t piece = ((size_t)t * c.kv_heads + kvh) * S + rank;
+    for (int i = tid; i < n_g * HD; i += THREADS) {
+      const int h = i / HD, d = i % HD;
+      float x = owner ? sm.wfac[GROUPS][h] * sm.tail_o[h][d] : 0.f;
+#pragma unroll
+      for (int w = 0; w < GROUPS; ++w) x += sm.wfac[w][h] * sm.o[w][h][d];
+      p.piece_o[piece * GH * HD + i] = x;
+    }
+    if (tid < GH) {
+      float mm = -INFINITY, ll = 0.f;
+      for (int k = 0; k < parts; ++k) { mm = fmaxf(mm, sm.ml[k][tid][0]); ll += sm.wfac[k][tid] * sm.ml[k][tid][1]; }
+      *reinterpret_cast<float2*>(p.piece_ml + (piece * GH + tid) * 2) = make_float2(mm, ll);
+    }
+  } else {
+  // ---- the CTA's partial result, its groups' blocks and the unfinished one, goes to the CTAs that add up its pieces
   const int share = (n_g * HD + S - 1) / S;
-  auto merged = [&](int h, float& mm, float& f0, float& f1) {
-    const float m0 = sm.ml[0][h][0], m1 = owner ? sm.ml[1][h][0] : -INFINITY;
-    mm = fmaxf(m0, m1);
-    f0 = m0 == mm ? 1.f : ex2(m0 - mm);
-    f1 = !owner ? 0.f : m1 == mm ? 1.f : ex2(m1 - mm);
-  };
   for (int i = tid; i < n_g * HD; i += THREADS) {
     const int h = i / HD, d = i % HD, to = i / share;
-    float mm, f0, f1;
-    merged(h, mm, f0, f1);
-    const float x = f0 * sm.o[h][d] + (owner ? f1 * sm.tail_o[h][d] : 0.f);
+    float x = owner ? sm.wfac[GROUPS][h] * sm.tail_o[h][d] : 0.f;
+#pragma unroll
+    for (int w = 0; w < GROUPS; ++w) x += sm.wfac[w][h] * sm.o[w][h][d];
     cluster.map_shared_rank(&sm.o_in[0], to)[rank * share + i - to * share] = x;
   }
   if (tid < S * GH) {
     const int to = tid / GH, h = tid % GH;
-    float mm, f0, f1;
-    merged(h, mm, f0, f1);
-    *reinterpret_cast<float2*>(cluster.map_shared_rank(&sm.ml_in[rank][h][0], to)) =
-        make_float2(mm, f0 * sm.ml[0][h][1] + (owner ? f1 * sm.ml[1][h][1] : 0.f));
+    float mm = -INFINITY, ll = 0.f;
+    for (int k = 0; k < parts; ++k) { mm = fmaxf(mm, sm.ml[k][h][0]); ll += sm.wfac[k][h] * sm.ml[k][h][1]; }
+    *reinterpret_cast<float2*>(cluster.map_shared_rank(&sm.ml_in[rank][h][0], to)) = make_float2(mm, ll);
   }
   cluster.sync();
 
@@ -575,6 +613,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       p.weight_out[i] = w;
     }
   }
+  }
   if (owner && pos - base == BLK - 1) {            // the block is full: from the next step on it is read in 8 bits
     const int page = block_page(c, slot, nb / per_page, p.err);
     if (page >= 0) {
@@ -585,67 +624,156 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   }
 }
 
-// The levels of a pool as rows of 128 bytes, fetched as boxes of a block's 16.
-bool level_map(const void* levels, long long rows, CUtensorMap* out) {
+// Adds up what the CTAs of a (sequence, kv head) have left, in their order, and the weights of its blocks.  The third axis of the grid
+// shares a pair: columns of the outputs, and blocks.
+template <typename T>
+__global__ void __launch_bounds__(MERGE_THREADS) block_attention_umma_merge_kernel(UmmaParams p, IertBatchView b, IertBlockView c, int C) {
+  __shared__ float fac[MAX_PIECES][GH];
+  __shared__ float lse[GH][2];
+  pdl_launch_dependents();
+  const int kvh = blockIdx.x, s = blockIdx.y, z = blockIdx.z, Z = gridDim.z, tid = threadIdx.x;
+  const int n_g = p.heads / c.kv_heads, per_page = c.page_tokens / BLK;
+  int slot = block_slot(c, b, s, p.err);
+  const int pos = b.pos0[s];
+  if (slot >= 0 && !block_reaches(c, pos, p.err)) slot = -1;
+  T* out = (T*)p.out + ((size_t)s * p.heads + (size_t)kvh * n_g) * HD;
+  pdl_wait();
+  if (slot < 0) {
+    for (int i = z * MERGE_THREADS + tid; i < n_g * HD; i += Z * MERGE_THREADS) out[i] = from_f32<T>(0.f);
+    return;
+  }
+  const float* ml = p.piece_ml + ((size_t)s * c.kv_heads + kvh) * C * GH * 2;
+  const float* po = p.piece_o + ((size_t)s * c.kv_heads + kvh) * C * GH * HD;
+  {                                                // sixteen threads per head
+    const int h = tid >> 4, l16 = tid & 15;
+    float mm = -INFINITY, ll = 0.f;
+    for (int k = l16; k < C; k += 16) mm = fmaxf(mm, ml[(k * GH + h) * 2]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+    for (int k = l16; k < C; k += 16) {
+      const float2 x = *reinterpret_cast<const float2*>(ml + (k * GH + h) * 2);
+      const float f = x.x == mm ? 1.f : ex2(x.x - mm);
+      fac[k][h] = f;
+      ll += f * x.y;
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) ll += __shfl_xor_sync(0xffffffffu, ll, o);
+    if (l16 == 0) { lse[h][0] = mm; lse[h][1] = ll == 0.f ? 0.f : 1.f / ll; }
+  }
+  __syncthreads();
+  for (int i = z * MERGE_THREADS + tid; i < n_g * HD; i += Z * MERGE_THREADS) {
+    float acc = 0.f;
+#pragma unroll 8
+    for (int k = 0; k < C; ++k) acc += fac[k][i / HD] * po[(size_t)k * GH * HD + i];
+    out[i] = from_f32<T>(acc * lse[i / HD][1]);
+  }
+  if (c.weight) {
+    const int nb = pos / BLK;
+    const float* part = p.part + ((size_t)s * c.kv_heads + kvh) * p.blocks * GH;
+    for (int x = z * MERGE_THREADS + tid; x <= nb; x += Z * MERGE_THREADS) {
+      const int page = block_page(c, slot, x / per_page, p.err);
+      if (page < 0) continue;
+      const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + x % per_page;
+      float w = x == nb && pos % BLK == 0 ? 0.f : c.weight[i];
+      const float4 a = *reinterpret_cast<const float4*>(part + (size_t)x * GH), b4 = *reinterpret_cast<const float4*>(part + (size_t)x * GH + 4);
+      const float e[GH] = {a.x, a.y, a.z, a.w, b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+      for (int h = 0; h < GH; ++h)
+        if (h < n_g) w += ex2(e[h] - lse[h][0]) * lse[h][1];
+      p.weight_out[i] = w;
+    }
+  }
+}
+
+// The levels of a pool as rows of 128 bytes, fetched as boxes of `run` blocks.
+bool level_map(const void* levels, long long rows, int run, CUtensorMap* out) {
   tma_host::EncodeTiledFn fn = tma_host::encode_fn();
   if (!fn || rows <= 0 || rows > 0x7fffffffLL) return false;
   cuuint64_t dims[2] = {HD, (cuuint64_t)rows}, strides[1] = {HD};
-  cuuint32_t box[2] = {HD, BLK}, estr[2] = {1, 1};
+  cuuint32_t box[2] = {HD, (cuuint32_t)(BLK * run)}, estr[2] = {1, 1};
   return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(levels), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T>
+template <typename T, int GROUPS, int NSTAGE, bool WIDE>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
-  auto kernel = block_attention_umma_kernel<T>;
-  const size_t smem = sizeof(Shared<T>);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-    return iert_check_launch("block_attention (attributes)");
+  auto kernel = block_attention_umma_kernel<T, GROUPS, NSTAGE, WIDE>;
+  const size_t smem = sizeof(Shared<T, GROUPS, NSTAGE>);
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return iert_check_launch("block_attention (shared memory)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(GROUPS * SOFT + 64);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (!WIDE) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = splits; attr[n].val.clusterDim.y = 1; attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (iert_pdl_enabled) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = iert_pdl_enabled ? 2 : 1;
+  cfg.numAttrs = n;
   cudaLaunchKernelEx(&cfg, kernel, mk, mv, p, b, c);
-  return iert_check_launch("block_attention");
+  const int status = iert_check_launch("block_attention");
+  if (status || !WIDE) return status;
+  launch_dep(block_attention_umma_merge_kernel<T>, dim3(c.kv_heads, b.n_seqs, 8), dim3(MERGE_THREADS), 0, stream, p, b, c, splits);
+  return iert_check_launch("block_attention (merge)");
+}
+
+template <typename T>
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, int groups, bool wide,
+           cudaStream_t stream) {
+  if (wide) return launch<T, 2, 4, true>(mk, mv, p, b, c, splits, stream);
+  return groups == 2 ? launch<T, 2, 4, false>(mk, mv, p, b, c, splits, stream) : launch<T, 1, 2, false>(mk, mv, p, b, c, splits, stream);
 }
 
 }  // namespace
 
-// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule below.
+// Floats of scratch in front of the blocks' weights (block_attention_tc.cu).
+long long block_attention_piece_floats() { return (long long)MAX_PIECES * GH * (HD + 2); }
+
+// `splits`: CTAs that share a sequence's kv head (1, 2, 4, 8: a cluster; more: not); `groups` (1, 2) of softmax warps in each; 0: by the rule below.
 IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
-                                       float* part, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
-                                       int* err, cudaStream_t stream) {
+                                       float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
+                                       int groups, int* err, cudaStream_t stream) {
   if (batch->n_tokens <= 0) return IERT_OK;
   const IertBlockView& c = *view;
   if (c.head_dim != HD || c.format != IERT_LEVEL_INT8 || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || heads / c.kv_heads > GH ||
       batch->n_tokens != batch->n_seqs || batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 ||
       c.ring_pages <= 0 || c.ring_pages > c.table_width || c.n_pages <= 0 || c.n_slots <= 0 || c.window < 0 ||
-      (c.weight && (c.window || !part || !weight_out)) ||
-      ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)part) % 16 ||
+      !scratch || (c.weight && (c.window || !weight_out)) ||
+      ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)scratch) % 16 ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > HD || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
     return IERT_BAD_ARGUMENT;
-  if (splits < 0 || splits > 16 || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
   const long long pairs = (long long)c.kv_heads * batch->n_seqs;
+  if (splits < 0 || groups < 0 || groups > 2 || (splits > MAX_SPLITS ? pairs * splits > MAX_PIECES : (splits & (splits - 1)) != 0)) return IERT_BAD_ARGUMENT;
+  const int sms = iert_sm_count_cached();
   if (splits == 0) {
-    splits = 1;
-    while (splits < 16 && pairs * splits * 2 <= 2LL * iert_sm_count_cached()) splits *= 2;
+    const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
+    if (pairs * 2 * MAX_SPLITS <= sms && reach >= WIDE_FROM) splits = (int)(sms / pairs);
+    else
+      for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= sms;) splits *= 2;
   }
+  const bool wide = splits > MAX_SPLITS;
+  if (groups == 0) groups = pairs * splits <= sms ? 2 : 1;
   CUtensorMap mk, mv;
   const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
-  if (!level_map(c.k, rows, &mk) || !level_map(c.v, rows, &mv)) return IERT_BAD_ARGUMENT;
   UmmaParams p = {};
-  p.qkv = qkv; p.out = out; p.part = part; p.weight_out = weight_out;
+  p.run = TILE_BLOCKS;
+  while ((c.page_tokens / BLK) % p.run) p.run >>= 1;
+  if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;
+  p.qkv = qkv; p.out = out; p.weight_out = weight_out;
+  p.piece_o = scratch; p.piece_ml = scratch + (long long)MAX_PIECES * GH * HD; p.part = scratch + block_attention_piece_floats();
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
-  return c.tail_dtype == IERT_BF16 ? launch<__nv_bfloat16>(mk, mv, p, *batch, c, splits, stream) : launch<float>(mk, mv, p, *batch, c, splits, stream);
+  return c.tail_dtype == IERT_BF16 ? launch<__nv_bfloat16>(mk, mv, p, *batch, c, splits, groups, wide, stream)
+                                   : launch<float>(mk, mv, p, *batch, c, splits, groups, wide, stream);
 }
