@@ -37,6 +37,7 @@ struct BlockTcParams {
   float* part;                 // [T][kv_heads][slices of 8 heads][blocks][8]: base-2 logarithm of a block's unnormalised weight
   float* weight_out;
   int heads, blocks;
+  int by_length;               // longest sequences first
   float scale_log2e;
   const float* inv_freq;
   int rope, rotary_dim, pairing;
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS_PER_SM / WARPS) block_attent
   cg::cluster_group cluster = cg::this_cluster();
   const int S = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's first axis
   pdl_launch_dependents();
-  const int kvh = blockIdx.y, t = blockIdx.z, group = p.heads / c.kv_heads;
+  const int kvh = blockIdx.y, t = p.by_length ? rank_th_longest(b, blockIdx.z, reinterpret_cast<int*>(smem_raw)) : blockIdx.z, group = p.heads / c.kv_heads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
   const int s = sequence_of_token(b, t);
   int slot = block_slot(c, b, s, p.err);
@@ -590,6 +591,7 @@ IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatch
     while (splits < 16 && pairs * splits * 2 <= 2LL * sms) splits *= 2;
   }
   BlockTcParams p = {};
+  p.by_length = pairs * splits * warps > (long long)WARPS_PER_SM * sms;
   p.qkv = qkv; p.out = out; p.part = part; p.weight_out = weight_out;
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;

@@ -11,9 +11,10 @@
 //   warps 0-3  softmax, a position per thread: a head's score from its digits, times the block's key scale; the probability times the
 //              block's value scale, as digits, into (swizzled) shared memory.  The references (a maximum per head, a largest value scale) move
 //              only where a fixed-point number would pass 2^31; O is then read out, added up in registers and begun again.
-//   warp 4     TMA producer: page numbers and scales of 32 blocks at a time, one per lane; boxes of up to 128
+//   then       two TMA producers, of keys and of values: page numbers (and scales) of 32 blocks at a time, one per lane; boxes of up to 128
 //              positions, as a page's size allows, into a ring of tiles.
-//   warp 5     MMA issuer: the scores of the next tile, then the weighted sum of this one.
+//   then       two MMA issuers, of the scores and of the weighted sums.  (One warp for both kinds of either took 1,450 cycles a tile: every
+//              product, commit, copy and wait stands in one row there.)
 // A cluster of up to 8 CTAs shares a (sequence, kv head): each takes a run of its blocks and adds up a share of the outputs from what
 // the others have put into its shared memory.  Few long sequences need more CTAs than that to fill the device (an SM reads 42 GB/s at most, and
 // clusters of 16 fit only seven of its eight groups of SMs): theirs are not clusters, put their results into scratch memory, and a
@@ -25,6 +26,8 @@
 // and returns.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+#include <type_traits>
 #include <utility>
 
 #include "block_cache.cuh"
@@ -43,7 +46,7 @@ constexpr uint32_t TMEM_COLS = 128;            // S twice, O once per group
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int P_BITS = 25;                     // a probability of 1 (times the largest value scale) is 2^25; 2^31 is the bound
 constexpr int MAX_RUN = 256;                   // tiles that O adds up at most: 255 * 127 * 128 * 256 < 2^31
-constexpr int WIDE_FROM = 32768;               // positions that a sequence may hold from which few sequences' CTAs are no clusters
+constexpr int WIDE_FROM = 16384;               // positions that a sequence may hold from which few sequences' CTAs are no clusters
 constexpr int TAIL_BLOCKS = 16;                // finished blocks that cost a CTA about as much time as the unfinished one
 
 struct UmmaParams {
@@ -54,6 +57,7 @@ struct UmmaParams {
   float* piece_ml;             // and [T][kv_heads][CTAs][8][2], maximum and sum
   float* weight_out;
   int heads, blocks;
+  int by_length;               // longest sequences first
   int run;                     // blocks of a box: they stand side by side in a page (1, 2, 4 or 8)
   float scale_log2e;
   const float* inv_freq;
@@ -63,7 +67,9 @@ struct UmmaParams {
 };
 
 template <typename T, int GROUPS, int NSTAGE> struct __align__(1024) Shared {
-  static constexpr int SLOTS = 2 * NSTAGE;       // of the tiles' scales: the softmax may read a tile's after its stage is filled again
+  // of the tiles' scales.  Those of tile i are written over when the keys of tile i + 4 have been used, which takes the scores of tile
+  // i + 2 to have been read, by the group that read those of tile i before
+  static constexpr int SLOTS = NSTAGE + 4;
   uint8_t ring[NSTAGE][2][TILE_BYTES];          // keys, values: rows of 128 bytes, 128-byte swizzle
   uint8_t qd[NCOL * HD];                         // digits of the queries: row 8 j + h is digit j of head h
   uint8_t pd[2][NCOL * TILE];                    // digits of the probabilities, likewise
@@ -80,10 +86,10 @@ template <typename T, int GROUPS, int NSTAGE> struct __align__(1024) Shared {
   float wfac[GROUPS + 1][GH];                    // what each of them counts for in the CTA's result
   float lse[GH][2];
   float rs[GH];                                  // what makes scores of the integers
-  float top[GROUPS][4][GH];
+  __align__(16) float top[GROUPS][4][GH];
   float sum[GROUPS][4][GH];
   float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there: key scale NaN of its own kind (see NOWHERE)
-  uint32_t red[GROUPS * 4 + 2];
+  uint32_t red[GROUPS * 4 + 4];
   uint64_t k_full[NSTAGE], v_full[NSTAGE], k_empty[NSTAGE], v_empty[NSTAGE], s_full[2], s_empty[2], p_ready[2], pv_done[2], drained;
   uint32_t tmem;
   int restart[2];
@@ -110,6 +116,13 @@ __device__ __forceinline__ void mma_i8(uint32_t leader, uint32_t d, uint64_t a, 
       "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
       ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(leader) : "memory");
 }
+// A box of rows from `row` on, asked for by the lane of a converged warp whose `who` is set.
+__device__ __forceinline__ void ask(uint32_t who, void* dst, const CUtensorMap* map, uint64_t* bar, int row) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(0), "r"(row), "r"(who) : "memory");
+}
 // s8 x (s8 or u8) -> s32, M x N; A MN-major on request, B K-major.
 __host__ __device__ constexpr uint32_t instr_desc_i8(uint32_t M, uint32_t N, uint32_t b_signed, uint32_t a_mn) {
   return (2u << 4) | (1u << 7) | (b_signed << 10) | (a_mn << 15) | ((N >> 3) << 17) | ((M >> 4) << 24);
@@ -130,6 +143,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   tmem_ld_wait();
 }
 
+// The largest of a number over the warp (NaN apart).
+__device__ __forceinline__ float warp_top(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <typename T>
 __device__ __forceinline__ float head_value(const T* src, int d, const UmmaParams& p, const float* cs) {
   const float x = to_f32(src[d]);
@@ -145,20 +165,21 @@ __device__ __forceinline__ float head_value(const T* src, int d, const UmmaParam
 // an SM where there are CTAs enough, else two groups and a deeper ring in one CTA an SM: a tile takes a group about 1.1 us, an SM's share of the
 // memory's rate brings one in 0.75 us.
 template <typename T, int GROUPS, int NSTAGE, bool WIDE>
-__global__ void __launch_bounds__(GROUPS * SOFT + 64, 3 - GROUPS)
+__global__ void __launch_bounds__(GROUPS * SOFT + 128, 3 - GROUPS)
 block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, UmmaParams p, IertBatchView b,
                             IertBlockView c) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];        // no static shared memory: the window starts 1024-byte aligned
   using Sh = Shared<T, GROUPS, NSTAGE>;
   Sh& sm = *reinterpret_cast<Sh*>(smem_raw);
-  constexpr int THREADS = GROUPS * SOFT + 64, PRODUCER = 4 * GROUPS, ISSUER = PRODUCER + 1, SLOTS = Sh::SLOTS;
-  static_assert(THREADS >= MAX_SPLITS * GH && SLOTS >= NSTAGE + 2, "a thread per (CTA, head); see sm.scale");
+  constexpr int THREADS = GROUPS * SOFT + 128, KEYS = 4 * GROUPS, VALUES = KEYS + 1, SCORES = KEYS + 2, SUMS = KEYS + 3, SLOTS = Sh::SLOTS;
+  static_assert(THREADS >= MAX_SPLITS * GH, "a thread per (CTA, head)");
   constexpr int DIG = sizeof(T) == 4 ? 4 : 3;
   cg::cluster_group cluster = cg::this_cluster();
   const int S = gridDim.x, rank = blockIdx.x;                  // the cluster is the grid's first axis
-  const int kvh = blockIdx.y, t = blockIdx.z, n_g = p.heads / c.kv_heads;
+  const int kvh = blockIdx.y, n_g = p.heads / c.kv_heads;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int t = p.by_length ? rank_th_longest(b, blockIdx.z, reinterpret_cast<int*>(smem_raw)) : blockIdx.z;
   const int s = sequence_of_token(b, t);
   int slot = block_slot(c, b, s, p.err);
   if (slot >= 0 && !block_reaches(c, b.pos0[s], p.err)) slot = -1;
@@ -188,11 +209,11 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   if (tid == 0) {
     for (int i = 0; i < NSTAGE; ++i) { mbar_init(&sm.k_full[i], 1); mbar_init(&sm.v_full[i], 1); mbar_init(&sm.k_empty[i], 1); mbar_init(&sm.v_empty[i], 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(&sm.s_full[i], 1); mbar_init(&sm.s_empty[i], SOFT); mbar_init(&sm.p_ready[i], SOFT); mbar_init(&sm.pv_done[i], 1); }
-    mbar_init(&sm.drained, 1);
+    mbar_init(&sm.drained, 2);
     sm.abort_flag = 0; sm.asked_k = 0; sm.asked_v = 0;
     mbar_fence_init();
   }
-  if (warp == ISSUER) tmem_alloc(&sm.tmem, TMEM_COLS);
+  if (warp == SUMS) tmem_alloc(&sm.tmem, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -200,51 +221,72 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   const uint32_t tmem = sm.tmem, o_col = 2 * NCOL;
   bool ok = true;
 
-  if (warp == PRODUCER) {
-    // ---------------- TMA producer ----------------
-    if (lane == 0) { tma_prefetch_desc(&map_k); tma_prefetch_desc(&map_v); }
+  // ---------------- TMA producers ----------------
+  auto produce = [&](auto values) {
+    constexpr bool V = decltype(values)::value;
+    const CUtensorMap* map = V ? &map_v : &map_k;
+    uint64_t *full = V ? sm.v_full : sm.k_full, *empty = V ? sm.v_empty : sm.k_empty;
+    if (lane == 0) tma_prefetch_desc(map);
+    const uint32_t leader = elect_leader();
+    const int run = p.run, n_box = TILE_BLOCKS / run;
+    // Pages of the 32 blocks after the next and scales of the next 32 are on their way while these 32 are asked for.  Like the step's
+    // description, the page table does not depend on the kernel before.
     auto page_at = [&](int x) { return x < hi ? block_page(c, slot, x / per_page, p.err) : -1; };
-    int page = page_at(lo + lane);                             // like the step's description, the page table does not depend on the kernel before
+    int at_next;
+    float ks_next, vs_next;
+    auto scales_at = [&](int x, int page) {
+      at_next = page >= 0 ? (page * c.kv_heads + kvh) * per_page + x % per_page : -1;
+      if (V) return;
+      ks_next = __uint_as_float(NOWHERE); vs_next = 0.f;
+      if (page >= 0) {
+        ks_next = c.k_scale[at_next];
+        vs_next = c.v_scale[at_next];
+      }
+    };
+    const int page0 = page_at(lo + lane);
+    int page = page_at(lo + 32 + lane);
     pdl_wait();
+    scales_at(lo + lane, page0);
+    int st = 0, slot_i = 0;
+    uint32_t phase = 1;                                        // the stage's use before: there was none in the first round
+    uint8_t* dst = sm.ring[0][V];
     for (int i0 = 0; i0 < n_tiles && ok; i0 += 32 / TILE_BLOCKS) {
       const int x = lo + i0 * TILE_BLOCKS + lane;
-      int at = -1;
-      float ks = __uint_as_float(NOWHERE), vs = 0.f;
-      if (page >= 0) {
-        at = (page * c.kv_heads + kvh) * per_page + x % per_page;
-        ks = c.k_scale[at];
-        vs = c.v_scale[at];
-      }
-      page = page_at(x + 32);                                  // (of the next 32)
-      for (int k = 0; k < 32 / TILE_BLOCKS && i0 + k < n_tiles && ok; ++k) {
-        const int i = i0 + k, st = i % NSTAGE;
-        const uint32_t again = ((i / NSTAGE) - 1) & 1;
-        const bool asks = (lane >> 3) == k && at >= 0 && lane % p.run == 0;        // a lane per box
-        const unsigned here = __ballot_sync(0xffffffffu, asks);
-        if (i >= NSTAGE) ok = wait_bar(&sm.k_empty[st], again, abort_flag);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        if ((lane >> 3) == k) sm.scale[i % SLOTS][lane & 7] = make_float2(ks, vs);
-        __syncwarp();
-        for (int kv = 0; kv < 2; ++kv) {
-          if (kv == 1 && i >= NSTAGE) {
-            ok = wait_bar(&sm.v_empty[st], again, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          }
-          uint64_t* full = kv ? &sm.v_full[st] : &sm.k_full[st];
-          if (lane == 0) {
-            mbar_expect_tx(full, __popc(here) * p.run * BLOCK_BYTES);
-            if (kv) sm.asked_v = i + 1; else sm.asked_k = i + 1;
-          }
-          __syncwarp();
-          if (asks) tma_load_2d(sm.ring[st][kv] + (lane & 7) * BLOCK_BYTES, kv ? &map_v : &map_k, full, 0, at * BLK);
+      const int at = at_next;
+      const float2 scales = make_float2(ks_next, vs_next);
+      scales_at(x + 32, page);
+      page = page_at(x + 64);
+      const unsigned heads_of_boxes = __ballot_sync(0xffffffffu, at >= 0 && (lane & (run - 1)) == 0);
+#pragma unroll 1
+      for (int k = 0; k < 32 / TILE_BLOCKS && i0 + k < n_tiles; ++k) {
+        const int i = i0 + k;
+        if (i >= NSTAGE && !__all_sync(0xffffffffu, wait_bar(&empty[st], phase, abort_flag))) { ok = false; break; }
+        if (!V && (lane >> 3) == k) sm.scale[slot_i][lane & 7] = scales;
+        if (!V) __syncwarp();
+        if (lane == 0) {
+          mbar_expect_tx(&full[st], __popc(heads_of_boxes >> (k * TILE_BLOCKS) & 0xffu) * run * BLOCK_BYTES);
+          if (V) sm.asked_v = i + 1; else sm.asked_k = i + 1;
         }
+        __syncwarp();
+        for (int j = 0; j < n_box; ++j) {
+          const int a = __shfl_sync(0xffffffffu, at, k * TILE_BLOCKS + j * run);
+          ask(leader && a >= 0, dst + j * run * BLOCK_BYTES, map, &full[st], a * BLK);
+        }
+        if (++slot_i == SLOTS) slot_i = 0;
+        dst += 2 * TILE_BYTES;
+        if (++st == NSTAGE) { st = 0; phase ^= 1u; dst = sm.ring[0][V]; }
       }
     }
+  };
+  if (warp == KEYS) {
+    produce(std::false_type());
+  } else if (warp == VALUES) {
+    produce(std::true_type());
   } else {
-    // ---------------- the queries' digits (softmax and MMA warps) ----------------
+    // ---------------- the queries' digits (all warps but the producers) ----------------
     pdl_wait();
-    const int me = warp == ISSUER ? GROUPS * SOFT + lane : tid;
-    constexpr int N = GROUPS * SOFT + 32;
+    const int me = warp > VALUES ? tid - 64 : tid;
+    constexpr int N = GROUPS * SOFT + 64;
     if (p.rope) {
       const float where = (float)(pos + (c.shift ? c.shift[slot] : 0));
       for (int k = me; k < p.rotary_dim / 2; k += N) {
@@ -281,7 +323,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       sm.q[r][d] = r < n_g ? head_value(row + (size_t)r * HD + (size_t)kvh * n_g * HD, d, p, sm.cs) : 0.f;
     }
     early_sync<N>();
-    for (int h = warp == ISSUER ? PRODUCER : warp; h < GH; h += PRODUCER + 1) {       // a warp per head: four numbers a lane
+    for (int h = warp > VALUES ? warp - 2 : warp; h < GH; h += KEYS + 2) {       // a warp per head: four numbers a lane
       const float4 x = *reinterpret_cast<const float4*>(&sm.q[h][4 * lane]);
       uint32_t largest = max(max(abs_bits(x.x), abs_bits(x.y)), max(abs_bits(x.z), abs_bits(x.w)));
 #pragma unroll
@@ -312,34 +354,41 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     fence_proxy_async_smem();
     early_sync<N>();
 
-    if (warp == ISSUER) {
-      // ---------------- MMA issuer (the whole warp, one lane of it acting) ----------------
+    if (warp >= SCORES) {
+      // ---------------- MMA issuers (whole warps, one lane of each acting) ----------------
       constexpr uint32_t IDESC_S = instr_desc_i8(TILE, NCOL, 1, 0), IDESC_O = instr_desc_i8(HD, NCOL, 0, 1);
       const uint32_t leader = elect_leader();
+      const uint32_t ring0 = smem_addr(sm.ring[0][0]);
       auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag)) != 0; };
-      auto scores = [&](int i) {
-        const int st = i % NSTAGE;
-        if (!warp_wait(&sm.k_full[st], (i / NSTAGE) & 1) || (i >= 2 && !warp_wait(&sm.s_empty[i & 1], ((i >> 1) - 1) & 1))) return false;
-        tc_fence_after();
-        const uint64_t kd = smem_desc_k128(smem_addr(sm.ring[st][0])), qd = smem_desc_k128(smem_addr(sm.qd));
+      int st = 0;
+      uint32_t phase = 0;                          // of stage st
+      if (warp == SCORES) {
+        const uint64_t qd = smem_desc_k128(smem_addr(sm.qd));
+        for (int i = 0; i < n_tiles; ++i) {
+          if (!warp_wait(&sm.k_full[st], phase) || (i >= 2 && !warp_wait(&sm.s_empty[i & 1], ((i >> 1) - 1) & 1))) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t kd = smem_desc_k128(ring0 + st * 2 * TILE_BYTES);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + (i & 1) * NCOL, kd + k * 2, qd + k * 2, IDESC_S, k > 0);
-        mma_commit(leader, &sm.s_full[i & 1]);
-        mma_commit(leader, &sm.k_empty[st]);
-        return true;
-      };
-      ok = n_tiles == 0 || scores(0);
-      for (int i = 0; ok && i < n_tiles; ++i) {
-        const int st = i % NSTAGE;
-        if (i + 1 < n_tiles && !scores(i + 1)) { ok = false; break; }
-        if (!warp_wait(&sm.p_ready[i & 1], (i >> 1) & 1) || !warp_wait(&sm.v_full[st], (i / NSTAGE) & 1)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t more = *(volatile int*)&sm.restart[i & 1] ? 0u : 1u;
-        const uint64_t vd = smem_desc_mn128(smem_addr(sm.ring[st][1]), TILE_BYTES), pd = smem_desc_k128(smem_addr(sm.pd[i & 1]));
+          for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + (i & 1) * NCOL, kd + k * 2, qd + k * 2, IDESC_S, k > 0);
+          mma_commit(leader, &sm.s_full[i & 1]);
+          mma_commit(leader, &sm.k_empty[st]);
+          if (++st == NSTAGE) { st = 0; phase ^= 1u; }
+        }
+      } else {
+        const uint64_t pd0 = smem_desc_k128(smem_addr(sm.pd[0]));
+        for (int i = 0; i < n_tiles; ++i) {
+          if (!warp_wait(&sm.v_full[st], phase) || !warp_wait(&sm.p_ready[i & 1], (i >> 1) & 1)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t more = *(volatile int*)&sm.restart[i & 1] ? 0u : 1u;
+          const uint64_t vd = smem_desc_mn128(ring0 + (st * 2 + 1) * TILE_BYTES, TILE_BYTES), pd = pd0 + (i & 1) * (NCOL * TILE >> 4);
+          const uint32_t o = tmem + o_col + (GROUPS == 2 ? (i & 1) * NCOL : 0);
+          mma_i8(leader, o, vd, pd, IDESC_O, more);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_i8(leader, tmem + o_col + (GROUPS == 2 ? (i & 1) * NCOL : 0), vd + k * (32 * HD >> 4), pd + k * 2, IDESC_O, k > 0 ? 1u : more);
-        mma_commit(leader, &sm.pv_done[i & 1]);
-        mma_commit(leader, &sm.v_empty[st]);
+          for (int k = 1; k < 4; ++k) mma_i8(leader, o, vd + k * (32 * HD >> 4), pd + k * 2, IDESC_O, 1u);
+          mma_commit(leader, &sm.pv_done[i & 1]);
+          mma_commit(leader, &sm.v_empty[st]);
+          if (++st == NSTAGE) { st = 0; phase ^= 1u; }
+        }
       }
       mma_commit(leader, &sm.drained);
     } else {
@@ -433,18 +482,17 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         bool far = !ok;
 #pragma unroll
         for (int h = 0; h < GH; ++h) far |= !(y[h] * vu < 2147483648.f) || !(y[h] < 1e30f);
-        if (soft_any(grp, far || run == MAX_RUN)) {       // (the same for all four warps)
-          if (soft_any(grp, !ok)) { ok = false; break; }
+        if (soft_any(grp, far || run == MAX_RUN)) {  // (the same for all four warps)
           // new references: the largest of the tile per head, the largest value scale; what was added up moves to them
           if (run > 0) flush(i - GROUPS);
+          float mx[GH];
 #pragma unroll
-          for (int h = 0; h < GH; ++h) {
-            float mx = v[h];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            if (lane == 0) sm.top[grp][warp & 3][h] = mx;
+          for (int h = 0; h < GH; ++h) mx[h] = warp_top(v[h]);
+          if (lane == 0) {
+            *reinterpret_cast<float4*>(&sm.top[grp][warp & 3][0]) = make_float4(mx[0], mx[1], mx[2], mx[3]);
+            *reinterpret_cast<float4*>(&sm.top[grp][warp & 3][4]) = make_float4(mx[4], mx[5], mx[6], mx[7]);
           }
-          soft_sync(grp);
+          if (soft_any(grp, !ok)) { ok = false; break; }       // (sm.top is written again only behind the next barrier of the group)
           float v_new = v_ref;
 #pragma unroll
           for (int k = 0; k < TILE_BLOCKS; ++k) {
@@ -463,7 +511,6 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
             acc[h] *= alpha * v_move;
             y[h] = v[h] == -INFINITY ? 0.f : ex2(v[h] - to);
           }
-          soft_sync(grp);                             // (sm.top may be written again)
         }
         const float unit = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
         if (i >= 2 && !wait_bar(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, abort_flag)) ok = false;      // the buffer is free
@@ -541,7 +588,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
   }
   if (!WIDE) cluster.barrier_wait(std::move(started));        // every CTA runs
   __syncthreads();
-  if (warp == ISSUER) {
+  if (warp == SUMS) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
@@ -703,7 +750,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, co
     return iert_check_launch("block_attention (shared memory)");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
-  cfg.blockDim = dim3(GROUPS * SOFT + 64);
+  cfg.blockDim = dim3(GROUPS * SOFT + 128);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -723,15 +770,17 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, co
   cudaLaunchKernelEx(&cfg, kernel, mk, mv, p, b, c);
   const int status = iert_check_launch("block_attention");
   if (status || !WIDE) return status;
-  launch_dep(block_attention_umma_merge_kernel<T>, dim3(c.kv_heads, b.n_seqs, 8), dim3(MERGE_THREADS), 0, stream, p, b, c, splits);
+  // a thread per output, and per block where weights are kept: a chain of three loads each (8 CTAs a pair took 10 us for 8,192 blocks)
+  const int Z = c.weight ? std::min(64, std::max(8, p.blocks / MERGE_THREADS)) : 8;
+  launch_dep(block_attention_umma_merge_kernel<T>, dim3(c.kv_heads, b.n_seqs, Z), dim3(MERGE_THREADS), 0, stream, p, b, c, splits);
   return iert_check_launch("block_attention (merge)");
 }
 
 template <typename T>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, int groups, bool wide,
            cudaStream_t stream) {
-  if (wide) return launch<T, 2, 4, true>(mk, mv, p, b, c, splits, stream);
-  return groups == 2 ? launch<T, 2, 4, false>(mk, mv, p, b, c, splits, stream) : launch<T, 1, 2, false>(mk, mv, p, b, c, splits, stream);
+  if (wide) return launch<T, 2, 5, true>(mk, mv, p, b, c, splits, stream);
+  return groups == 2 ? launch<T, 2, 5, false>(mk, mv, p, b, c, splits, stream) : launch<T, 1, 2, false>(mk, mv, p, b, c, splits, stream);
 }
 
 }  // namespace
@@ -766,6 +815,7 @@ IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBat
   CUtensorMap mk, mv;
   const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
   UmmaParams p = {};
+  p.by_length = pairs * splits > (groups == 2 ? sms : 2 * sms);
   p.run = TILE_BLOCKS;
   while ((c.page_tokens / BLK) % p.run) p.run >>= 1;
   if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;

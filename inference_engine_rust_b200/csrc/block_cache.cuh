@@ -76,6 +76,26 @@ __device__ __forceinline__ bool block_reaches(const IertBlockView& c, int pos, i
   return false;
 }
 
+// Which sequence the blocks of threads of grid index `rank` take: the rank-th longest (of equal ones the first), so that those that take long
+// do not begin last.  For a step of more blocks than the device holds at once; the whole block of threads calls it, `len` is room for
+// ORDERED numbers and one more in shared memory.  With more sequences than that: the rank-th.
+constexpr int ORDERED = 256;
+__device__ __forceinline__ int rank_th_longest(const IertBatchView& b, int rank, int* len) {
+  if (b.n_seqs > ORDERED) return rank;
+  for (int i = threadIdx.x; i < b.n_seqs; i += blockDim.x) len[i] = b.slot_ids[i] < 0 ? -1 : b.pos0[i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < b.n_seqs; i += blockDim.x) {
+    const int mine = len[i];
+    int longer = 0;
+    for (int j = 0; j < b.n_seqs; ++j) longer += len[j] > mine || (len[j] == mine && j < i);
+    if (longer == rank) len[ORDERED] = i;
+  }
+  __syncthreads();
+  const int s = len[ORDERED];
+  __syncthreads();
+  return s;
+}
+
 template <int FMT> __device__ __forceinline__ float level_top() { return FMT == IERT_LEVEL_INT8 ? 127.f : 448.f; }
 
 // max |x| over a block from the largest bit pattern of |x|: a NaN is larger than every number, so that it reaches the scale
