@@ -220,7 +220,7 @@ def _declare(lib) -> None:
         "iert_rglru_gates": [P, P, P, P, P, c_int, P, c_float, P, P, c_int, c_int, c_int, S],
         "iert_rglru_scan": [P, P, P, LL, P, P, P, LL, P, c_int, c_float, c_int, c_int, c_int, P, POINTER(BatchView), S],
     })
-    lib.iert_block_attention_scratch.argtypes = [c_int, c_int, POINTER(BlockView)]
+    lib.iert_block_attention_scratch.argtypes = []
     lib.iert_block_attention_scratch.restype = c_longlong
     lib.iert_attention_decode.argtypes = [P, P, POINTER(BatchView), POINTER(KvView), c_int, c_float, c_int, P, P, S]
     lib.iert_attention_decode.restype = c_int
@@ -1301,7 +1301,16 @@ def block_store(qkv, batch: BatchView, view: BlockView, heads: int, err, stream)
 
 def block_attention_scratch_floats(n_seqs: int, heads: int, view: BlockView) -> int:
     """Floats of scratch that `block_attention` needs for steps of up to `n_seqs` sequences."""
-    return core().iert_block_attention_scratch(n_seqs, heads, byref(view))
+    global _piece_floats
+    if _piece_floats is None:
+        _piece_floats = core().iert_block_attention_scratch()
+    if not view.weight:
+        return _piece_floats
+    G = view.kv_heads
+    return _piece_floats + n_seqs * G * -(-heads // G // 8) * 8 * view.table_width * (view.page_tokens // BLOCK_TOKENS)    # heads in slices of eight
+
+
+_piece_floats = None
 
 
 def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,

@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS_PER_SM / WARPS) block_attent
     const int page = block_page(c, slot, nb / per_page, p.err);
     if (page >= 0) {
       const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + nb % per_page;
-      finish_block<FMT>(&sm.tail[0][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.k + i * BLK * HD, c.k_scale + i, sm.red);
-      finish_block<FMT>(&sm.tail[1][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.v + i * BLK * HD, c.v_scale + i, sm.red);
+      finish_block<FMT>(&sm.tail[0][0][0], HD, (uint8_t*)c.k + i * BLK * HD, c.k_scale + i, sm.red);
+      finish_block<FMT>(&sm.tail[1][0][0], HD, (uint8_t*)c.v + i * BLK * HD, c.v_scale + i, sm.red);
     }
   }
 }
@@ -531,9 +531,13 @@ template <int HD, int FMT, typename T, int WARPS>
 int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
   auto kernel = block_attention_tc_kernel<HD, FMT, T, WARPS>;
   const size_t smem = sizeof(Shared<HD, T, WARPS>);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
-    return iert_check_launch("block_attention (attributes)");
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+      return iert_check_launch("block_attention (attributes)");
+    configured = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
   cfg.blockDim = dim3(WARPS * 32);
@@ -559,26 +563,16 @@ int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& 
 
 }  // namespace
 
-long long block_attention_piece_floats();          // block_attention_umma.cu
-
-// Floats of scratch: what CTAs leave for one another, and the blocks' weights, if the view keeps them.
-IERT_API long long iert_block_attention_scratch(int n_seqs, int heads, const IertBlockView* view) {
-  const IertBlockView& c = *view;
-  if (!c.weight || n_seqs <= 0 || c.kv_heads <= 0 || heads <= 0) return block_attention_piece_floats();
-  const long long pairs = (long long)n_seqs * c.kv_heads * ((heads / c.kv_heads + GH - 1) / GH);
-  return block_attention_piece_floats() + pairs * c.table_width * (c.page_tokens / BLK) * GH;
-}
-
 // `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head, and `warps` (4, 8, 16) of each; 0: by the rule below.
 IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
-                                     float* part, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
+                                     float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
                                      int warps, int* err, cudaStream_t stream) {
   if (batch->n_tokens <= 0) return IERT_OK;
   const IertBlockView& c = *view;
   if ((c.head_dim != 64 && c.head_dim != 128) || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || batch->n_tokens != batch->n_seqs ||
       batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 || c.ring_pages <= 0 ||
       c.ring_pages > c.table_width || c.n_pages <= 0 || c.n_slots <= 0 || c.window < 0 ||
-      (c.weight && (c.window || !part || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)part) % 16 ||
+      !scratch || (c.weight && (c.window || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)scratch) % 16 ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > c.head_dim || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
     return IERT_BAD_ARGUMENT;
   if (warps != 0 && warps != 4 && warps != 8 && warps != 16) return IERT_BAD_ARGUMENT;
@@ -592,7 +586,7 @@ IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatch
   }
   BlockTcParams p = {};
   p.by_length = pairs * splits * warps > (long long)WARPS_PER_SM * sms;
-  p.qkv = qkv; p.out = out; p.part = part; p.weight_out = weight_out;
+  p.qkv = qkv; p.out = out; p.part = scratch; p.weight_out = weight_out;
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;

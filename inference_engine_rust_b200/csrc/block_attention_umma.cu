@@ -665,8 +665,8 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
     const int page = block_page(c, slot, nb / per_page, p.err);
     if (page >= 0) {
       const size_t i = ((size_t)page * c.kv_heads + kvh) * per_page + nb % per_page;
-      finish_block<IERT_LEVEL_INT8>(&sm.tail[0][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.k + i * BLK * HD, c.k_scale + i, sm.red);
-      finish_block<IERT_LEVEL_INT8>(&sm.tail[1][0][0], (const T*)nullptr, 0, BLK, HD, (uint8_t*)c.v + i * BLK * HD, c.v_scale + i, sm.red);
+      finish_block<IERT_LEVEL_INT8>(&sm.tail[0][0][0], HD, (uint8_t*)c.k + i * BLK * HD, c.k_scale + i, sm.red);
+      finish_block<IERT_LEVEL_INT8>(&sm.tail[1][0][0], HD, (uint8_t*)c.v + i * BLK * HD, c.v_scale + i, sm.red);
     }
   }
 }
@@ -746,8 +746,12 @@ template <typename T, int GROUPS, int NSTAGE, bool WIDE>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
   auto kernel = block_attention_umma_kernel<T, GROUPS, NSTAGE, WIDE>;
   const size_t smem = sizeof(Shared<T, GROUPS, NSTAGE>);
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
-    return iert_check_launch("block_attention (shared memory)");
+  static bool configured = false;
+  if (!configured) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+      return iert_check_launch("block_attention (shared memory)");
+    configured = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
   cfg.blockDim = dim3(GROUPS * SOFT + 128);
@@ -785,8 +789,8 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, co
 
 }  // namespace
 
-// Floats of scratch in front of the blocks' weights (block_attention_tc.cu).
-long long block_attention_piece_floats() { return (long long)MAX_PIECES * GH * (HD + 2); }
+// Floats of scratch for what the CTAs of a step leave for one another, in front of the blocks' weights.
+IERT_API long long iert_block_attention_scratch() { return (long long)MAX_PIECES * GH * (HD + 2); }
 
 // `splits`: CTAs that share a sequence's kv head (1, 2, 4, 8: a cluster; more: not); `groups` (1, 2) of softmax warps in each; 0: by the rule below.
 IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
@@ -820,7 +824,7 @@ IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBat
   while ((c.page_tokens / BLK) % p.run) p.run >>= 1;
   if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;
   p.qkv = qkv; p.out = out; p.weight_out = weight_out;
-  p.piece_o = scratch; p.piece_ml = scratch + (long long)MAX_PIECES * GH * HD; p.part = scratch + block_attention_piece_floats();
+  p.piece_o = scratch; p.piece_ml = scratch + (long long)MAX_PIECES * GH * HD; p.part = scratch + iert_block_attention_scratch();
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;

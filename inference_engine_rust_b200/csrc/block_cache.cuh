@@ -129,18 +129,13 @@ __device__ __forceinline__ uint32_t block_max_bits(uint32_t v, uint32_t* red) {
   return v;
 }
 
-// The whole block of threads turns 16 rows into levels and their scale: row r is rows[r] of the tail (r < n_old) or, from n_old
-// on, `fresh` + (r - n_old) * ld.
+// The whole block of threads turns the 16 rows of a tail into levels and their scale.
 template <int FMT, typename T>
-__device__ void finish_block(const T* tail, const T* fresh, long long ld, int n_old, int hd, uint8_t* levels, float* scale, uint32_t* red) {
-  auto value = [&](int i) {
-    const int r = i / hd, d = i - r * hd;
-    return to_f32(r < n_old ? tail[r * hd + d] : fresh[(long long)(r - n_old) * ld + d]);
-  };
+__device__ void finish_block(const T* tail, int hd, uint8_t* levels, float* scale, uint32_t* red) {
   uint32_t largest = 0;
-  for (int i = threadIdx.x; i < BLK * hd; i += blockDim.x) largest = max(largest, abs_bits(value(i)));
+  for (int i = threadIdx.x; i < BLK * hd; i += blockDim.x) largest = max(largest, abs_bits(to_f32(tail[i])));
   const float s = block_scale<FMT>(block_max_bits(largest, red));
-  for (int i = threadIdx.x; i < BLK * hd; i += blockDim.x) levels[i] = to_level<FMT>(value(i), s);
+  for (int i = threadIdx.x; i < BLK * hd; i += blockDim.x) levels[i] = to_level<FMT>(to_f32(tail[i]), s);
   if (threadIdx.x == 0) *scale = s;
 }
 

@@ -3,8 +3,10 @@
 //   i among the history's answer, c > 0 times: x - freq * c - pres       (products and differences rounded one by one, in this order)
 //   x + bias[i];  -infinity where the mask has no bit for i
 // A cluster of eight CTAs shares a row: each owns an eighth of the vocabulary, counts the history's tokens that fall into it in
-// shared memory, applies the rules to its logits as they stream by and keeps the best; the eight bests meet in the first CTA's
+// shared memory, applies the rules to its logits and keeps the best; the eight bests meet in the first CTA's
 // shared memory, which appends the choice to the row's history.  One launch, and nothing but the logits crosses the memory.
+// Its bound is the logits' way from and to memory, so a thread asks for all its logits of a window (32) before the counting begins,
+// which they cross meanwhile; 64 rows of 131,072 took 38 us with four at a time behind it.
 #include <cooperative_groups.h>
 
 #include <utility>
@@ -17,8 +19,8 @@ using namespace iert;
 namespace {
 
 constexpr int THREADS = 512, CLUSTER = 8;
-constexpr int WINDOW = 24576;                 // ids whose counts stand in shared memory at a time (96 KB)
-constexpr uint32_t SEEN = 0x80000000u;
+constexpr int PER_THREAD = 32;                // logits of a thread in a window
+constexpr int WINDOW = THREADS * PER_THREAD;  // ids whose counts stand in shared memory at a time
 
 struct RulesParams {
   const float* logits; long long ld;
@@ -32,14 +34,20 @@ struct RulesParams {
   const uint32_t* mask; long long ld_mask;    // words of 32 ids, bit i % 32 of word i / 32; ld 0: one row for all
   int* chosen;                                // null: no choice is made
   int* lens_out;                              // null: nothing is appended
-  int chunk, vec;
+  int chunk;
   int* err;
 };
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
 
-__global__ void __launch_bounds__(THREADS) logit_rules_kernel(RulesParams p) {
-  extern __shared__ uint32_t counts[];
+// Count: 16-bit words serve histories of up to 32,767 tokens (32 KB a window), 32-bit words longer ones.  The highest bit: seen at all.
+// VEC: rows, biases and results in 16-byte runs.
+template <typename Count, bool VEC>
+__global__ void __launch_bounds__(THREADS, 2) logit_rules_kernel(RulesParams p) {
+  extern __shared__ uint32_t words[];
+  constexpr int PER_WORD = 4 / sizeof(Count);
+  constexpr uint32_t SEEN = 1u << (8 * sizeof(Count) - 1);
+  const Count* counts = reinterpret_cast<const Count*>(words);
   __shared__ float vs[THREADS / 32];
   __shared__ int is[THREADS / 32];
   __shared__ float best_v[CLUSTER];
@@ -50,6 +58,28 @@ __global__ void __launch_bounds__(THREADS) logit_rules_kernel(RulesParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int rank = cluster.block_rank(), r = blockIdx.x / CLUSTER, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float* row = p.logits + (long long)r * p.ld;
+  float* out = p.out ? p.out + (long long)r * p.ld_out : nullptr;
+  const float* bias = p.bias ? p.bias + (long long)r * p.ld_bias : nullptr;
+  const uint32_t* mask = p.mask ? p.mask + (long long)r * p.ld_mask : nullptr;
+  const int lo = min(p.vocab, rank * p.chunk), hi = min(p.vocab, lo + p.chunk);
+  // the k-th number of a thread in the window that begins with w0 (VEC: four neighbours at a time)
+  auto id_of = [&](int w0, int k) { return VEC ? w0 + 4 * (tid + (k >> 2) * THREADS) + (k & 3) : w0 + tid + k * THREADS; };
+  float x[PER_THREAD];
+  auto load = [&](int w0, int w1) {
+#pragma unroll
+    for (int k = 0; k < PER_THREAD; k += VEC ? 4 : 1) {
+      const int i = id_of(w0, k);
+      if (i >= w1) continue;
+      if (VEC) {
+        const float4 f = *reinterpret_cast<const float4*>(row + i);
+        x[k] = f.x; x[k + 1] = f.y; x[k + 2] = f.z; x[k + 3] = f.w;
+      } else {
+        x[k] = row[i];
+      }
+    }
+  };
+  load(lo, min(hi, lo + WINDOW));
   int h = p.rows ? p.rows[r] : r;
   if (h < 0 || h >= p.hist_rows) {            // no such history: the row is treated as one without
     if (p.hist_rows > 0 && rank == 0 && tid == 0) atomicOr(p.err, IERT_ERR_HISTORY);
@@ -59,58 +89,70 @@ __global__ void __launch_bounds__(THREADS) logit_rules_kernel(RulesParams p) {
   const int prompt = h >= 0 ? p.prompt_lens[h] : 0;
   const bool counted = p.penalties && h >= 0;
   const float rep = counted ? p.penalties[3 * h] : 1.f, pres = counted ? p.penalties[3 * h + 1] : 0.f, freq = counted ? p.penalties[3 * h + 2] : 0.f;
-  const float* row = p.logits + (long long)r * p.ld;
-  float* out = p.out ? p.out + (long long)r * p.ld_out : nullptr;
-  const float* bias = p.bias ? p.bias + (long long)r * p.ld_bias : nullptr;
-  const uint32_t* mask = p.mask ? p.mask + (long long)r * p.ld_mask : nullptr;
   const int* hist = p.history + (long long)max(h, 0) * p.width;
-  const int lo = min(p.vocab, rank * p.chunk), hi = min(p.vocab, lo + p.chunk);
 
   float bv = -INFINITY;
   int bi = 0x7fffffff;
   bool bad = false;
-  auto rule = [&](float x, uint32_t c, int i, float b, bool allowed) {
-    if (allowed && !isfinite(x)) bad = true;  // the model's logits are finite, as for the samplers
-    if (c) x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+  auto rule = [&](float y, uint32_t c, int i, float b, bool allowed) {
+    if (allowed && !isfinite(y)) bad = true;  // the model's logits are finite, as for the samplers
+    if (c) y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
     c &= ~SEEN;
-    if (c) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)c)), pres);
-    if (bias) x = __fadd_rn(x, b);
-    if (!allowed) x = -INFINITY;
-    else if (!(x < INFINITY)) bad = true;     // a bias of -infinity rules an id out; one of +infinity or NaN is a mistake
-    if (x > -INFINITY && better(x, i, bv, bi)) { bv = x; bi = i; }
-    return x;
+    if (c) y = __fsub_rn(__fsub_rn(y, __fmul_rn(freq, (float)c)), pres);
+    if (bias) y = __fadd_rn(y, b);
+    if (!allowed) y = -INFINITY;
+    else if (!(y < INFINITY)) bad = true;     // a bias of -infinity rules an id out; one of +infinity or NaN is a mistake
+    if (y > -INFINITY && better(y, i, bv, bi)) { bv = y; bi = i; }
+    return y;
   };
   for (int w0 = lo; w0 < hi; w0 += WINDOW) {
     const int w1 = min(hi, w0 + WINDOW);
+    if (w0 > lo) load(w0, w1);
     if (counted) {
       __syncthreads();                        // the counts of the window before are read
-      for (int i = tid; i < w1 - w0; i += THREADS) counts[i] = 0;
+      for (int i = tid; i < (w1 - w0 + 4 * PER_WORD - 1) / (4 * PER_WORD); i += THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0, 0, 0, 0);
       __syncthreads();
+#pragma unroll 4
       for (int j = tid; j < len; j += THREADS) {
         const int id = hist[j] - w0;
         if (id >= 0 && id < w1 - w0) {
-          if (j >= prompt) atomicAdd(&counts[id], 1u); else atomicOr(&counts[id], SEEN);
+          const int shift = PER_WORD == 1 ? 0 : 16 * (id % PER_WORD);
+          if (j >= prompt) atomicAdd(&words[id / PER_WORD], 1u << shift); else atomicOr(&words[id / PER_WORD], SEEN << shift);
         }
       }
       __syncthreads();
     }
-    if (p.vec) {
-      for (int i = w0 + 4 * tid; i < w1; i += 4 * THREADS) {      // chunks, windows and rows are whole runs of four here
-        const float4 x = *reinterpret_cast<const float4*>(row + i);
-        const uint4 c = counted ? *reinterpret_cast<const uint4*>(counts + (i - w0)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < PER_THREAD; k += 4) {
+      if (VEC) {
+        const int i = id_of(w0, k);
+        if (i >= w1) continue;
+        uint32_t c[4] = {0, 0, 0, 0};
+        if (counted) {
+          if (PER_WORD == 2) {
+            const uint2 q = *reinterpret_cast<const uint2*>(counts + (i - w0));
+            c[0] = q.x & 0xffffu; c[1] = q.x >> 16; c[2] = q.y & 0xffffu; c[3] = q.y >> 16;
+          } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(counts + (i - w0));
+            c[0] = q.x; c[1] = q.y; c[2] = q.z; c[3] = q.w;
+          }
+        }
         const float4 b = bias ? __ldg(reinterpret_cast<const float4*>(bias + i)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const uint32_t m = mask ? mask[i >> 5] >> (i & 31) : 0xfu;
+        const uint32_t m = mask ? __ldg(mask + (i >> 5)) >> (i & 31) : 0xfu;
         float4 y;
-        y.x = rule(x.x, c.x, i, b.x, m & 1);
-        y.y = rule(x.y, c.y, i + 1, b.y, m & 2);
-        y.z = rule(x.z, c.z, i + 2, b.z, m & 4);
-        y.w = rule(x.w, c.w, i + 3, b.w, m & 8);
+        y.x = rule(x[k], c[0], i, b.x, m & 1);
+        y.y = rule(x[k + 1], c[1], i + 1, b.y, m & 2);
+        y.z = rule(x[k + 2], c[2], i + 2, b.z, m & 4);
+        y.w = rule(x[k + 3], c[3], i + 3, b.w, m & 8);
         if (out) *reinterpret_cast<float4*>(out + i) = y;
-      }
-    } else {
-      for (int i = w0 + tid; i < w1; i += THREADS) {
-        const float y = rule(row[i], counted ? counts[i - w0] : 0u, i, bias ? bias[i] : 0.f, !mask || ((mask[i >> 5] >> (i & 31)) & 1));
-        if (out) out[i] = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = id_of(w0, k + e);
+          if (i >= w1) continue;
+          const float y = rule(x[k + e], counted ? (uint32_t)counts[i - w0] : 0u, i, bias ? __ldg(bias + i) : 0.f, !mask || ((__ldg(mask + (i >> 5)) >> (i & 31)) & 1));
+          if (out) out[i] = y;
+        }
       }
     }
   }
@@ -178,10 +220,13 @@ IERT_API int iert_logit_rules(const float* logits, int rows_n, int vocab, long l
   const long long chunk = (((long long)vocab + CLUSTER - 1) / CLUSTER + 127) / 128 * 128;
   p.chunk = (int)(chunk < 0x7fffff80LL / CLUSTER ? chunk : 0x7fffff80LL / CLUSTER / 128 * 128);
   if ((long long)p.chunk * CLUSTER < vocab) return IERT_BAD_ARGUMENT;
-  p.vec = vocab % 4 == 0 && ld % 4 == 0 && (uintptr_t)logits % 16 == 0 && (!out || (ld_out % 4 == 0 && (uintptr_t)out % 16 == 0)) &&
-          (!bias || (ld_bias % 4 == 0 && (uintptr_t)bias % 16 == 0));
-  const size_t smem = penalties ? sizeof(uint32_t) * (size_t)(p.chunk < WINDOW ? p.chunk : WINDOW) : 0;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(logit_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const bool vec = vocab % 4 == 0 && ld % 4 == 0 && (uintptr_t)logits % 16 == 0 && (!out || (ld_out % 4 == 0 && (uintptr_t)out % 16 == 0)) &&
+                   (!bias || (ld_bias % 4 == 0 && (uintptr_t)bias % 16 == 0));
+  const bool small = width < 32768;
+  const size_t smem = penalties ? (small ? 2 : 4) * (size_t)(p.chunk < WINDOW ? p.chunk : WINDOW) : 0;
+  auto kernel = small ? (vec ? logit_rules_kernel<uint16_t, true> : logit_rules_kernel<uint16_t, false>)
+                      : (vec ? logit_rules_kernel<uint32_t, true> : logit_rules_kernel<uint32_t, false>);
+  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows_n * CLUSTER));
   cfg.blockDim = dim3(THREADS);
@@ -194,7 +239,7 @@ IERT_API int iert_logit_rules(const float* logits, int rows_n, int vocab, long l
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = iert_pdl_enabled ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, logit_rules_kernel, p);
+  cudaLaunchKernelEx(&cfg, kernel, p);
   return iert_check_launch("logit_rules");
 }
 

@@ -181,7 +181,19 @@ def test_what_sets_the_error_word():
 
 def test_counts_in_more_than_one_window():
     """A vocabulary whose eighth is larger than the counts that stand in shared memory at a time."""
-    c = Case(1, 8 * 24576 + 1000, width=3000, seed=9)
+    for pad in (0, 1):
+        c = Case(1, 8 * 24576 + 1000, width=3000, seed=9, pad=pad)
+        c.check(c.run(), c.logits.cpu().numpy())
+
+
+@pytest.mark.parametrize("width", [32767, 32768, 40000])
+@pytest.mark.parametrize("V", [1000, 1001])
+def test_histories_whose_counts_need_more_than_fifteen_bits(width, V):
+    """One id stands in nearly all places of the longest histories: its count is right on both sides of the border between word sizes."""
+    c = Case(2, V, width=width, seed=11)
+    c.lens[c.rows] = width - 1
+    c.prompt[c.rows] = [0, 5]
+    c.history[:, 3:] = 77
     c.check(c.run(), c.logits.cpu().numpy())
 
 
