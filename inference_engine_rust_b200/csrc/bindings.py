@@ -1292,7 +1292,8 @@ def _packed_rows(qkv, heads: int, view: BlockView) -> None:
 
 def block_store(qkv, batch: BatchView, view: BlockView, heads: int, err, stream) -> None:
     """Write the keys and values of the step's tokens (packed [T, heads | kv_heads | kv_heads] x head_dim, as they stand) into the
-    cache: finished blocks as levels and scales, the rest of a sequence as it is; the weights of blocks that begin here are set to 0."""
+    cache: finished blocks as levels and scales, the rest of a sequence as it is; the weights of blocks that begin here are set to 0.
+    The slots of a step are all different.  Batch and page table are read while the kernel in front may still run: it must not write them."""
     _packed_rows(qkv, heads, view)
     _need(qkv.shape[0] >= batch.n_tokens, "fewer rows than tokens")
     _on_current_device(qkv, view.tensors[0], err)
@@ -1316,7 +1317,8 @@ _piece_floats = None
 def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,
                     weight_out=None, plain: bool = False, splits: int = 0, warps: int = 0, groups: int = 0) -> None:
     """One-token attention over the 8-bit cache, which the step's own key and value join; `out` [n_seqs, heads * head_dim] of the
-    projection's type (rows of padding sequences: 0).
+    projection's type (rows of padding sequences: 0).  The slots of a step are all different, and steps that may run at the same time
+    need scratch of their own.  Batch and page table are read while the kernel in front may still run: it must not write them.
 
     rope         (inv_freq, rotary_dim, pairing, factor): the kernel rotates queries and the new key by the position, evicted ones included
     weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
@@ -1361,9 +1363,10 @@ def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, 
     equal ones the lower index), in their order, copied with scales and weights to `new_pages`; the weight of an unfinished block goes along.
 
     k, v, k_scale, v_scale, weight   the pools of all layers, as `block_view` takes them with an axis of layers in front
-    page_table     int32 [rows, width]; sequence i is row slots[i] (slots int32 [n], None: row i)
+    page_table     int32 [rows, width]; sequence i is row slots[i] (slots int32 [n], all different; None: row i)
     lengths        int32 [n]: positions that each sequence holds; one with at most `keep` finished blocks keeps them all
-    new_pages      int32 [n, >= keep * 16 / page_tokens, and room for the unfinished block]: pages that no sequence uses, all different
+    new_pages      int32 [n, >= keep * 16 / page_tokens, and room for the unfinished block (an error bit where it lacks)]: pages that no
+                   sequence uses, all different
     kept           int32 [layers, n, kv_heads, keep]: the numbers of the kept blocks (-1 behind the last of a sequence with fewer)
     shift          int32 [rows] or None: grows by the positions that a sequence loses
     """

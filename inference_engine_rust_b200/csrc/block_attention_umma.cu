@@ -810,7 +810,7 @@ IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBat
   const int sms = iert_sm_count_cached();
   if (splits == 0) {
     const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
-    if (pairs * 2 * MAX_SPLITS <= sms && reach >= WIDE_FROM) splits = (int)(sms / pairs);
+    if (pairs * 2 * MAX_SPLITS <= sms && reach >= WIDE_FROM) splits = (int)(std::min(sms, MAX_PIECES) / pairs);
     else
       for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= sms;) splits *= 2;
   }

@@ -14,7 +14,7 @@ namespace {
 // positions, kv head), half of it for the keys and half for the values.  The blocks of sequence s are the units [cu_q[s] / 16 + 2 s, ...): q
 // tokens touch at most q / 16 + 2 blocks.  A step reads and writes each number once, and its time is that of one chain of loads: so a
 // thread asks for all its numbers (VEC: eight at a time, `RUNS` runs of them), keeps them in registers over the search for the
-// largest, and writes their levels (2,048 tokens of 8 heads of 128 take 5 us, 38 with two passes of single numbers).
+// largest, and writes their levels (2,048 tokens of 8 heads of 128 take 7 us, 38 with two passes of single numbers).
 constexpr int STORE_THREADS = 128, HALF = STORE_THREADS / 2;
 
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
@@ -51,11 +51,11 @@ __global__ void __launch_bounds__(STORE_THREADS) block_store_kernel(const T* __r
     if (b.cu_q[mid] / BLK + 2 * mid <= u) lo = mid; else hi = mid;
   }
   const int s = lo, slot = block_slot(c, b, s, err);
-  if (slot < 0 || b.pos0[s] < 0) return;
+  if (slot < 0 || b.pos0[s] < 0) { pdl_wait(); return; }     // (a kernel that ends before the one in front of it would let the next one pass both)
   const int p0 = b.pos0[s], q0 = b.cu_q[s], end = p0 + b.cu_q[s + 1] - q0;
   const int first = p0 / BLK, blk = first + u - (q0 / BLK + 2 * s), open = end / BLK;     // `open`: the block that stays unfinished, if any
-  if (blk * BLK >= end || end == p0) return;
   pdl_wait();
+  if (blk * BLK >= end || end == p0) return;
   const long long ld = (long long)(heads + 2 * c.kv_heads) * hd;
   const size_t t_off = ((size_t)slot * c.kv_heads + h) * BLK * hd;
   const int v = threadIdx.x / HALF, me = threadIdx.x % HALF;                              // keys or values

@@ -46,9 +46,11 @@ __device__ __forceinline__ int evict_blocks(const EvictParams& p, int i) {
   return min(max(p.lengths[i], 0) / BLK, min(p.max_blocks, p.width * p.per_page));
 }
 
-// Which blocks stay: one CTA per (kv head, sequence, layer).  The keys stand in shared memory; the key of rank `need` is found
-// eight bits at a time from counts of its leading digits (four passes, whole-number counts: the order of the additions cannot
-// matter), then one ordered pass writes the numbers of the blocks above it, of as many equal ones as are missing, and of the last.
+// Which blocks stay: one CTA per (kv head, sequence, layer).  The keys stand in shared memory (STAGED; where they do not fit, in memory
+// only, and are looked up again in each pass); the key of rank `need` is found eight bits at a time from counts of its leading digits (four
+// passes, whole-number counts: the order of the additions cannot matter), then one ordered pass writes the numbers of the blocks above
+// it, of as many equal ones as are missing, and of the last.
+template <bool STAGED>
 __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictParams p) {
   extern __shared__ uint32_t keys[];
   __shared__ int hist[256], warp_gt[SELECT_THREADS / 32], warp_eq[SELECT_THREADS / 32], found[2];
@@ -65,16 +67,19 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictParam
   const int cand = nb - p.recent;                        // recent <= keep < nb
   int need = p.keep - p.recent;                          // this many of the first `cand`
   const float* w = p.weight + (size_t)layer * p.n_pages * p.kv_heads * p.per_page;
-  for (int x = tid; x < cand; x += SELECT_THREADS) {
+  auto look_up = [&](int x) {
     const int page = evict_page(p, row, x);
-    keys[x] = page < 0 ? 0u : weight_key(w[((size_t)page * p.kv_heads + h) * p.per_page + x % p.per_page]);
-  }
+    return page < 0 ? 0u : weight_key(w[((size_t)page * p.kv_heads + h) * p.per_page + x % p.per_page]);
+  };
+  if (STAGED)
+    for (int x = tid; x < cand; x += SELECT_THREADS) keys[x] = look_up(x);       // (read again by the thread that wrote it)
+  auto key = [&](int x) { return STAGED ? keys[x] : look_up(x); };
   uint32_t prefix = 0;
   for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
     for (int x = tid; x < 256; x += SELECT_THREADS) hist[x] = 0;
     __syncthreads();
     for (int x = tid; x < cand; x += SELECT_THREADS) {
-      const uint32_t k = keys[x];
+      const uint32_t k = key(x);
       if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
     }
     __syncthreads();
@@ -105,7 +110,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictParam
   int written = 0, equal = 0;                            // so far, over the whole block
   for (int base = 0; base < nb; base += SELECT_THREADS) {
     const int x = base + tid;
-    const uint32_t k = x < cand && any ? keys[x] : 0;
+    const uint32_t k = x < cand && any ? key(x) : 0;
     const bool gt = (x < cand && any && k > prefix) || (x >= cand && x < nb), eq = x < cand && any && k == prefix;
     const unsigned bq = __ballot_sync(0xffffffffu, eq);
     if (lane == 0) warp_eq[warp] = __popc(bq);
@@ -160,7 +165,10 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, CopyPara
     to = x;
     if (from < 0 || from >= nb) return;
   }
-  if (to / p.per_page >= p.new_width) return;
+  if (to / p.per_page >= p.new_width) {                // no room for the unfinished block
+    if (lane == 0) atomicOr(p.err, IERT_ERR_PAGE_RANGE);
+    return;
+  }
   const int src = evict_page(p, row, from), dst = p.new_pages[(size_t)i * p.new_width + to / p.per_page];
   if (src < 0) return;
   if (dst < 0 || dst >= p.n_pages) {
@@ -201,14 +209,15 @@ IERT_API int iert_block_evict(void* k, void* v, float* k_scale, float* v_scale, 
   if (n_pages <= 0 || kv_heads <= 0 || page_tokens <= 0 || page_tokens % BLK || head_dim <= 0 || width <= 0 || rows <= 0 || keep <= 0 || recent < 0 ||
       recent > keep || max_blocks <= 0 || n > 65535 || layers > 65535 || (long long)new_width * page_tokens < (long long)keep * BLK)
     return IERT_BAD_ARGUMENT;
-  const size_t smem = (size_t)max_blocks * sizeof(uint32_t);
-  if (smem > 200 * 1024) return IERT_BAD_ARGUMENT;
+  const bool staged = max_blocks <= 50 * 1024;
+  const size_t smem = staged ? (size_t)max_blocks * sizeof(uint32_t) : 0;
   EvictParams p = {};
   p.weight = weight; p.table = table; p.slots = slots; p.lengths = lengths; p.new_pages = new_pages; p.kept = kept; p.shift = shift;
   p.n = n; p.layers = layers; p.n_pages = n_pages; p.kv_heads = kv_heads; p.per_page = page_tokens / BLK; p.width = width; p.rows = rows;
   p.new_width = new_width; p.keep = keep; p.recent = recent; p.max_blocks = max_blocks; p.err = err;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  evict_select_kernel<<<dim3(kv_heads, n, layers), SELECT_THREADS, smem, stream>>>(p);
+  if (smem > 40 * 1024) cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (staged) evict_select_kernel<true><<<dim3(kv_heads, n, layers), SELECT_THREADS, smem, stream>>>(p);
+  else evict_select_kernel<false><<<dim3(kv_heads, n, layers), SELECT_THREADS, 0, stream>>>(p);
   const int status = iert_check_launch("block_evict (choice)");
   if (status) return status;
   CopyParams q = {(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, BLK * head_dim};

@@ -416,3 +416,124 @@ def test_equal_calls_give_equal_bits(plain):
         got.append((r.step(slots, plain=plain), torch.nan_to_num(r.weight)))
     for o, w in got[1:]:
         assert torch.equal(o, got[0][0]) and torch.equal(w, got[0][1])
+
+
+def test_more_tiles_than_a_sum_of_integers_may_take():
+    """40,000 positions done by one CTA: the 32-bit sums of products of levels and digits are emptied on the way."""
+    r = Rig(1, 3, 128, torch.int8, torch.bfloat16, n_slots=1, width=626, weights=True, seed=17)
+    r.store([0], [40_000])
+    r.blocks_weight[0] = [torch.zeros(1, dtype=torch.float64) for _ in range(2500)]
+    r.step([0], plain=False, splits=1, groups=1)
+
+
+def test_values_and_probabilities_at_their_largest():
+    """Every probability alike and every value's level 127 (or -127): the largest sums there are.  The answer is the value itself: levels
+    and scale give it back with the rounding of the scale and of one product."""
+    b = B()
+    r = Rig(1, 8, 128, torch.int8, torch.float32, n_slots=1, width=626, seed=18)
+    x = torch.zeros(40_001, 10, 128)
+    x[:, 9, ::2], x[:, 9, 1::2] = 3.7, -3.7
+    x = x.reshape(40_001, -1).to(DEV)
+    view, keep = r.batch([0], [40_000], [0])
+    b.block_store(x[:40_000], view, r.view, 8, r.err, b.stream_ptr())
+    view, keep = r.batch([0], [1], [40_000])
+    out, scratch = torch.empty(1, 1024, device=DEV), torch.empty(b.block_attention_scratch_floats(1, 8, r.view), device=DEV)
+    b.block_attention(x[40_000:], out, view, r.view, 8, 1.0, scratch, r.err, b.stream_ptr(), splits=1, groups=1)
+    want = x[40_000:, -128:].repeat(1, 8)
+    # scale, product and quotient; the sum of 40,000 weights in one CTA: below 320 additions a thread, then 7 of partial sums, and as many of the outputs
+    assert (out - want).abs().max().item() <= 3.7 * (2 * 330 + 6) * 2.0 ** -24
+    assert r.err.item() == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("G, n", [(2, 160), (1, 300)])
+def test_more_sequences_than_run_at_once(fmt, G, n):
+    """The longest first where they can be put in order (up to 256), as they stand where not."""
+    r = Rig(G, 4, 128, fmt, torch.bfloat16, n_slots=n, width=4, weights=True, seed=n)
+    g = np.random.default_rng(n)
+    slots, lens = list(g.permutation(n)), g.integers(1, 250, n)
+    lens[:5] = 200                                    # equal ones
+    r.store(slots, list(lens))
+    for s, x in zip(slots, lens):
+        r.blocks_weight[s] = [torch.zeros(G, dtype=torch.float64) for _ in range(-(-int(x) // BLOCK))]
+    r.step(slots, plain=False, pad=5)
+    r.check_content(slots)
+
+
+def test_a_table_that_reaches_far():
+    """Few sequences that may become long: CTAs that are no cluster, and a second kernel, by the kernel's own rule."""
+    r = Rig(1, 5, 128, torch.int8, torch.bfloat16, n_slots=3, width=260, weights=True, seed=19)
+    r.store([2, 0], [3000, 15])
+    r.blocks_weight = {s: [torch.zeros(1, dtype=torch.float64) for _ in range(-(-n // BLOCK))] for s, n in ((2, 3000), (0, 15))}
+    for pad in (0, 1):
+        r.step([2, 0, 1], plain=False, pad=pad)
+    r.check_content([0, 1, 2])
+
+
+@pytest.mark.parametrize("groups, splits", [(1, 2), (2, 1), (2, 9)])
+def test_bad_pages_and_numbers_where_integers_are_multiplied(groups, splits):
+    """Heads of 128 over int8 levels: a page that is not there counts for nothing and sets the error word, a scale that is no number
+    reaches the heads of its key head alone."""
+    b = B()
+    r = Rig(2, 8, 128, torch.int8, torch.bfloat16, n_slots=3, width=5, weights=True, seed=20)
+    r.store([0, 1, 2], [300, 300, 300])
+    r.weight.zero_()
+    good, x = r.table.clone(), r.rows(3).reshape(3, -1).to(DEV)
+    scratch = torch.zeros(b.block_attention_scratch_floats(3, 8, r.view), device=DEV)
+
+    def go(slots, pos):
+        view, keep = r.batch(slots, [1] * len(slots), pos)
+        out = torch.full((len(slots), 8 * 128), 7.0, dtype=torch.bfloat16, device=DEV)
+        b.block_attention(x[:len(slots)], out, view, r.view, 8, 0.1, scratch, r.err, b.stream_ptr(), splits=splits, groups=groups)
+        torch.cuda.synchronize()
+        err = r.err.item()
+        r.err.zero_()
+        return out.float(), err
+    for bad in (-1, r.n_pages, 1 << 30):
+        r.table[1, 1] = bad
+        out, err = go([0, 1, 2], [300] * 3)
+        assert err == b.ERR_PAGE_RANGE and torch.isfinite(out).all()
+        r.table.copy_(good)
+    out, err = go([0, 3, 2], [300] * 3)                       # a slot that the cache does not have
+    assert err == b.ERR_PAGE_RANGE and (out[1] == 0).all() and torch.isfinite(out).all()
+    out, err = go([0], [320])                                 # longer than its row of the table
+    assert err == b.ERR_PAGE_RANGE and (out == 0).all()
+    for scale in (r.k_scale, r.v_scale):
+        at = (int(good[1, 2]), 0, 1)
+        was = scale[at].item()
+        scale[at] = float("nan")
+        out, err = go([0, 1, 2], [300] * 3)
+        out = out.view(3, 8, 128)
+        assert err == 0 and torch.isfinite(out[0]).all() and torch.isfinite(out[2]).all()
+        assert torch.isnan(out[1, :4]).all() and torch.isfinite(out[1, 4:]).all()
+        scale[at] = was
+    out, err = go([0, 1, 2], [300] * 3)
+    assert err == 0 and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_two_steps_at_once(fmt):
+    """Two steps of different sequences on two streams, each with scratch of its own."""
+    b = B()
+    outs = []
+    for apart in (False, True):
+        rigs = [Rig(2, 8, 128, fmt, torch.bfloat16, n_slots=4, width=20, weights=True, seed=21 + i) for i in range(2)]
+        for r in rigs:
+            r.store([0, 1, 2, 3], [1000, 31, 700, 16])
+            r.weight.zero_()
+        torch.cuda.synchronize()
+        got, keep = [], []
+        for r, stream in zip(rigs, [torch.cuda.Stream() for _ in rigs] if apart else [torch.cuda.current_stream()] * 2):
+            with torch.cuda.stream(stream):
+                x = r.rows(4).reshape(4, -1).to(DEV)
+                view, arrs = r.batch([0, 1, 2, 3], [1] * 4, [1000, 31, 700, 16])
+                out, scratch = torch.empty(4, 8 * 128, dtype=torch.bfloat16, device=DEV), torch.empty(b.block_attention_scratch_floats(4, 8, r.view), device=DEV)
+                for _ in range(5):
+                    b.block_attention(x, out, view, r.view, 8, 0.1, scratch, r.err, b.stream_ptr())
+                got.append((out, r.weight))
+                keep.append((x, view, arrs, scratch))
+        torch.cuda.synchronize()
+        outs.append(got)
+    for one, two in zip(*outs):
+        for a, c in zip(one, two):
+            assert torch.equal(a, c)

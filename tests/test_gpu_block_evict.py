@@ -111,6 +111,19 @@ def test_a_wide_table_and_many_layers():
     run([100, 160], 3, 1, layers=40, G=1, D=16, seed=3, width=200)
 
 
+def test_more_blocks_than_shared_memory_holds():
+    run([52_003 * BLOCK + 7, 100 * BLOCK], keep=300, recent=20, layers=1, G=1, D=1, page_tokens=16, weights="ties")
+
+
+def test_no_room_for_an_unfinished_block_sets_the_error_word():
+    k, v = (torch.zeros((1, 6, 1, 16, 16), dtype=torch.int8, device=DEV) for _ in range(2))
+    ks, vs, w = (torch.ones((1, 6, 1, 1), device=DEV) for _ in range(3))
+    for length, want in ((48, 0), (49, 4)):
+        err, kept = torch.zeros(1, dtype=torch.int32, device=DEV), torch.zeros((1, 1, 1, 2), dtype=torch.int32, device=DEV)
+        B().block_evict(k, v, ks, vs, w, dev([[0, 1, 2, 3]]), dev([length]), dev([[4, 5]]), 2, 1, kept, err, B().stream_ptr())
+        assert err.item() == want
+
+
 def test_bad_pages_and_rows_set_the_error_word():
     b = B()
     k = torch.zeros(1, 8, 1, 64, 16, dtype=torch.int8, device=DEV)
