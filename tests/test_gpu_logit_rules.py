@@ -246,3 +246,10 @@ def test_on_another_stream_and_captured():
     assert torch.equal(out, want["out"]) and torch.equal(chosen, want["chosen"]) and torch.equal(lens, want["lens"])
     graph.replay()                                              # the second token: its history has one more
     assert torch.equal(lens, torch.where(torch.isin(torch.arange(len(c.lens), device=DEV), rows), want["lens"] + 1, want["lens"]))
+
+
+@pytest.mark.parametrize("R, V", [(40, 140_000), (40, 70_001), (100, 70_001), (100, 70_016), (300, 70_016), (300, 4099)])
+def test_rows_that_fewer_ctas_share(R, V):
+    """Clusters of four, two and one: a CTA's ids then are more than it counts at a time."""
+    c = Case(R, V, seed=R + V)
+    c.check(c.run(), c.logits.cpu().numpy())
