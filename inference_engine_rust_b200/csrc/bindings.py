@@ -447,8 +447,11 @@ def _on_current_device(*tensors) -> None:
         raise KernelError(f"the tensors are on cuda:{here}, which is not the current device")
 
 
+_I32, _F32 = torch.int32, torch.float32
+
+
 def _int_row(t, n: int) -> bool:
-    return t is not None and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)
+    return t is not None and t.dtype is _I32 and t.numel() == n and t.dim() == 1 and t.is_contiguous()
 
 
 def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, penalties=None, bias=None, mask=None, chosen=None,
@@ -466,15 +469,14 @@ def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, p
     chosen       int32 [R]: the id of the largest result, the lowest of equal ones; 0 and an error bit where nothing is left
     lens_out     int32 [H] (may be `lens`): the choice is appended to its history and the length plus one is written here
     """
-    i32, f32 = torch.int32, torch.float32
-    if logits.dim() != 2 or logits.dtype != f32 or logits.stride(1) != 1:
+    if logits.dim() != 2 or logits.dtype is not _F32 or logits.stride(1) != 1:
         raise KernelError("logits must be float32 [rows, vocab] with contiguous rows")
     R, vocab = logits.shape
-    if out is not None and (out.shape != logits.shape or out.dtype != f32 or out.stride(1) != 1):
+    if out is not None and (out.dtype is not _F32 or out.shape != logits.shape or out.stride(1) != 1):
         raise KernelError("out must be float32 like logits")
     H = width = 0
     if history is not None:
-        if history.dim() != 2 or history.dtype != i32 or not history.is_contiguous():
+        if history.dim() != 2 or history.dtype is not _I32 or not history.is_contiguous():
             raise KernelError("history must be contiguous int32 [histories, width]")
         H, width = history.shape
         if not _int_row(lens, H):
@@ -489,16 +491,18 @@ def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, p
         raise KernelError("penalties and lens_out need a history")
     else:
         lens = prompt_lens = rows = None
-    if penalties is not None and (penalties.dtype != f32 or penalties.shape != (H, 3) or not penalties.is_contiguous()):
+    if penalties is not None and (penalties.dtype is not _F32 or penalties.shape != (H, 3) or not penalties.is_contiguous()):
         raise KernelError(f"penalties must be float32 [{H}, 3]")
     ld_bias = ld_mask = 0
     if bias is not None:
-        if bias.dtype != f32 or bias.shape[-1] != vocab or bias.stride(-1) != 1 or not (bias.dim() == 1 or bias.shape == (R, vocab)):
+        per_row = bias.dim() == 2
+        if bias.dtype is not _F32 or bias.shape != ((R, vocab) if per_row else (vocab,)) or bias.stride(-1) != 1:
             raise KernelError("bias must be float32 [vocab] or [rows, vocab]")
-        ld_bias = bias.stride(0) if bias.dim() == 2 else 0
+        if per_row:
+            ld_bias = bias.stride(0)
     if mask is not None:
         words = -(-vocab // 32)
-        if mask.dtype != i32 or mask.dim() != 2 or mask.shape[1] != words or mask.shape[0] not in (1, R) or mask.stride(1) != 1:
+        if mask.dtype is not _I32 or mask.dim() != 2 or mask.shape[1] != words or mask.shape[0] not in (1, R) or mask.stride(1) != 1:
             raise KernelError(f"mask must be int32 [rows or 1, {words}]")
         ld_mask = mask.stride(0) if mask.shape[0] == R and R > 1 else 0
     if chosen is not None and not _int_row(chosen, R):
