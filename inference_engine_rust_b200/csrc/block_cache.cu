@@ -39,12 +39,13 @@ __device__ __forceinline__ void save8(__nv_bfloat16* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = raw;
 }
 
-// RUNS > 0: head sizes up to 32 RUNS, multiples of eight, all rows 16-byte aligned.  0: any.
-template <int FMT, typename T, int RUNS>
+// RUNS > 0: head sizes up to 32 RUNS, multiples of eight, all rows 16-byte aligned; HD > 0: that size alone, so that places in rows are
+// found without divisions.  0, 0: any.
+template <int FMT, typename T, int RUNS, int HD>
 __global__ void __launch_bounds__(STORE_THREADS) block_store_kernel(const T* __restrict__ qkv, int heads, IertBatchView b, IertBlockView c, int* __restrict__ err) {
   __shared__ uint32_t red[STORE_THREADS / 32];
   pdl_launch_dependents();
-  const int u = blockIdx.x, h = blockIdx.y, hd = c.head_dim;
+  const int u = blockIdx.x, h = blockIdx.y, hd = HD ? HD : c.head_dim;
   int lo = 0, hi = b.n_seqs;                           // the last sequence whose units start at or below u
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -64,11 +65,12 @@ __global__ void __launch_bounds__(STORE_THREADS) block_store_kernel(const T* __r
   const int per_page = c.page_tokens / BLK;
   auto one = [&](int x) {
     const int base = x * BLK, n_old = max(0, p0 - base);       // rows that are in the tail already
+    const int pg = x / per_page, in_page = x - pg * per_page;
     const bool whole = x < open, stays = whole && x + c.ring_pages * per_page >= open;
     int page = -1;
     // a ring keeps its latest blocks only: those that a later block of this step takes the place of are not written
-    if (stays || c.weight) page = block_page(c, slot, base / c.page_tokens, err);
-    const size_t at = page >= 0 ? ((size_t)page * c.kv_heads + h) * per_page + x % per_page : 0;
+    if (stays || c.weight) page = block_page(c, slot, pg, err);
+    const size_t at = page >= 0 ? ((size_t)page * c.kv_heads + h) * per_page + in_page : 0;
     if (page >= 0 && c.weight && base >= p0 && threadIdx.x == 0) c.weight[at] = 0.f;
     if (whole && (page < 0 || !stays)) return;
     const T* fresh = rows + (long long)(max(p0, base) - p0) * ld;
@@ -99,15 +101,12 @@ __global__ void __launch_bounds__(STORE_THREADS) block_store_kernel(const T* __r
       largest = __reduce_max_sync(0xffffffffu, largest);
       if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = largest;
       __syncthreads();
-      const float scale = block_scale<FMT>(max(red[2 * v], red[2 * v + 1]));
+      const float scale = block_scale<FMT>(max(red[2 * v], red[2 * v + 1])), inv = inverse_of_scale(scale);
 #pragma unroll
       for (int k = 0; k < RUNS; ++k) {
         const int i = (me + k * HALF) * 8;
         if (i >= n) break;
-        uint32_t w[2] = {0, 0};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)to_level<FMT>(val[k][e], scale) << (8 * (e & 3));
-        *reinterpret_cast<uint2*>(levels + i) = make_uint2(w[0], w[1]);
+        *reinterpret_cast<uint2*>(levels + i) = make_uint2(to_levels4<FMT>(&val[k][0], scale, inv), to_levels4<FMT>(&val[k][4], scale, inv));
       }
       if (me == 0) (v ? c.v_scale : c.k_scale)[at] = scale;
     } else {
@@ -338,10 +337,10 @@ IERT_API int iert_block_store(const void* qkv, int heads, const IertBatchView* b
     using T = std::remove_const_t<std::remove_pointer_t<decltype(rows)>>;
     constexpr int FMT = decltype(fmt)::value;
     auto with = [&](auto kernel) { launch_dep(kernel, grid, dim3(STORE_THREADS), 0, stream, rows, heads, *batch, *view, err); };
-    if (!vec) with(block_store_kernel<FMT, T, 0>);
-    else if (hd <= 64) with(block_store_kernel<FMT, T, 2>);
-    else if (hd <= 128) with(block_store_kernel<FMT, T, 4>);
-    else with(block_store_kernel<FMT, T, 8>);
+    if (!vec) with(block_store_kernel<FMT, T, 0, 0>);
+    else if (hd == 64) with(block_store_kernel<FMT, T, 2, 64>);
+    else if (hd == 128) with(block_store_kernel<FMT, T, 4, 128>);
+    else with(block_store_kernel<FMT, T, 8, 0>);
   };
   using I8 = std::integral_constant<int, IERT_LEVEL_INT8>;
   using E4 = std::integral_constant<int, IERT_LEVEL_E4M3>;
