@@ -14,7 +14,8 @@ namespace {
 // positions, kv head), half of it for the keys and half for the values.  The blocks of sequence s are the units [cu_q[s] / 16 + 2 s, ...): q
 // tokens touch at most q / 16 + 2 blocks.  A step reads and writes each number once, and its time is that of one chain of loads: so a
 // thread asks for all its numbers (VEC: eight at a time, `RUNS` runs of them), keeps them in registers over the search for the
-// largest, and writes their levels (2,048 tokens of 8 heads of 128 take 7 us, 38 with two passes of single numbers).
+// largest, and writes their levels; the page is looked up while they are on their way.  2,048 tokens of 8 heads of 128 take 6 us (38 with two
+// passes of single numbers), 16,001 of 4 heads of 64, 25 MB, 12; two heads of 64 a CTA, with half the overhead, took 15.
 constexpr int STORE_THREADS = 128, HALF = STORE_THREADS / 2;
 
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
@@ -67,62 +68,62 @@ __global__ void __launch_bounds__(STORE_THREADS) block_store_kernel(const T* __r
     const int base = x * BLK, n_old = max(0, p0 - base);       // rows that are in the tail already
     const int pg = x / per_page, in_page = x - pg * per_page;
     const bool whole = x < open, stays = whole && x + c.ring_pages * per_page >= open;
-    int page = -1;
     // a ring keeps its latest blocks only: those that a later block of this step takes the place of are not written
-    if (stays || c.weight) page = block_page(c, slot, pg, err);
-    const size_t at = page >= 0 ? ((size_t)page * c.kv_heads + h) * per_page + in_page : 0;
-    if (page >= 0 && c.weight && base >= p0 && threadIdx.x == 0) c.weight[at] = 0.f;
-    if (whole && (page < 0 || !stays)) return;
+    if (whole && !stays) return;                               // (a ring keeps no weights)
     const T* fresh = rows + (long long)(max(p0, base) - p0) * ld;
-    uint8_t* levels = (uint8_t*)(v ? c.v : c.k) + at * BLK * hd;
     const int n = (whole ? BLK : end - base) * hd;
     auto source = [&](int i) { const int r = i / hd; return r < n_old ? tail + i : fresh + (long long)(r - n_old) * ld + (i - r * hd); };
+    float val[RUNS > 0 ? RUNS : 1][8];
     if constexpr (RUNS > 0) {
-      float val[RUNS][8];
-      uint32_t largest = 0;
 #pragma unroll
       for (int k = 0; k < RUNS; ++k) {
         const int i = (me + k * HALF) * 8;
         if (i < n) load8(source(i), val[k]);
       }
-      if (!whole) {
+    }
+    // (looked up while the numbers are on their way)
+    const int page = whole || c.weight ? block_page(c, slot, pg, err) : -1;
+    const size_t at = page >= 0 ? ((size_t)page * c.kv_heads + h) * per_page + in_page : 0;
+    if (page >= 0 && c.weight && base >= p0 && threadIdx.x == 0) c.weight[at] = 0.f;
+    if (whole && page < 0) return;
+    uint8_t* levels = (uint8_t*)(v ? c.v : c.k) + at * BLK * hd;
+    if (!whole) {
+      if constexpr (RUNS > 0) {
 #pragma unroll
         for (int k = 0; k < RUNS; ++k) {
           const int i = (me + k * HALF) * 8;
           if (i < n && i / hd >= n_old) save8(tail + i, val[k]);
         }
-        return;
+      } else {
+        for (int i = n_old * hd + me; i < n; i += HALF) tail[i] = *source(i);
       }
+      return;
+    }
+    uint32_t largest = 0;
+    if constexpr (RUNS > 0) {
 #pragma unroll
       for (int k = 0; k < RUNS; ++k)
         if ((me + k * HALF) * 8 < n)
 #pragma unroll
           for (int e = 0; e < 8; ++e) largest = max(largest, abs_bits(val[k][e]));
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = largest;
-      __syncthreads();
-      const float scale = block_scale<FMT>(max(red[2 * v], red[2 * v + 1])), inv = inverse_of_scale(scale);
+    } else {
+      for (int i = me; i < n; i += HALF) largest = max(largest, abs_bits(to_f32(*source(i))));
+    }
+    largest = __reduce_max_sync(0xffffffffu, largest);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = largest;
+    __syncthreads();
+    const float scale = block_scale<FMT>(max(red[2 * v], red[2 * v + 1])), inv = inverse_of_scale(scale);
+    if constexpr (RUNS > 0) {
 #pragma unroll
       for (int k = 0; k < RUNS; ++k) {
         const int i = (me + k * HALF) * 8;
         if (i >= n) break;
         *reinterpret_cast<uint2*>(levels + i) = make_uint2(to_levels4<FMT>(&val[k][0], scale, inv), to_levels4<FMT>(&val[k][4], scale, inv));
       }
-      if (me == 0) (v ? c.v_scale : c.k_scale)[at] = scale;
     } else {
-      if (!whole) {
-        for (int i = n_old * hd + me; i < n; i += HALF) tail[i] = *source(i);
-        return;
-      }
-      uint32_t largest = 0;
-      for (int i = me; i < n; i += HALF) largest = max(largest, abs_bits(to_f32(*source(i))));
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = largest;
-      __syncthreads();
-      const float scale = block_scale<FMT>(max(red[2 * v], red[2 * v + 1]));
       for (int i = me; i < n; i += HALF) levels[i] = to_level<FMT>(to_f32(*source(i)), scale);
-      if (me == 0) (v ? c.v_scale : c.k_scale)[at] = scale;
     }
+    if (me == 0) (v ? c.v_scale : c.k_scale)[at] = scale;
   };
   // the tail is read by the first block and written by the unfinished one: the same CTA does them one after the other
   const bool together = p0 % BLK != 0 && first < open;
