@@ -13,7 +13,7 @@ namespace {
 // Store: the keys and values of a step's tokens, positions [pos0, pos0 + q) of each sequence.  One CTA per (block of 16
 // positions, kv head), half of it for the keys and half for the values.  The blocks of sequence s are the units [cu_q[s] / 16 + 2 s, ...): q
 // tokens touch at most q / 16 + 2 blocks.  A step reads and writes each number once, and its time is that of one chain of loads: so a
-// thread asks for all its numbers (VEC: eight at a time, `RUNS` runs of them), keeps them in registers over the search for the
+// thread asks for all its numbers (eight at a time, `RUNS` runs of them), keeps them in registers over the search for the
 // largest, and writes their levels; the page is looked up while they are on their way.  2,048 tokens of 8 heads of 128 take 6 us (38 with two
 // passes of single numbers), 16,001 of 4 heads of 64, 25 MB, 12; two heads of 64 a CTA, with half the overhead, took 15.
 constexpr int STORE_THREADS = 128, HALF = STORE_THREADS / 2;

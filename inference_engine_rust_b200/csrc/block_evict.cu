@@ -55,6 +55,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictParam
   extern __shared__ uint32_t keys[];
   __shared__ int hist[256], warp_gt[SELECT_THREADS / 32], warp_eq[SELECT_THREADS / 32], found[2];
   const int h = blockIdx.x, i = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_launch_dependents();
+  pdl_wait();
   const int row = evict_row(p, i);
   int* kept = p.kept + (((size_t)layer * p.n + i) * p.kv_heads + h) * p.keep;
   const int nb = row < 0 ? 0 : evict_blocks(p, i);
@@ -141,16 +143,17 @@ struct CopyParams {
 };
 
 // The copies: a warp per kept block (and one more per sequence, layer and head for the weight of the unfinished block, which the
-// sequence keeps).  VEC: 16 bytes at a time.
+// sequence keeps).  VEC: 16 bytes at a time.  Their bound is memory: 8 layers of 8 sequences of 4,096 positions, half of which stay
+// (539 MB read and written), take 92 us with the choice in front, 5.9 TB/s; 32 layers of one sequence of 1,088 (135 MB) 28 us, of which the
+// two starts, the choice and the chain kept -> page -> levels are about 8.  Copying after the choice in the same kernel would leave a CTA per
+// head to copy all its blocks.
 template <bool VEC>
 __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, CopyParams q) {
-  const long long unit = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31, per = p.keep + 1;
-  const long long total = (long long)p.layers * p.n * p.kv_heads * per;
-  if (unit >= total) return;
-  const int x = (int)(unit % per);
-  const long long lsh = unit / per;
-  const int h = (int)(lsh % p.kv_heads), i = (int)(lsh / p.kv_heads % p.n), layer = (int)(lsh / p.kv_heads / p.n);
+  const int lane = threadIdx.x & 31, groups = p.keep / 8 + 1;       // eight kept blocks, neighbours where they go, to a block of threads
+  const int lsh = blockIdx.x / groups, x = (blockIdx.x - lsh * groups) * 8 + (threadIdx.x >> 5);
+  const int li = lsh / p.kv_heads, h = lsh - li * p.kv_heads, layer = li / p.n, i = li - layer * p.n;
+  pdl_wait();                                            // the choice has been made
+  if (x > p.keep) return;
   const int row = evict_row(p, i);
   if (row < 0) return;
   const int nb = evict_blocks(p, i);
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, CopyPara
     from = nb;
     to = min(nb, p.keep);
   } else {
-    from = p.kept[lsh * p.keep + x];
+    from = p.kept[(size_t)lsh * p.keep + x];
     to = x;
     if (from < 0 || from >= nb) return;
   }
@@ -177,25 +180,28 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, CopyPara
   }
   const size_t l0 = (size_t)layer * p.n_pages;
   const size_t a = ((l0 + src) * p.kv_heads + h) * p.per_page + from % p.per_page, z = ((l0 + dst) * p.kv_heads + h) * p.per_page + to % p.per_page;
-  if (lane == 0) q.weight[z] = q.weight[a];
-  if (open) return;
-  if (lane == 0) { q.k_scale[z] = q.k_scale[a]; q.v_scale[z] = q.v_scale[a]; }
-  const uint8_t *ka = q.k + a * q.bytes, *va = q.v + a * q.bytes;
-  uint8_t *kz = q.k + z * q.bytes, *vz = q.v + z * q.bytes;
-  if (VEC) {
-    const int n = q.bytes / 16;
-    for (int j0 = lane; j0 < n; j0 += 128) {           // eight loads on their way before the first store
-      uint4 r[8];
+  // lane 0 and, of a finished block, 1 and 2: weight and scales, on their way together with the levels
+  float* small = lane == 0 ? q.weight : open || lane > 2 ? nullptr : lane == 1 ? q.k_scale : q.v_scale;
+  const float was = small ? small[a] : 0.f;
+  if (!open) {
+    const uint8_t *ka = q.k + a * q.bytes, *va = q.v + a * q.bytes;
+    uint8_t *kz = q.k + z * q.bytes, *vz = q.v + z * q.bytes;
+    if (VEC) {
+      const int n = q.bytes / 16;
+      for (int j0 = lane; j0 < n; j0 += 128) {           // eight loads on their way before the first store
+        uint4 r[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j0 + 32 * j < n) { r[2 * j] = __ldcs((const uint4*)ka + j0 + 32 * j); r[2 * j + 1] = __ldcs((const uint4*)va + j0 + 32 * j); }
+        for (int j = 0; j < 4; ++j)
+          if (j0 + 32 * j < n) { r[2 * j] = __ldcs((const uint4*)ka + j0 + 32 * j); r[2 * j + 1] = __ldcs((const uint4*)va + j0 + 32 * j); }
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j0 + 32 * j < n) { __stcs((uint4*)kz + j0 + 32 * j, r[2 * j]); __stcs((uint4*)vz + j0 + 32 * j, r[2 * j + 1]); }
+        for (int j = 0; j < 4; ++j)
+          if (j0 + 32 * j < n) { __stcs((uint4*)kz + j0 + 32 * j, r[2 * j]); __stcs((uint4*)vz + j0 + 32 * j, r[2 * j + 1]); }
+      }
+    } else {
+      for (int j = lane; j < q.bytes; j += 32) { kz[j] = ka[j]; vz[j] = va[j]; }
     }
-  } else {
-    for (int j = lane; j < q.bytes; j += 32) { kz[j] = ka[j]; vz[j] = va[j]; }
   }
+  if (small) small[z] = was;
 }
 
 }  // namespace
@@ -216,15 +222,13 @@ IERT_API int iert_block_evict(void* k, void* v, float* k_scale, float* v_scale, 
   p.n = n; p.layers = layers; p.n_pages = n_pages; p.kv_heads = kv_heads; p.per_page = page_tokens / BLK; p.width = width; p.rows = rows;
   p.new_width = new_width; p.keep = keep; p.recent = recent; p.max_blocks = max_blocks; p.err = err;
   if (smem > 40 * 1024) cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (staged) evict_select_kernel<true><<<dim3(kv_heads, n, layers), SELECT_THREADS, smem, stream>>>(p);
-  else evict_select_kernel<false><<<dim3(kv_heads, n, layers), SELECT_THREADS, 0, stream>>>(p);
+  launch_dep(staged ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(kv_heads, n, layers), dim3(SELECT_THREADS), smem, stream, p);
   const int status = iert_check_launch("block_evict (choice)");
   if (status) return status;
   CopyParams q = {(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, BLK * head_dim};
-  const long long warps = (long long)layers * n * kv_heads * (keep + 1);
-  const long long grid = (warps * 32 + 255) / 256;
+  const long long grid = (long long)layers * n * kv_heads * (keep / 8 + 1);
   if (grid > 0x7fffffffLL) return IERT_BAD_ARGUMENT;
-  if (((uintptr_t)k | (uintptr_t)v) % 16 == 0) evict_copy_kernel<true><<<(unsigned)grid, 256, 0, stream>>>(p, q);   // a block is 16 x head_dim bytes
-  else evict_copy_kernel<false><<<(unsigned)grid, 256, 0, stream>>>(p, q);
+  const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;        // (a block is 16 x head_dim bytes)
+  launch_dep(vec ? evict_copy_kernel<true> : evict_copy_kernel<false>, dim3((unsigned)grid), dim3(256), 0, stream, p, q);
   return iert_check_launch("block_evict (copy)");
 }
