@@ -162,7 +162,7 @@ def _declare(lib) -> None:
         "iert_history_append": [P, c_int, c_int, P, P, P, c_int, P, S],
         "iert_block_store": [P, c_int, POINTER(BatchView), POINTER(BlockView), P, S],
         "iert_block_attention_plain": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, P, S],
-        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, c_int, P, S],
+        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, P, S],
         "iert_block_attention_umma": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, c_int, P, S],
         "iert_block_evict": [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int,
                              P, P, P, S],
@@ -1319,7 +1319,7 @@ _piece_floats = None
 
 
 def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, scale: float, scratch, err, stream, *, rope=None,
-                    weight_out=None, plain: bool = False, splits: int = 0, warps: int = 0, groups: int = 0) -> None:
+                    weight_out=None, plain: bool = False, splits: int = 0, groups: int = 0) -> None:
     """One-token attention over the 8-bit cache, which the step's own key and value join; `out` [n_seqs, heads * head_dim] of the
     projection's type (rows of padding sequences: 0).  The slots of a step are all different, and steps that may run at the same time
     need scratch of their own.  Batch and page table are read while the kernel in front may still run: it must not write them.
@@ -1328,9 +1328,9 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
                  sequences' own blocks are written
     plain        the kernel that computes as the equations say (head sizes other than 64 and 128 always run it)
-    splits       CTAs that share a sequence's kv head (1, 2, 4, 8; on tcgen05 any number above, on mma.sync 16); 0: by the kernel's own rule
-    warps        of each CTA in the kernel on mma.sync (4, 8, 16), which is then the one that runs; 0: int8 levels with heads of 128 and up to
-                 eight of them to a key head run on tcgen05 with `groups` (1, 2; 0: by a rule) of softmax warps, else by that kernel's own rule
+    splits       CTAs that share a sequence's kv head (1, 2, 4, 8, 16; int8 levels with heads of 128 and up to eight of them to a key
+                 head, which run on tcgen05: also any number above 8 that the scratch has room for); 0: by the kernel's own rule
+    groups       on tcgen05, of softmax warps in each (1, 2); 0: by a rule
     """
     _packed_rows(qkv, heads, view)
     n = batch.n_seqs
@@ -1350,13 +1350,11 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     weights = weight_out.data_ptr() if weight_out is not None else view.weight
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
     args = (qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq), rotary_dim, pairing, factor)
-    if not plain and not warps:
-        status = core().iert_block_attention_umma(*args, splits, groups, err.data_ptr(), stream)
-        if status != 1:
-            return check(status, "block_attention")
     if not plain:
-        status = core().iert_block_attention_tc(*args, splits, warps, err.data_ptr(), stream)
-        if status != 1:
+        status = core().iert_block_attention_umma(*args, splits, groups, err.data_ptr(), stream)
+        if status == 1:
+            status = core().iert_block_attention_tc(*args, splits, err.data_ptr(), stream)
+        if status != 1 or splits:                # (1: not a case of theirs; with `splits`: or a number that they do not take)
             return check(status, "block_attention")
     check(core().iert_block_attention_plain(*args, err.data_ptr(), stream), "block_attention")
 

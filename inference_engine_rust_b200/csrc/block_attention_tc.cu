@@ -3,6 +3,8 @@
 // The sequences' keys and values in 8 bits are all that has to come from memory, so everything is arranged around that stream:
 //   * A cluster of up to 16 CTAs shares one (sequence, kv head): each takes a run of its blocks, and each adds up a share of the
 //     outputs from what the others have put into its shared memory.  One launch, no scratch memory for partial outputs.
+//     (Two CTAs of eight warps an SM: in fours, two to a pair, 64 sequences of 4,096 positions take as long in bfloat16 runs, 69 us, and 83 for 74 in
+//     float32 runs.)
 //   * A warp owns a block (16 positions) at a time, with a ring of its own that cp.async fills: no barrier inside the loop.
 //   * Levels become fp16 in registers, exactly (int8: 1024 + (q + 128) by a byte permutation, minus 1152; e4m3: a conversion
 //     instruction), and are the 16-row operand of mma.m16n8k16: S^T = K Q^T has 16 positions x 8 heads, O^T = V^T P^T 16 dimensions x 8
@@ -26,7 +28,7 @@ using namespace iert;
 
 namespace {
 
-constexpr int NSTAGE = 2, GH = 8, MAX_SPLITS = 16, WARPS_PER_SM = 16;
+constexpr int NSTAGE = 2, GH = 8, MAX_SPLITS = 16, WARPS = 8;
 constexpr float HEADROOM = 15.f;          // probabilities stay below 2^15 (fp16's largest is just under 2^16)
 constexpr float BELOW = 4.f;              // where the reference moves it goes to 2^-4 of the largest: scores may grow 2^11-fold before the next time
 constexpr int TAIL_BLOCKS = 8;            // finished blocks that cost a CTA about as much time as the unfinished one
@@ -96,7 +98,7 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
 template <int HD> __device__ __forceinline__ int k_chunk(int c) { return HD == 128 ? c ^ (((c >> 3) & 1) << 2) : c; }
 template <int HD> __device__ __forceinline__ int v_chunk(int c) { return HD == 128 ? c ^ (((c >> 4) & 3) << 1) : c ^ (((c >> 3) & 3) << 1); }
 
-template <int HD, typename T, int WARPS> struct Shared {
+template <int HD, typename T> struct Shared {
   uint8_t ring[WARPS][NSTAGE][2][BLK * HD];        // (later each warp's partial output, [GH][HD] fp32, in its own ring)
   T tail[2][BLK][HD];
   float q[GH][HD + 4];
@@ -124,10 +126,10 @@ __device__ __forceinline__ float head_value(const T* src, int d, const BlockTcPa
   return to_f32(from_f32<T>(second ? y * cs[half + k] + x * cs[k] : x * cs[k] - y * cs[half + k]));
 }
 
-template <int HD, int FMT, typename T, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, WARPS_PER_SM / WARPS) block_attention_tc_kernel(BlockTcParams p, IertBatchView b, IertBlockView c) {
+template <int HD, int FMT, typename T>
+__global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(BlockTcParams p, IertBatchView b, IertBlockView c) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
-  using Sh = Shared<HD, T, WARPS>;
+  using Sh = Shared<HD, T>;
   constexpr int THREADS = WARPS * 32;
   static_assert(NSTAGE * 2 * BLK >= GH * 4, "a warp's partial output fits in its ring");
   static_assert(THREADS >= MAX_SPLITS * GH && THREADS >= BLK * GH, "a thread per (CTA, head) and per (row, head)");
@@ -527,10 +529,10 @@ __global__ void __launch_bounds__(WARPS * 32, WARPS_PER_SM / WARPS) block_attent
   }
 }
 
-template <int HD, int FMT, typename T, int WARPS>
+template <int HD, int FMT, typename T>
 int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
-  auto kernel = block_attention_tc_kernel<HD, FMT, T, WARPS>;
-  const size_t smem = sizeof(Shared<HD, T, WARPS>);
+  auto kernel = block_attention_tc_kernel<HD, FMT, T>;
+  const size_t smem = sizeof(Shared<HD, T>);
   static bool configured = false;
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
@@ -554,19 +556,12 @@ int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& 
   return iert_check_launch("block_attention");
 }
 
-template <int HD, int FMT, typename T>
-int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, int warps, cudaStream_t stream) {
-  if (warps == 4) return launch<HD, FMT, T, 4>(p, b, c, splits, stream);
-  if (warps == 8) return launch<HD, FMT, T, 8>(p, b, c, splits, stream);
-  return launch<HD, FMT, T, 16>(p, b, c, splits, stream);
-}
-
 }  // namespace
 
-// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head, and `warps` (4, 8, 16) of each; 0: by the rule below.
+// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule below.
 IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
                                      float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
-                                     int warps, int* err, cudaStream_t stream) {
+                                     int* err, cudaStream_t stream) {
   if (batch->n_tokens <= 0) return IERT_OK;
   const IertBlockView& c = *view;
   if ((c.head_dim != 64 && c.head_dim != 128) || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || batch->n_tokens != batch->n_seqs ||
@@ -575,30 +570,34 @@ IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatch
       !scratch || (c.weight && (c.window || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)scratch) % 16 ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > c.head_dim || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
     return IERT_BAD_ARGUMENT;
-  if (warps != 0 && warps != 4 && warps != 8 && warps != 16) return IERT_BAD_ARGUMENT;
   const long long pairs = (long long)c.kv_heads * batch->n_seqs;
   const int sms = iert_sm_count_cached();
-  if (warps == 0) warps = pairs > 2 * sms ? 4 : 8;
-  if (splits < 0 || splits > 16 || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
+  if (splits < 0 || splits > MAX_SPLITS || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
   if (splits == 0) {
-    splits = pairs > 2 * sms ? 2 : 1;
-    while (splits < 16 && pairs * splits * 2 <= 2LL * sms) splits *= 2;
+    // As many CTAs as run at once, two an SM (8 sequences of 2,048 positions with 8 key heads: 22.8, 16.7, 13.7, 23.8 us with 1, 2, 4, 8 CTAs
+    // to a pair).  Clusters of 16 only where they all fit, two times seven of them, and for sequences that may be long (one sequence of 700
+    // positions: 7.9 us, 6.8 in clusters of 8; of 6,000: 10.5 and 11.4; two of 3,000: 18.8 and 11.9).  Between one and two pairs an SM a second CTA
+    // evens out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 36.7 us for 44.3, of 1,024: 22.8 for 20.0).
+    const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
+    for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= 2LL * sms;) splits *= 2;
+    if (splits == 16 && (pairs > 14 || reach < 2048)) splits = 8;
+    if (splits == 1 && pairs <= 2LL * sms && reach >= 4096) splits = 2;
   }
   BlockTcParams p = {};
-  p.by_length = pairs * splits * warps > (long long)WARPS_PER_SM * sms;
+  p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 71.5 us as they stand, 69.5 so)
   p.qkv = qkv; p.out = out; p.part = scratch; p.weight_out = weight_out;
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
   const int which = (c.head_dim == 128 ? 4 : 0) + (c.format == IERT_LEVEL_E4M3 ? 2 : 0) + (c.tail_dtype == IERT_BF16 ? 1 : 0);
   switch (which) {
-    case 0: return launch<64, IERT_LEVEL_INT8, float>(p, *batch, c, splits, warps, stream);
-    case 1: return launch<64, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
-    case 2: return launch<64, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, warps, stream);
-    case 3: return launch<64, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
-    case 4: return launch<128, IERT_LEVEL_INT8, float>(p, *batch, c, splits, warps, stream);
-    case 5: return launch<128, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
-    case 6: return launch<128, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, warps, stream);
-    default: return launch<128, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, warps, stream);
+    case 0: return launch<64, IERT_LEVEL_INT8, float>(p, *batch, c, splits, stream);
+    case 1: return launch<64, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, stream);
+    case 2: return launch<64, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, stream);
+    case 3: return launch<64, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, stream);
+    case 4: return launch<128, IERT_LEVEL_INT8, float>(p, *batch, c, splits, stream);
+    case 5: return launch<128, IERT_LEVEL_INT8, __nv_bfloat16>(p, *batch, c, splits, stream);
+    case 6: return launch<128, IERT_LEVEL_E4M3, float>(p, *batch, c, splits, stream);
+    default: return launch<128, IERT_LEVEL_E4M3, __nv_bfloat16>(p, *batch, c, splits, stream);
   }
 }

@@ -95,7 +95,7 @@ class Rig:
                 assert torch.equal(t[s, :, :n - done * BLOCK].double().cpu(), want.double()), (s, i)
         assert self.err.item() == 0
 
-    def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, warps=0, groups=0, scale=None, spread=1.0, check=True, scratch=None):
+    def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, groups=0, scale=None, spread=1.0, check=True, scratch=None):
         """One token for each of `slots`; compares with 64 bits and returns the outputs."""
         b = B()
         scale = self.D ** -0.5 if scale is None else scale
@@ -109,7 +109,7 @@ class Rig:
         if scratch is None:
             scratch = torch.full((b.block_attention_scratch_floats(len(slots) + pad, self.H, self.view),), float("nan"), device=DEV)
         b.block_attention(full, out, view, self.view, self.H, scale, scratch, self.err, b.stream_ptr(), weight_out=weight_out, plain=plain,
-                          splits=splits, warps=warps, groups=groups)
+                          splits=splits, groups=groups)
         torch.cuda.synchronize()
         assert (out[-1] == 7).all(), "a row behind the last sequence was written"
         assert (out[len(slots):-1] == 0).all(), "padding sequences"
@@ -219,21 +219,20 @@ def test_one_token_steps(plain, fmt, dtype, G, H, D):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("warps, groups, splits", [(0, 1, 1), (0, 1, 4), (0, 1, 8), (0, 2, 1), (0, 2, 2), (0, 2, 8), (0, 2, 9), (0, 2, 16), (4, 0, 1),
-                                                   (4, 0, 2), (4, 0, 16), (8, 0, 4), (16, 0, 1), (16, 0, 8)])
-@pytest.mark.parametrize("D", [64, 128])
-def test_a_key_head_shared_by_ctas(fmt, warps, groups, splits, D):
+@pytest.mark.parametrize("groups, splits", [(1, 1), (1, 4), (1, 8), (2, 1), (2, 2), (2, 8), (2, 9), (2, 16)])
+@pytest.mark.parametrize("D, H", [(64, 5), (128, 5), (128, 12)])
+def test_a_key_head_shared_by_ctas(fmt, groups, splits, D, H):
     """Long and short sequences, more CTAs than blocks among them, more than 64 blocks for a warp."""
     lens = [0, 5, 16, 40, 100, 1023, 2500, 16 * 32 * 4 * 2 + 17]
-    r = Rig(1, 5, D, fmt, torch.bfloat16, n_slots=8, width=66, weights=True, seed=splits)
+    r = Rig(1, H, D, fmt, torch.bfloat16, n_slots=8, width=66, weights=True, seed=splits)
     slots = [3, 1, 0, 7, 2, 5, 6, 4]
     live = [(s, x) for s, x in zip(slots, lens) if x]
     r.store([s for s, _ in live], [x for _, x in live])
     for s, x in live:
         r.blocks_weight[s] = [torch.zeros(1, dtype=torch.float64) for _ in range(-(-x // BLOCK))]
-    umma = warps == 0 and D == 128 and fmt == torch.int8
+    umma = D == 128 and H <= 8 and fmt == torch.int8
     for pad in (0, 8):
-        r.step(slots, plain=False, splits=splits if umma or splits != 9 else 8, warps=warps, groups=groups, pad=pad)
+        r.step(slots, plain=False, splits=splits if umma or splits != 9 else 8, groups=groups, pad=pad)
     r.check_content(slots)
 
 
@@ -537,3 +536,11 @@ def test_two_steps_at_once(fmt):
     for one, two in zip(*outs):
         for a, c in zip(one, two):
             assert torch.equal(a, c)
+
+
+def test_numbers_of_ctas_that_no_kernel_takes():
+    from inference_engine_rust_b200.csrc.bindings import KernelError
+    for D, splits in ((128, 3), (128, 200), (64, 9), (64, 32), (24, 2)):
+        r = Rig(1, 5, D, torch.int8, torch.bfloat16, n_slots=1, width=2, seed=22)
+        with pytest.raises(KernelError):
+            r.step([0], plain=False, splits=splits)
