@@ -808,18 +808,22 @@ IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBat
   const long long pairs = (long long)c.kv_heads * batch->n_seqs;
   if (splits < 0 || groups < 0 || groups > 2 || (splits > MAX_SPLITS ? pairs * splits > MAX_PIECES : (splits & (splits - 1)) != 0)) return IERT_BAD_ARGUMENT;
   const int sms = iert_sm_count_cached();
+  const long long reach = (long long)c.ring_pages * c.page_tokens;         // the most that a sequence holds
   if (splits == 0) {
     // One CTA an SM, in clusters of up to eight (8 sequences of 2,048 positions with 8 key heads: 15.9, 13.0, 21.0 us with 1, 2, 4 CTAs to a pair).
     // Pairs that leave more than eight SMs each, and may be long, take them all without a cluster (one sequence of 8,192 positions: 11.4 us, 10.9 as
     // a cluster; 16,384: 13.9 and 15.2; 32,768: 19.6 and 24.0; 131,071: 54 and 86; two of 32,768: 25.4 and 26.9).
-    const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
     if (pairs * (MAX_SPLITS + 1) <= sms && reach >= WIDE_FROM) splits = (int)(std::min(sms, MAX_PIECES) / pairs);
     else
       for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= sms;) splits *= 2;
+    // Half an SM to a CTA where half of the SMs would have none, unless sequences are short (16 of 4,096: 26.6 us, 24.3 so; of 1,024: 13.7 and 13.8)
+    if (splits == 1 && pairs <= sms && reach >= 2048) splits = 2;
   }
   const bool wide = splits > MAX_SPLITS;
-  // (64 sequences of 4,096 positions: 72 us with one group, 84 with two; 8 of 2,048, two CTAs to a pair: 14.7 and 13.0)
-  if (groups == 0) groups = pairs * splits <= sms ? 2 : 1;
+  // One group where two CTAs an SM have work (64 sequences of 4,096 positions: 72 us, 84 with two groups), two where one has.  Between one and two pairs
+  // an SM, long sequences one after the other even out what the SMs have to do (24 of 4,096: 35.2 us for 37.2; 36 of 4,096: 45.7 and 43.1, of 8,192:
+  // 68.6 and 72.6; 20 of 2,048: 25.4 and 22.9).
+  if (groups == 0) groups = pairs * splits <= sms || (splits == 1 && pairs <= 2LL * sms && pairs * 3000 <= reach * sms) ? 2 : 1;
   CUtensorMap mk, mv;
   const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
   UmmaParams p = {};
