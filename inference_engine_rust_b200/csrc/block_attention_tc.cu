@@ -9,7 +9,8 @@
 //   * Levels become fp16 in registers, exactly (int8: 1024 + (q + 128) by a byte permutation, minus 1152; e4m3: a conversion
 //     instruction), and are the 16-row operand of mma.m16n8k16: S^T = K Q^T has 16 positions x 8 heads, O^T = V^T P^T 16 dimensions x 8
 //     heads, so that a group of up to 8 query heads fills the narrow side.  Queries are scaled by a power of two of their row; bf16
-//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`), and probabilities likewise.
+//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`), and probabilities likewise: in bf16 runs they are
+//     rounded to 11 bits where they multiply values, 2^-12 beside the 2^-9 of the output's own rounding, and not in the sums.
 //   * The order of dimensions inside a product is free as long as both operands agree: a lane takes 16 neighbouring bytes of a key
 //     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.  P^T gets into operand form by
 //     two 8 x 8 transpositions in registers (movmatrix).
