@@ -1330,7 +1330,7 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     plain        the kernel that computes as the equations say (head sizes other than 64 and 128 always run it)
     splits       CTAs that share a sequence's kv head (1, 2, 4, 8, 16; int8 levels with heads of 128 and up to eight of them to a key
                  head, which run on tcgen05: also any number above 8 that the scratch has room for); 0: by the kernel's own rule
-    groups       on tcgen05, of softmax warps in each (1, 2); 0: by a rule
+    groups       of softmax warps in each CTA on tcgen05 (1, 2); 0: by a rule, which also leaves few and short sequences to mma.sync
     """
     _packed_rows(qkv, heads, view)
     n = batch.n_seqs

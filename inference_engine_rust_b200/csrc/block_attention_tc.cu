@@ -531,16 +531,29 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
 }
 
 template <int HD, int FMT, typename T>
-int launch(const BlockTcParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
+int launch(BlockTcParams p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
   auto kernel = block_attention_tc_kernel<HD, FMT, T>;
   const size_t smem = sizeof(Shared<HD, T>);
   static bool configured = false;
+  static int known[5];
   if (!configured) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return iert_check_launch("block_attention (attributes)");
     configured = true;
   }
+  const long long pairs = (long long)c.kv_heads * b.n_seqs;
+  const int sms = iert_sm_count_cached();
+  if (splits == 0) {
+    // The largest clusters that all run at once (8 sequences of 2,048 positions with 8 key heads: 22.8, 16.7, 13.7, 23.8 us with 1, 2, 4, 8 CTAs
+    // to a pair; two of 3,000: 18.8 us in clusters of 16, of which the device holds 14, and 11.9 of 8), those of 16 for sequences that may be long
+    // (one sequence of 700 positions: 7.9 us, 6.8 in clusters of 8; of 6,000: 10.5 and 11.4).  Between one and two pairs an SM a second CTA evens
+    // out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 36.7 us for 44.3, of 1,024: 22.8 for 20.0).
+    const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
+    for (splits = reach >= 2048 ? MAX_SPLITS : 8; splits > 1 && pairs > clusters_at_once(kernel, splits, WARPS * 32, smem, known);) splits >>= 1;
+    if (splits == 1 && pairs <= 2LL * sms && reach >= 4096) splits = 2;
+  }
+  p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 71.5 us as they stand, 69.5 so)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
   cfg.blockDim = dim3(WARPS * 32);
@@ -571,21 +584,8 @@ IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatch
       !scratch || (c.weight && (c.window || !weight_out)) || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.tail_k | (uintptr_t)c.tail_v | (uintptr_t)scratch) % 16 ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > c.head_dim || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
     return IERT_BAD_ARGUMENT;
-  const long long pairs = (long long)c.kv_heads * batch->n_seqs;
-  const int sms = iert_sm_count_cached();
   if (splits < 0 || splits > MAX_SPLITS || (splits & (splits - 1))) return IERT_BAD_ARGUMENT;
-  if (splits == 0) {
-    // As many CTAs as run at once, two an SM (8 sequences of 2,048 positions with 8 key heads: 22.8, 16.7, 13.7, 23.8 us with 1, 2, 4, 8 CTAs
-    // to a pair).  Clusters of 16 only where they all fit, two times seven of them, and for sequences that may be long (one sequence of 700
-    // positions: 7.9 us, 6.8 in clusters of 8; of 6,000: 10.5 and 11.4; two of 3,000: 18.8 and 11.9).  Between one and two pairs an SM a second CTA
-    // evens out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 36.7 us for 44.3, of 1,024: 22.8 for 20.0).
-    const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
-    for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= 2LL * sms;) splits *= 2;
-    if (splits == 16 && (pairs > 14 || reach < 2048)) splits = 8;
-    if (splits == 1 && pairs <= 2LL * sms && reach >= 4096) splits = 2;
-  }
   BlockTcParams p = {};
-  p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 71.5 us as they stand, 69.5 so)
   p.qkv = qkv; p.out = out; p.part = scratch; p.weight_out = weight_out;
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;

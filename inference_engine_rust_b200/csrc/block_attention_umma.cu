@@ -742,6 +742,16 @@ bool level_map(const void* levels, long long rows, int run, CUtensorMap* out) {
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Clusters of `size` CTAs that run at once: one CTA an SM, two softmax groups in it (GROUPS 2), or two with one.  Shared memory decides, and an empty
+// kernel with as much is asked about: of one that takes tensor memory the runtime says one CTA an SM, though two run.
+__global__ void room_kernel() {}
+template <typename T, int GROUPS, int NSTAGE> int at_once(int size) {
+  static int known[5];
+  const size_t smem = sizeof(Shared<T, GROUPS, NSTAGE>);
+  if (!known[0] && cudaFuncSetAttribute(room_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared<float, 2, 5>)) != cudaSuccess) return 1;
+  return clusters_at_once(room_kernel, size, GROUPS * SOFT + 128, smem, known);
+}
+
 template <typename T, int GROUPS, int NSTAGE, bool WIDE>
 int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, cudaStream_t stream) {
   auto kernel = block_attention_umma_kernel<T, GROUPS, NSTAGE, WIDE>;
@@ -781,8 +791,31 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, co
 }
 
 template <typename T>
-int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, const IertBatchView& b, const IertBlockView& c, int splits, int groups, bool wide,
-           cudaStream_t stream) {
+int launch(UmmaParams p, const IertBatchView& b, const IertBlockView& c, int splits, int groups, cudaStream_t stream) {
+  const long long pairs = (long long)c.kv_heads * b.n_seqs, reach = (long long)c.ring_pages * c.page_tokens;         // the most that a sequence holds
+  const int sms = iert_sm_count_cached();
+  if (splits == 0) {
+    // The largest clusters, up to eight, that all run at once with a CTA an SM (8 sequences of 2,048 positions with 8 key heads: 15.9, 13.0, 21.0 us
+    // with 1, 2, 4 CTAs to a pair; two of 3,500: 17.4 us in clusters of eight, of which the device holds 15, and 10.7 of four).  Pairs that leave more
+    // than eight SMs each, and may be long, take them all without a cluster (one sequence of 8,192 positions: 11.4 us, 10.9 as a cluster; 16,384: 13.9
+    // and 15.2; 32,768: 19.6 and 24.0; 131,071: 54 and 86; two of 32,768: 25.4 and 26.9).
+    if (pairs * (MAX_SPLITS + 1) <= sms && reach >= WIDE_FROM) splits = (int)(std::min(sms, MAX_PIECES) / pairs);
+    else
+      for (splits = MAX_SPLITS; splits > 1 && pairs > at_once<T, 2, 5>(splits);) splits >>= 1;
+    // Twice the CTAs, two an SM with one group each, where they all run at once and sequences may be long enough for a second start (16 of 4,096, 128
+    // pairs: 26.6 us, 24.3 so, of 1,024: 13.7 and 13.8; 56 pairs of 14,000: 37.7 and 31.8, of 3,500: 15.0 and 15.0; 24 pairs of 14,000: 20.9 and 19.5,
+    // of 7,000: 13.7 and 13.9; inside a model a start costs more: four layers, 8 sequences of 2,048 of at most 4,096: 448 us a step, 460 so).
+    if (splits < MAX_SPLITS && groups != 2 && reach >= 4096 * splits && pairs <= at_once<T, 1, 2>(2 * splits)) splits *= 2;
+  }
+  const bool wide = splits > MAX_SPLITS;
+  // Two groups where a CTA has an SM to itself, one where two share it (64 sequences of 4,096 positions: 84 us and 72).  Between one and two pairs an SM,
+  // long sequences one after the other even out what the SMs have to do (24 of 4,096: 35.2 us for 37.2; 36 of 4,096: 45.7 and 43.1, of 8,192: 68.6 and
+  // 72.6; 20 of 2,048: 25.4 and 22.9).
+  if (groups == 0) groups = wide || pairs <= at_once<T, 2, 5>(splits) || (splits == 1 && pairs <= 2LL * sms && pairs * 3000 <= reach * sms) ? 2 : 1;
+  p.by_length = pairs * splits > (groups == 2 ? sms : 2 * sms);      // (64 sequences of up to 4,096 positions: 80 us as they stand, 73 so)
+  CUtensorMap mk, mv;
+  const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
+  if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;
   if (wide) return launch<T, 2, 5, true>(mk, mv, p, b, c, splits, stream);
   return groups == 2 ? launch<T, 2, 5, false>(mk, mv, p, b, c, splits, stream) : launch<T, 1, 2, false>(mk, mv, p, b, c, splits, stream);
 }
@@ -792,7 +825,8 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const UmmaParams& p, co
 // Floats of scratch for what the CTAs of a step leave for one another, in front of the blocks' weights.
 IERT_API long long iert_block_attention_scratch() { return (long long)MAX_PIECES * GH * (HD + 2); }
 
-// `splits`: CTAs that share a sequence's kv head (1, 2, 4, 8: a cluster; more: not); `groups` (1, 2) of softmax warps in each; 0: by the rule below.
+// `splits`: CTAs that share a sequence's kv head (1, 2, 4, 8: a cluster; more: not); `groups` (1, 2) of softmax warps in each; 0: by rules.
+// IERT_BAD_ARGUMENT: not a case of this kernel.
 IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
                                        float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
                                        int groups, int* err, cudaStream_t stream) {
@@ -807,35 +841,17 @@ IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBat
     return IERT_BAD_ARGUMENT;
   const long long pairs = (long long)c.kv_heads * batch->n_seqs;
   if (splits < 0 || groups < 0 || groups > 2 || (splits > MAX_SPLITS ? pairs * splits > MAX_PIECES : (splits & (splits - 1)) != 0)) return IERT_BAD_ARGUMENT;
-  const int sms = iert_sm_count_cached();
-  const long long reach = (long long)c.ring_pages * c.page_tokens;         // the most that a sequence holds
-  if (splits == 0) {
-    // One CTA an SM, in clusters of up to eight (8 sequences of 2,048 positions with 8 key heads: 15.9, 13.0, 21.0 us with 1, 2, 4 CTAs to a pair).
-    // Pairs that leave more than eight SMs each, and may be long, take them all without a cluster (one sequence of 8,192 positions: 11.4 us, 10.9 as
-    // a cluster; 16,384: 13.9 and 15.2; 32,768: 19.6 and 24.0; 131,071: 54 and 86; two of 32,768: 25.4 and 26.9).
-    if (pairs * (MAX_SPLITS + 1) <= sms && reach >= WIDE_FROM) splits = (int)(std::min(sms, MAX_PIECES) / pairs);
-    else
-      for (splits = 1; splits < MAX_SPLITS && pairs * splits * 2 <= sms;) splits *= 2;
-    // Half an SM to a CTA where half of the SMs would have none, unless sequences are short (16 of 4,096: 26.6 us, 24.3 so; of 1,024: 13.7 and 13.8)
-    if (splits == 1 && pairs <= sms && reach >= 2048) splits = 2;
-  }
-  const bool wide = splits > MAX_SPLITS;
-  // One group where two CTAs an SM have work (64 sequences of 4,096 positions: 72 us, 84 with two groups), two where one has.  Between one and two pairs
-  // an SM, long sequences one after the other even out what the SMs have to do (24 of 4,096: 35.2 us for 37.2; 36 of 4,096: 45.7 and 43.1, of 8,192:
-  // 68.6 and 72.6; 20 of 2,048: 25.4 and 22.9).
-  if (groups == 0) groups = pairs * splits <= sms || (splits == 1 && pairs <= 2LL * sms && pairs * 3000 <= reach * sms) ? 2 : 1;
-  CUtensorMap mk, mv;
-  const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
+  // Few and short sequences are left to block_attention_tc.cu: its start overlaps the kernel in front and its end the one behind, which this one's shared and
+  // tensor memory do not allow (four layers of a model with 8 key heads: one sequence of 700 positions 408 us a step, 416 here; of 12,000 443 and 451;
+  // two of 7,000 448 and 464, of 12,000 498 and 488; three of 2,048 423 and 432, four 455 and 437; alone this kernel is the faster one by up to 1 us).
+  if (splits == 0 && groups == 0 && pairs <= 24 && pairs * c.ring_pages * c.page_tokens < 120000) return IERT_BAD_ARGUMENT;
   UmmaParams p = {};
-  p.by_length = pairs * splits > (groups == 2 ? sms : 2 * sms);      // (64 sequences of up to 4,096 positions: 80 us as they stand, 73 so)
   p.run = TILE_BLOCKS;
   while ((c.page_tokens / BLK) % p.run) p.run >>= 1;
-  if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;
   p.qkv = qkv; p.out = out; p.weight_out = weight_out;
   p.piece_o = scratch; p.piece_ml = scratch + (long long)MAX_PIECES * GH * HD; p.part = scratch + iert_block_attention_scratch();
   p.heads = heads; p.blocks = c.table_width * (c.page_tokens / BLK);
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
-  return c.tail_dtype == IERT_BF16 ? launch<__nv_bfloat16>(mk, mv, p, *batch, c, splits, groups, wide, stream)
-                                   : launch<float>(mk, mv, p, *batch, c, splits, groups, wide, stream);
+  return c.tail_dtype == IERT_BF16 ? launch<__nv_bfloat16>(p, *batch, c, splits, groups, stream) : launch<float>(p, *batch, c, splits, groups, stream);
 }

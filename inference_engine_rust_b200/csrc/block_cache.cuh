@@ -169,4 +169,30 @@ __device__ void finish_block(const T* tail, int hd, uint8_t* levels, float* scal
   if (threadIdx.x == 0) *scale = s;
 }
 
+// How many clusters of `size` CTAs the device holds at once of a kernel whose attributes are set (asked once; fewer than its SMs suggest, for a
+// cluster stays inside a group of SMs).  `known`: the kernel's own, zeros at first; sizes 1, 2, 4, 8, 16.
+template <typename Kernel>
+inline int clusters_at_once(Kernel kernel, int size, int threads, size_t smem, int* known) {
+  int i = 0;
+  while (1 << i < size) ++i;
+  if (!known[i]) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1024 * size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+      cudaGetLastError();
+      n = 1;
+    }
+    known[i] = n;
+  }
+  return known[i];
+}
+
 }  // namespace iert

@@ -9,6 +9,11 @@ from block_reference import BLOCK, PlainCache, attend, attend_bounds, levels_of
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 FORMATS = [torch.int8, torch.float8_e4m3fn]
+KERNELS = [True, False, "digits"]            # plain; by the kernels' rules; on tcgen05 wherever it can be (int8 levels, heads of 128, up to eight to a key head)
+
+
+def how(plain):
+    return {"plain": plain is True, "groups": 1 if plain == "digits" else 0}
 
 
 def B():
@@ -98,6 +103,8 @@ class Rig:
     def step(self, slots, pad=0, weight_out=None, plain=True, splits=0, groups=0, scale=None, spread=1.0, check=True, scratch=None):
         """One token for each of `slots`; compares with 64 bits and returns the outputs."""
         b = B()
+        if plain == "digits":
+            plain, groups = False, 1
         scale = self.D ** -0.5 if scale is None else scale
         x = self.rows(len(slots), spread)
         pos0 = [len(self.cache_of(s).rows) for s in slots]
@@ -198,7 +205,7 @@ def test_blocks_of_zeros_and_of_extremes(fmt):
 LENS = [0, 1, 14, 15, 16, 17, 63, 64, 65, 127, 128, 200, 255]
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("G, H, D", [(1, 1, 64), (2, 8, 128), (8, 32, 128), (2, 24, 64), (1, 20, 128), (1, 5, 24), (3, 6, 48), (1, 2, 256)])
@@ -236,7 +243,7 @@ def test_a_key_head_shared_by_ctas(fmt, groups, splits, D, H):
     r.check_content(slots)
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 @pytest.mark.parametrize("window, ring", [(1, 1), (16, 1), (17, 1), (64, 1), (65, 2), (100, 2), (128, 2), (1000, None)])
 @pytest.mark.parametrize("D", [64, 128, 40])
 def test_windows_and_rings(plain, window, ring, D):
@@ -249,7 +256,7 @@ def test_windows_and_rings(plain, window, ring, D):
     r.check_content([0, 1, 2, 3])
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_pages_of_other_sizes(plain):
     for pt in (16, 48, 128):
         r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=2, width=9, weights=True, page_tokens=pt, seed=pt)
@@ -260,7 +267,7 @@ def test_pages_of_other_sizes(plain):
         r.check_content([0, 1])
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_weights_elsewhere(plain):
     """Weights into another array: the view's own stay, and of the other only the sequences' blocks are written."""
     r = Rig(2, 4, 128, torch.int8, torch.bfloat16, n_slots=2, width=3, weights=True, seed=5)
@@ -278,7 +285,7 @@ def test_weights_elsewhere(plain):
                 assert (out[page, :, part] == 5).all()
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 @pytest.mark.parametrize("D", [128, 24])
 @pytest.mark.parametrize("pairing", [0, 1])
 def test_rotation_inside_the_kernel(plain, D, pairing):
@@ -302,7 +309,7 @@ def test_rotation_inside_the_kernel(plain, D, pairing):
             if not fused:
                 b.rotate_qk(x, where, inv, 4, 2, D, rot, pairing, r.err, b.stream_ptr(), rot_mul=1.25)
             scratch = torch.empty(b.block_attention_scratch_floats(3, 4, r.view), device=DEV)
-            b.block_attention(x, out, view, r.view, 4, D ** -0.5, scratch, r.err, b.stream_ptr(), rope=(inv, rot, pairing, 1.25) if fused else None, plain=plain)
+            b.block_attention(x, out, view, r.view, 4, D ** -0.5, scratch, r.err, b.stream_ptr(), rope=(inv, rot, pairing, 1.25) if fused else None, **how(plain))
             outs.append(out)
         # the same rotation in fp32 (contracted or not: two roundings of a sum of two products) before the same sums
         assert (outs[0] - outs[1]).abs().max().item() <= 1e-4
@@ -311,7 +318,7 @@ def test_rotation_inside_the_kernel(plain, D, pairing):
     assert rs[0].err.item() == 0 and rs[1].err.item() == 0
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_bad_pages_and_slots_set_the_error_word(plain):
     b = B()
     r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=3, width=2, weights=True, seed=11)
@@ -322,18 +329,18 @@ def test_bad_pages_and_slots_set_the_error_word(plain):
         view, keep = r.batch([0, 1, 2], [1] * 3, [40] * 3)
         x, out = r.rows(3).reshape(3, -1).to(DEV), torch.empty(3, 4 * 64, dtype=torch.bfloat16, device=DEV)
         scratch = torch.zeros(b.block_attention_scratch_floats(3, 4, r.view), device=DEV)
-        b.block_attention(x, out, view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), plain=plain)
+        b.block_attention(x, out, view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), **how(plain))
         assert r.err.item() == b.ERR_PAGE_RANGE
         r.err.zero_()
         r.table.copy_(good)
     for slot in (3, 1000):                                      # a slot that the cache does not have: as padding
         view, keep = r.batch([0, slot, 2], [1] * 3, [40] * 3)
-        b.block_attention(x, out, view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), plain=plain)
+        b.block_attention(x, out, view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), **how(plain))
         assert r.err.item() == b.ERR_PAGE_RANGE and (out[1] == 0).all() and torch.isfinite(out.float()).all()
         r.err.zero_()
     # a sequence longer than its row of the table
     view, keep = r.batch([0], [1], [128])
-    b.block_attention(x[:1], out[:1], view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), plain=plain)
+    b.block_attention(x[:1], out[:1], view, r.view, 4, 0.125, scratch, r.err, b.stream_ptr(), **how(plain))
     assert r.err.item() == b.ERR_PAGE_RANGE and (out[0] == 0).all()
     r.err.zero_()
     r.table[1, 0] = -1
@@ -342,7 +349,7 @@ def test_bad_pages_and_slots_set_the_error_word(plain):
     assert r.err.item() == b.ERR_PAGE_RANGE
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_what_is_not_a_number_stays_where_it_is_seen(plain):
     """A NaN among one sequence's values reaches that sequence's heads alone; positions outside a window reach nobody."""
     r = Rig(2, 4, 64, torch.int8, torch.bfloat16, n_slots=3, width=3, window=30, seed=13)
@@ -359,7 +366,7 @@ def test_what_is_not_a_number_stays_where_it_is_seen(plain):
     assert clean is r.view
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_large_scores(plain):
     """Scores of several hundred: one position takes nearly all the weight; nothing overflows."""
     r = Rig(2, 8, 128, torch.int8, torch.float32, n_slots=2, width=4, weights=True, seed=14)
@@ -369,7 +376,7 @@ def test_large_scores(plain):
         r.step([0, 1], plain=plain, spread=spread)
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_on_another_stream_and_captured(plain):
     b = B()
     outs = []
@@ -381,7 +388,7 @@ def test_on_another_stream_and_captured(plain):
         out, scratch = torch.empty(2, 8 * 128, dtype=torch.bfloat16, device=DEV), torch.zeros(b.block_attention_scratch_floats(2, 8, r.view), device=DEV)
 
         def go():
-            b.block_attention(x, out, view, r.view, 8, 0.1, scratch, r.err, b.stream_ptr(), plain=plain)
+            b.block_attention(x, out, view, r.view, 8, 0.1, scratch, r.err, b.stream_ptr(), **how(plain))
         torch.cuda.synchronize()
         if mode == "eager":
             go()
@@ -402,7 +409,7 @@ def test_on_another_stream_and_captured(plain):
             assert torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(c.float()))
 
 
-@pytest.mark.parametrize("plain", [True, False])
+@pytest.mark.parametrize("plain", KERNELS)
 def test_equal_calls_give_equal_bits(plain):
     """No sum depends on what runs when."""
     got = []
