@@ -161,9 +161,7 @@ def _declare(lib) -> None:
         "iert_logit_rules": [P, c_int, c_int, c_longlong, P, c_longlong, P, c_int, c_int, P, P, P, P, P, c_longlong, P, c_longlong, P, P, P, S],
         "iert_history_append": [P, c_int, c_int, P, P, P, c_int, P, S],
         "iert_block_store": [P, c_int, POINTER(BatchView), POINTER(BlockView), P, S],
-        "iert_block_attention_plain": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, P, S],
-        "iert_block_attention_tc": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, P, S],
-        "iert_block_attention_umma": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, c_int, P, S],
+        "iert_block_attention": [P, P, POINTER(BatchView), POINTER(BlockView), c_int, c_float, P, P, P, c_int, c_int, c_float, c_int, c_int, c_int, P, S],
         "iert_block_evict": [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P, P, c_int, P, c_int, c_int, c_int, c_int,
                              P, P, P, S],
         "iert_gemm_tc": [P, c_longlong, P, c_longlong, P, c_int, c_longlong, c_int, c_int, c_int, c_int,
@@ -1349,14 +1347,8 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
     weights = weight_out.data_ptr() if weight_out is not None else view.weight
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
-    args = (qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, _ptr(scratch), weights, _ptr(inv_freq), rotary_dim, pairing, factor)
-    if not plain:
-        status = core().iert_block_attention_umma(*args, splits, groups, err.data_ptr(), stream)
-        if status == 1:
-            status = core().iert_block_attention_tc(*args, splits, err.data_ptr(), stream)
-        if status != 1 or splits:                # (1: not a case of theirs; with `splits`: or a number that they do not take)
-            return check(status, "block_attention")
-    check(core().iert_block_attention_plain(*args, err.data_ptr(), stream), "block_attention")
+    check(core().iert_block_attention(qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, scratch.data_ptr(), weights, _ptr(inv_freq),
+                                      rotary_dim, pairing, factor, plain, splits, groups, err.data_ptr(), stream), "block_attention")
 
 
 def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, keep: int, recent: int, kept, err, stream, *, slots=None,

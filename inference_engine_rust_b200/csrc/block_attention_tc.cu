@@ -547,10 +547,10 @@ int launch(BlockTcParams p, const IertBatchView& b, const IertBlockView& c, int 
   if (splits == 0) {
     // The largest clusters that all run at once (8 sequences of 2,048 positions with 8 key heads: 22.8, 16.7, 13.7, 23.8 us with 1, 2, 4, 8 CTAs
     // to a pair; two of 3,000: 18.8 us in clusters of 16, of which the device holds 14, and 11.9 of 8), those of 16 for sequences that may be long
-    // (one sequence of 700 positions: 7.9 us, 6.8 in clusters of 8; of 6,000: 10.5 and 11.4).  Between one and two pairs an SM a second CTA evens
+    // (one sequence of 700 positions: 7.9 us, 6.8 in clusters of 8; of 3,000: 8.9 and 9.3; of 6,000: 10.5 and 11.4).  Between one and two pairs an SM a second CTA evens
     // out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 36.7 us for 44.3, of 1,024: 22.8 for 20.0).
     const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
-    for (splits = reach >= 2048 ? MAX_SPLITS : 8; splits > 1 && pairs > clusters_at_once(kernel, splits, WARPS * 32, smem, known);) splits >>= 1;
+    for (splits = reach >= 4096 ? MAX_SPLITS : 8; splits > 1 && pairs > clusters_at_once(kernel, splits, WARPS * 32, smem, known);) splits >>= 1;
     if (splits == 1 && pairs <= 2LL * sms && reach >= 4096) splits = 2;
   }
   p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 71.5 us as they stand, 69.5 so)
@@ -573,10 +573,9 @@ int launch(BlockTcParams p, const IertBatchView& b, const IertBlockView& c, int 
 }  // namespace
 
 // `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule below.
-IERT_API int iert_block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
-                                     float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
-                                     int* err, cudaStream_t stream) {
-  if (batch->n_tokens <= 0) return IERT_OK;
+int block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
+                       float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
+                       int* err, cudaStream_t stream) {
   const IertBlockView& c = *view;
   if ((c.head_dim != 64 && c.head_dim != 128) || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || batch->n_tokens != batch->n_seqs ||
       batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 || c.ring_pages <= 0 ||

@@ -827,10 +827,9 @@ IERT_API long long iert_block_attention_scratch() { return (long long)MAX_PIECES
 
 // `splits`: CTAs that share a sequence's kv head (1, 2, 4, 8: a cluster; more: not); `groups` (1, 2) of softmax warps in each; 0: by rules.
 // IERT_BAD_ARGUMENT: not a case of this kernel.
-IERT_API int iert_block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
-                                       float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
-                                       int groups, int* err, cudaStream_t stream) {
-  if (batch->n_tokens <= 0) return IERT_OK;
+int block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
+                         float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
+                         int groups, int* err, cudaStream_t stream) {
   const IertBlockView& c = *view;
   if (c.head_dim != HD || c.format != IERT_LEVEL_INT8 || c.kv_heads <= 0 || heads <= 0 || heads % c.kv_heads || heads / c.kv_heads > GH ||
       batch->n_tokens != batch->n_seqs || batch->n_seqs > 65535 || c.kv_heads > 65535 || c.page_tokens <= 0 || c.page_tokens % BLK || c.table_width <= 0 ||

@@ -353,10 +353,8 @@ IERT_API int iert_block_store(const void* qkv, int heads, const IertBatchView* b
   return iert_check_launch("block_store");
 }
 
-IERT_API int iert_block_attention_plain(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
-                                        float* part, float* weight_out, const float* inv_freq, int rotary_dim, int pairing,
-                                        float rot_mul, int* err, cudaStream_t stream) {
-  if (batch->n_tokens <= 0) return IERT_OK;
+static int block_attention_plain(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale, float* part,
+                                 float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int* err, cudaStream_t stream) {
   if (!view_ok(*view) || heads <= 0 || heads % view->kv_heads || view->head_dim > 32 * MAXD || batch->n_tokens != batch->n_seqs ||
       batch->n_seqs > 65535 || (view->weight && (view->window || !part || !weight_out)) ||
       (inv_freq && (rotary_dim < 0 || rotary_dim > view->head_dim || (rotary_dim & 1) || (pairing != IERT_PAIR_HALF && pairing != IERT_PAIR_INTERLEAVED))))
@@ -381,4 +379,18 @@ IERT_API int iert_block_attention_plain(const void* qkv, void* out, const IertBa
     else go(block_attention_plain_kernel<IERT_LEVEL_E4M3, __nv_bfloat16>);
   }
   return iert_check_launch("block_attention_plain");
+}
+
+// `plain`: the kernel above alone.  Else the first that takes the case: tcgen05 (`splits`, `groups`), mma.sync (`splits`), and with `splits` 0 the one above.
+IERT_API int iert_block_attention(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale, float* scratch,
+                                  float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int plain, int splits, int groups,
+                                  int* err, cudaStream_t stream) {
+  if (batch->n_tokens <= 0) return IERT_OK;
+  if (!plain) {
+    int status = block_attention_umma(qkv, out, batch, view, heads, scale, scratch, weight_out, inv_freq, rotary_dim, pairing, rot_mul, splits, groups, err, stream);
+    if (status == IERT_BAD_ARGUMENT)
+      status = block_attention_tc(qkv, out, batch, view, heads, scale, scratch, weight_out, inv_freq, rotary_dim, pairing, rot_mul, splits, err, stream);
+    if (status != IERT_BAD_ARGUMENT || splits) return status;
+  }
+  return block_attention_plain(qkv, out, batch, view, heads, scale, scratch, weight_out, inv_freq, rotary_dim, pairing, rot_mul, err, stream);
 }

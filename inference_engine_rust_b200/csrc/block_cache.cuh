@@ -42,6 +42,13 @@ struct IertBlockView {
   int tail_dtype;
 };
 
+// One-token attention on tcgen05 (block_attention_umma.cu) and on mma.sync (block_attention_tc.cu); IERT_BAD_ARGUMENT: not a case of theirs.
+int block_attention_umma(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale, float* scratch,
+                         float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits, int groups, int* err,
+                         cudaStream_t stream);
+int block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale, float* scratch,
+                       float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits, int* err, cudaStream_t stream);
+
 namespace iert {
 
 constexpr int BLK = 16;                        // positions of a block
