@@ -1364,24 +1364,33 @@ def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, 
     kept           int32 [layers, n, kv_heads, keep]: the numbers of the kept blocks (-1 behind the last of a sequence with fewer)
     shift          int32 [rows] or None: grows by the positions that a sequence loses
     """
-    _need(k.dim() == 5 and k.dtype in LEVEL_TYPES and v.dtype == k.dtype and v.shape == k.shape and k.is_contiguous() and v.is_contiguous(),
-          "k and v must be contiguous int8 or float8_e4m3fn [layers, pages, kv_heads, page_tokens, head_dim]")
+    if (k.dim() != 5 or k.dtype not in LEVEL_TYPES or v.dtype is not k.dtype or v.shape != k.shape or not k.is_contiguous()
+            or not v.is_contiguous()):
+        raise KernelError("k and v must be contiguous int8 or float8_e4m3fn [layers, pages, kv_heads, page_tokens, head_dim]")
     layers, n_pages, kv_heads, page_tokens, head_dim = k.shape
-    _need(page_tokens % BLOCK_TOKENS == 0, f"a page must be a multiple of {BLOCK_TOKENS} positions")
+    if page_tokens % BLOCK_TOKENS:
+        raise KernelError(f"a page must be a multiple of {BLOCK_TOKENS} positions")
     scales = (layers, n_pages, kv_heads, page_tokens // BLOCK_TOKENS)
     for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale"), (weight, "weight")):
-        _need(t is not None and t.dtype == torch.float32 and t.shape == scales and t.is_contiguous(), f"{name} must be contiguous float32 {list(scales)}")
+        if t is None or t.dtype is not _F32 or t.shape != scales or not t.is_contiguous():
+            raise KernelError(f"{name} must be contiguous float32 {list(scales)}")
     n = lengths.shape[0]
-    _need(page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.is_contiguous(), "the page table must be contiguous int32")
+    if page_table.dim() != 2 or page_table.dtype is not _I32 or not page_table.is_contiguous():
+        raise KernelError("the page table must be contiguous int32")
     rows, width = page_table.shape
-    _need(lengths.dtype == torch.int32 and lengths.is_contiguous() and (slots is not None or n <= rows), "lengths must be int32, one per sequence")
-    _need(slots is None or (slots.dtype == torch.int32 and slots.shape == (n,) and slots.is_contiguous()), f"slots must be int32 [{n}]")
-    _need(0 < keep and 0 <= recent <= keep, f"keep {keep} must be positive and recent {recent} between 0 and keep")
-    _need(new_pages.dtype == torch.int32 and new_pages.dim() == 2 and new_pages.shape[0] == n and new_pages.is_contiguous()
-          and new_pages.shape[1] * page_tokens >= keep * BLOCK_TOKENS, "new_pages must be int32 [sequences, pages] with room for the kept blocks")
-    _need(kept.dtype == torch.int32 and kept.shape == (layers, n, kv_heads, keep) and kept.is_contiguous(),
-          f"kept must be int32 {[layers, n, kv_heads, keep]}")
-    _need(shift is None or (shift.dtype == torch.int32 and shift.shape == (rows,) and shift.is_contiguous()), f"shift must be int32 [{rows}]")
+    if not _int_row(lengths, n) or (slots is None and n > rows):
+        raise KernelError("lengths must be int32, one per sequence")
+    if slots is not None and not _int_row(slots, n):
+        raise KernelError(f"slots must be int32 [{n}]")
+    if not (0 < keep and 0 <= recent <= keep):
+        raise KernelError(f"keep {keep} must be positive and recent {recent} between 0 and keep")
+    if (new_pages.dtype is not _I32 or new_pages.dim() != 2 or new_pages.shape[0] != n or not new_pages.is_contiguous()
+            or new_pages.shape[1] * page_tokens < keep * BLOCK_TOKENS):
+        raise KernelError("new_pages must be int32 [sequences, pages] with room for the kept blocks")
+    if kept.dtype is not _I32 or kept.shape != (layers, n, kv_heads, keep) or not kept.is_contiguous():
+        raise KernelError(f"kept must be int32 {[layers, n, kv_heads, keep]}")
+    if shift is not None and not _int_row(shift, rows):
+        raise KernelError(f"shift must be int32 [{rows}]")
     _on_current_device(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, kept, slots, shift, err)
     check(core().iert_block_evict(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), weight.data_ptr(), layers, n_pages, kv_heads,
                                   page_tokens, head_dim, page_table.data_ptr(), width, rows, _ptr(slots), lengths.data_ptr(), n,
