@@ -9,8 +9,7 @@
 //   * Levels become fp16 in registers, exactly (int8: 1024 + (q + 128) by a byte permutation, minus 1152; e4m3: a conversion
 //     instruction), and are the 16-row operand of mma.m16n8k16: S^T = K Q^T has 16 positions x 8 heads, O^T = V^T P^T 16 dimensions x 8
 //     heads, so that a group of up to 8 query heads fills the narrow side.  Queries are scaled by a power of two of their row; bf16
-//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`), and probabilities likewise: in bf16 runs they are
-//     rounded to 11 bits where they multiply values, 2^-12 beside the 2^-9 of the output's own rounding, and not in the sums.
+//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`).  Probabilities go in twice in every run.
 //   * The order of dimensions inside a product is free as long as both operands agree: a lane takes 16 neighbouring bytes of a key
 //     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.  P^T gets into operand form by
 //     two 8 x 8 transpositions in registers (movmatrix).
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
   static_assert(NSTAGE * 2 * BLK >= GH * 4, "a warp's partial output fits in its ring");
   static_assert(THREADS >= MAX_SPLITS * GH && THREADS >= BLK * GH, "a thread per (CTA, head) and per (row, head)");
   Sh& sm = *reinterpret_cast<Sh*>(smem_raw);
-  constexpr bool LO = sizeof(T) == 4;              // both halves of queries and probabilities
+  constexpr bool LO = sizeof(T) == 4;              // both halves of queries
   constexpr int KSTEPS = HD / 16, DPL = HD / 8;    // dimensions of a value row that a lane group takes
   cg::cluster_group cluster = cg::this_cluster();
   const int S = gridDim.x, rank = blockIdx.x;      // the cluster is the grid's first axis
@@ -405,8 +404,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
       for (int e = 0; e < 4; ++e) y[e] *= vr;
       const uint32_t p0 = half2_bits(y[0], y[1]), p1 = half2_bits(y[2], y[3]);
       const uint32_t b0 = transposed(p0), b1 = transposed(p1);
-      uint32_t r0 = 0, r1 = 0;
-      if (LO) { r0 = transposed(rest_bits(y[0], y[1], p0)); r1 = transposed(rest_bits(y[2], y[3], p1)); }
+      const uint32_t r0 = transposed(rest_bits(y[0], y[1], p0)), r1 = transposed(rest_bits(y[2], y[3], p1));
       // values of rows 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions [DPL g, DPL (g + 1))
       uint32_t vw[4][DPL / 4];
 #pragma unroll
@@ -429,7 +427,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
           levels4<FMT>(__byte_perm(vw[0][w], vw[1][w], sel), f[0], f[1]);
           levels4<FMT>(__byte_perm(vw[2][w], vw[3][w], sel), f[2], f[3]);
           mma_f16(o[2 * w + z], f, b0, b1);
-          if (LO) mma_f16(o[2 * w + z], f, r0, r1);
+          mma_f16(o[2 * w + z], f, r0, r1);
         }
       __syncwarp();                                  // the stage may be filled again
     }
