@@ -4,13 +4,14 @@
 // tcgen05.mma multiplies 8-bit integers as they stand in shared memory, so no level is ever converted; the other operand is a
 // number written in 8-bit digits, a column of the product per digit, and sums of 32-bit integers are exact:
 //   S [128 positions x 32] = K [128 x 128] Q^T     Q: a head's query as fixed-point numbers, DIG signed digits of 7 bits (base 128)
-//   O [128 dimensions x 32] += V^T [128 x 128] P   P: a head's probabilities as 32-bit fixed-point numbers, four unsigned digits of 8 bits
+//   O [128 dimensions x 32] += V^T [128 x 128] P   P: a head's probabilities times value scales as 32-bit fixed-point numbers, four unsigned digits of 8 bits
 // A tile is eight blocks of 16 positions of a (sequence, kv head), keys row by row (K-major), the values' tile read with its columns as
 // rows (MN-major).  Every position is one thread of the softmax, which needs about 210 instructions a warp and tile (mma.sync with
 // its conversions: 3,100 for the same 128 positions): what remains is the stream of levels.
 //   warps 0-3  softmax, a position per thread: a head's score from its digits, times the block's key scale; the probability times the
-//              block's value scale, as digits, into (swizzled) shared memory.  The references (a maximum per head, a largest value scale) move
-//              only where a fixed-point number would pass 2^31; O is then read out, added up in registers and begun again.
+//              block's value scale, as digits, into (swizzled) shared memory.  A head's unit is a power of two of its own and goes by these
+//              products alone, so that a block of large values that has no weight takes no digits from the others.  It moves where a tile's heaviest
+//              product would pass 2^31 or lies below 2^P_LEAST; O is then read out, added up in registers and begun again.
 //   then       two TMA producers, of keys and of values: page numbers (and scales) of 32 blocks at a time, one per lane; boxes of up to 128
 //              positions, as a page's size allows, into a ring of tiles.
 //   then       two MMA issuers, of the scores and of the weighted sums.  (One warp for both kinds of either took 1,450 cycles a tile: every
@@ -20,8 +21,8 @@
 // clusters of 16 fit only seven of its eight groups of SMs): theirs are not clusters, put their results into scratch memory, and a
 // second kernel, started while the first ends, adds them up (`WIDE`).  The unfinished block, up to 16 rows in the run's type, is done in fp32 by the
 // last CTA, which also stores the step's own key and value and turns the block into levels when it is full.
-// Queries as fixed-point numbers: bfloat16 runs 20 bits below the row's largest (three digits), float32 runs 27 (four); probabilities 25 bits below
-// the reference, which is at least 2^-6 of the largest.
+// Queries as fixed-point numbers: bfloat16 runs 20 bits below the row's largest (three digits), float32 runs 27 (four).  A product of probability and value
+// scale is off by at most half a unit, 2^-21 (bfloat16 runs; float32 runs 2^-25) of the heaviest one of its tile.
 // Every wait is bounded; on expiry the kernel records IERT_ERR_WAIT_EXPIRED, waits (bounded) for its copies and MMAs, frees its TMEM
 // and returns.
 #include <cooperative_groups.h>
@@ -44,7 +45,11 @@ constexpr int HD = 128, TILE = 128, TILE_BLOCKS = TILE / BLK, GH = 8, SOFT = 128
 constexpr int TILE_BYTES = TILE * HD, BLOCK_BYTES = BLK * HD, NCOL = 32;
 constexpr uint32_t TMEM_COLS = 128;            // S twice, O once per group
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
-constexpr int P_BITS = 25;                     // a probability of 1 (times the largest value scale) is 2^25; 2^31 is the bound
+// Where a unit moves, the heaviest product of the tile goes to [2^(P_TOP - 1), 2^(P_TOP + 1)); 2^31 is the bound.  A tile whose heaviest lies below 2^P_LEAST
+// moves it too.  Tiles may thus be lighter by 2^7, in float32 runs, which are to keep more bits, by 2^3, and heavier by 2^2.
+constexpr int P_TOP = 28;
+template <typename T> constexpr int P_LEAST = sizeof(T) == 4 ? 24 : 20;
+constexpr float Y_TOP = 64.f;                  // a probability beyond moves its head's reference: its product with the largest scale there is still has a number
 constexpr int MAX_RUN = 256;                   // tiles that O adds up at most: 255 * 127 * 128 * 256 < 2^31
 constexpr int WIDE_FROM = 16384;               // positions that a sequence may hold from which few sequences' CTAs are no clusters
 constexpr int TAIL_BLOCKS = 16;                // finished blocks that cost a CTA about as much time as the unfinished one
@@ -86,7 +91,8 @@ template <typename T, int GROUPS, int NSTAGE> struct __align__(1024) Shared {
   float wfac[GROUPS + 1][GH];                    // what each of them counts for in the CTA's result
   float lse[GH][2];
   float rs[GH];                                  // what makes scores of the integers
-  __align__(16) float top[GROUPS][4][GH];
+  __align__(16) float top[GROUPS][2][4][GH];     // of each warp: largest scores, heaviest products
+  __align__(16) uint32_t seen[GROUPS][2][4];     // of each warp, tiles in turn: see `softmax`
   float sum[GROUPS][4][GH];
   float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there: key scale NaN of its own kind (see NOWHERE)
   uint32_t red[GROUPS * 4 + 4];
@@ -129,12 +135,6 @@ __host__ __device__ constexpr uint32_t instr_desc_i8(uint32_t M, uint32_t N, uin
 }
 // Barriers of one softmax group.
 __device__ __forceinline__ void soft_sync(int group) { asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(SOFT) : "memory"); }
-__device__ __forceinline__ bool soft_any(int group, bool x) {
-  int y;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, %3, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
-               : "=r"(y) : "r"((int)x), "r"(1 + group), "n"(SOFT) : "memory");
-  return y != 0;
-}
 // All but the producer.
 template <int N> __device__ __forceinline__ void early_sync() { asm volatile("bar.sync 3, %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -438,12 +438,16 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       const uint32_t lane_bits = (uint32_t)((warp & 3) * 32) << 16, my_o = tmem + lane_bits + o_col + (GROUPS == 2 ? grp * NCOL : 0);
       const int blk = me >> 4;
       float* part = c.weight ? p.part + ((size_t)t * c.kv_heads + kvh) * p.blocks * GH : nullptr;
+      // What a warp tells the others of a tile: a bit per head with a product of at least 2^P_LEAST, and whether a reference has to move, a product is too large
+      // (or no number), a wait has run out.
+      constexpr uint32_t HEADS = (1u << GH) - 1, MOVE = 1u << GH, LARGE = 2u << GH, GONE = 4u << GH;
+      constexpr float LEAST = (float)(1u << P_LEAST<T>);
       float rs[GH], ref[GH], l[GH], acc[GH];
+      float root[GH];                              // a product's unit is root^-2, a power of four: no factor on the way leaves fp32's range
 #pragma unroll
-      for (int h = 0; h < GH; ++h) { rs[h] = sm.rs[h]; ref[h] = -INFINITY; l[h] = 0.f; acc[h] = 0.f; }
-      float v_ref = 0.f, v_inv = 0.f;              // the value scale that probabilities are relative to, and its inverse
+      for (int h = 0; h < GH; ++h) { rs[h] = sm.rs[h]; ref[h] = -INFINITY; l[h] = 0.f; acc[h] = 0.f; root[h] = 1.f; }
       int run = 0;                                 // tiles in O
-      // O of the tiles so far, in units of v_ref 2^-P_BITS, joins acc (dimension `me`)
+      // O of the tiles so far joins acc (dimension `me`)
       auto flush = [&](int i) {                    // i: the last tile in O
         if (!wait_bar(&sm.pv_done[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
         __syncwarp();
@@ -454,11 +458,12 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
           const float hi2 = fmaf((float)(int)r[24 + h], 256.f, (float)(int)r[16 + h]), lo2 = fmaf((float)(int)r[8 + h], 256.f, (float)(int)r[h]);
-          acc[h] += fmaf(hi2, 65536.f, lo2);
+          const float back = __uint_as_float((254u << 23) - __float_as_uint(root[h]));      // 1 / root
+          acc[h] = fmaf(fmaf(hi2, 65536.f, lo2) * back, back, acc[h]);
         }
         run = 0;
       };
-      for (int i = GROUPS == 2 ? grp : 0; i < n_tiles; i += GROUPS) {
+      for (int i = GROUPS == 2 ? grp : 0, turn = 0; i < n_tiles; i += GROUPS, turn ^= 1) {
         if (!wait_bar(&sm.s_full[i & 1], (i >> 1) & 1, abort_flag)) ok = false;
         __syncwarp();
         tc_fence_after();
@@ -469,7 +474,9 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
         mbar_arrive(&sm.s_empty[i & 1]);
         const int x = lo + i * TILE_BLOCKS + blk;
         const bool there = __float_as_uint(sc.x) != NOWHERE && x * BLK + (me & 15) >= j_min;
-        float v[GH], y[GH];
+        const float v_scale = there ? sc.y : 0.f;
+        float v[GH], y[GH], w[GH];
+        uint32_t says = ok ? 0u : GONE;
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
           float f;
@@ -477,49 +484,61 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
           else f = fmaf((float)((int)r[h] * 128 + (int)r[8 + h]), 128.f, (float)(int)r[16 + h]);
           v[h] = there ? f * (sc.x * rs[h]) : -INFINITY;
           y[h] = ex2(v[h] - ref[h]);
+          w[h] = y[h] * v_scale * root[h] * root[h];
+          if (!(y[h] <= Y_TOP)) says |= MOVE;
+          if (!(w[h] < 2147483648.f)) says |= LARGE;
+          if (w[h] >= LEAST) says |= 1u << h;
         }
-        const float vu = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
-        bool far = !ok;
-#pragma unroll
-        for (int h = 0; h < GH; ++h) far |= !(y[h] * vu < 2147483648.f) || !(y[h] < 1e30f);
-        if (soft_any(grp, far || run == MAX_RUN)) {  // (the same for all four warps)
-          // new references: the largest of the tile per head, the largest value scale; what was added up moves to them
+        says = __reduce_or_sync(0xffffffffu, says);
+        if (lane == 0) sm.seen[grp][turn][warp & 3] = says;
+        soft_sync(grp);                            // (the other turn's words are written again only behind the next tile's barrier)
+        const uint4 all = *reinterpret_cast<const uint4*>(&sm.seen[grp][turn][0]);
+        says = all.x | all.y | all.z | all.w;
+        if (says & GONE) { ok = false; break; }
+        if ((says & (HEADS | MOVE | LARGE)) != HEADS || run == MAX_RUN) {        // (the same for all four warps)
           if (run > 0) flush(i - GROUPS);
-          float mx[GH];
+          auto over_group = [&](const float (&z)[GH], int which) {               // the largest of the tile per head, for all to read
+            float mx[GH];
 #pragma unroll
-          for (int h = 0; h < GH; ++h) mx[h] = warp_top(v[h]);
-          if (lane == 0) {
-            *reinterpret_cast<float4*>(&sm.top[grp][warp & 3][0]) = make_float4(mx[0], mx[1], mx[2], mx[3]);
-            *reinterpret_cast<float4*>(&sm.top[grp][warp & 3][4]) = make_float4(mx[4], mx[5], mx[6], mx[7]);
-          }
-          if (soft_any(grp, !ok)) { ok = false; break; }       // (sm.top is written again only behind the next barrier of the group)
-          float v_new = v_ref;
+            for (int h = 0; h < GH; ++h) mx[h] = warp_top(z[h]);
+            if (lane == 0) {
+              *reinterpret_cast<float4*>(&sm.top[grp][which][warp & 3][0]) = make_float4(mx[0], mx[1], mx[2], mx[3]);
+              *reinterpret_cast<float4*>(&sm.top[grp][which][warp & 3][4]) = make_float4(mx[4], mx[5], mx[6], mx[7]);
+            }
+            soft_sync(grp);                        // (written again only behind another barrier of the group)
+          };
+          auto top = [&](int which, int h) {
+            return fmaxf(fmaxf(sm.top[grp][which][0][h], sm.top[grp][which][1][h]), fmaxf(sm.top[grp][which][2][h], sm.top[grp][which][3][h]));
+          };
+          if (says & MOVE) {
+            over_group(v, 0);
 #pragma unroll
-          for (int k = 0; k < TILE_BLOCKS; ++k) {
-            const float2 z = sm.scale[i % SLOTS][k];
-            if (__float_as_uint(z.x) != NOWHERE) v_new = fmaxf(v_new, z.y);
+            for (int h = 0; h < GH; ++h) {
+              const float to = fmaxf(ref[h], top(0, h));
+              const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
+              ref[h] = to;
+              l[h] *= alpha;
+              acc[h] *= alpha;
+              y[h] = v[h] == -INFINITY ? 0.f : ex2(v[h] - to);
+            }
           }
-          const float v_move = v_new > 0.f ? v_ref / v_new : 1.f;
-          v_ref = v_new;
-          v_inv = v_ref > 0.f ? 1.f / v_ref : 0.f;
+#pragma unroll
+          for (int h = 0; h < GH; ++h) w[h] = y[h] * v_scale;
+          over_group(w, 1);
 #pragma unroll
           for (int h = 0; h < GH; ++h) {
-            const float to = fmaxf(ref[h], fmaxf(fmaxf(sm.top[grp][0][h], sm.top[grp][1][h]), fmaxf(sm.top[grp][2][h], sm.top[grp][3][h])));
-            const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
-            ref[h] = to;
-            l[h] *= alpha;
-            acc[h] *= alpha * v_move;
-            y[h] = v[h] == -INFINITY ? 0.f : ex2(v[h] - to);
+            const int e = (int)(__float_as_uint(top(1, h)) >> 23);
+            // 2^k with k even, the heaviest times which lies in [2^(P_TOP - 1), 2^(P_TOP + 1)); a tile without any leaves the unit as it is
+            if (top(1, h) > 0.f) root[h] = __uint_as_float((uint32_t)(((P_TOP + 127 - max(e, 1)) >> 1) + 127) << 23);
+            w[h] = w[h] * root[h] * root[h];
           }
         }
-        const float unit = there ? (sc.y * v_inv) * (float)(1 << P_BITS) : 0.f;
         if (i >= 2 && !wait_bar(&sm.pv_done[i & 1], ((i >> 1) - 1) & 1, abort_flag)) ok = false;      // the buffer is free
         uint8_t* pd = sm.pd[i & 1] + (me & 15);
 #pragma unroll
         for (int h = 0; h < GH; ++h) {
-          const float w = y[h] * unit;
-          l[h] = fmaf(w, 0.f, l[h] + y[h]);        // (a value scale that is no number makes the head's sum none)
-          const uint32_t z = __float2uint_rn(w);
+          l[h] = fmaf(w[h], 0.f, l[h] + y[h]);     // (a value scale that is no number makes the head's sum none)
+          const uint32_t z = __float2uint_rn(w[h]);
           uint8_t* at = pd + h * TILE + ((blk ^ h) << 4);
           at[0] = (uint8_t)z;
           at[8 * TILE] = (uint8_t)(z >> 8);
@@ -550,7 +569,7 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       if (ok && run > 0) flush(GROUPS == 2 ? (n_tiles - 1 - grp) / 2 * 2 + grp : n_tiles - 1);       // its last tile
 #pragma unroll
       for (int h = 0; h < GH; ++h) {
-        sm.o[grp][h][me] = acc[h] * (v_ref * (1.f / (1 << P_BITS)));
+        sm.o[grp][h][me] = acc[h];
         float z = l[h];
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);

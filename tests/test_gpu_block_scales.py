@@ -101,3 +101,81 @@ def test_bfloat16_outputs_are_rounded_once(kernel, fmt, D, H):
         r.fill(slot, noise(r.g, n, 2, D), noise(r.g, n, 2, D))
     for _ in range(4):
         r.ask([0, 1, 2, 3], noise(r.g, 4, 2 * H, D) * 0.05, noise(r.g, 4, 2, D), noise(r.g, 4, 2, D), D ** -0.5, kernel)
+
+
+SHAPES = [(torch.int8, 128, 8)]
+
+
+@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt, D, H", SHAPES)
+@pytest.mark.parametrize("power", [10, 20, 30, 60])
+def test_large_values_that_have_next_to_no_weight(kernel, dtype, fmt, D, H, power):
+    """A block whose values are 2^power times the others': its keys lie so far below that it contributes a millionth of the output.  In front, in the middle,
+    last, and both the first and the last of a sequence."""
+    n, scale = 700, D ** -0.5
+    r = Apart(1, H, D, fmt, dtype, n_slots=4, width=11, seed=power)
+    below = (power + 20) * 0.6931472
+    for slot, where in enumerate([(0,), (21,), (42,), (0, 42)]):
+        k, v = noise(r.g, n, 1, D) * 0.5, noise(r.g, n, 1, D)
+        k[..., 0] = 0
+        for blk in where:
+            rows = slice(blk * BLOCK, (blk + 1) * BLOCK)
+            k[rows] *= 0.01
+            k[rows, :, 0] = -below / (4 * scale)
+            v[rows] *= 2.0 ** power
+        r.fill(slot, k, v)
+    for splits in (0, 1) if kernel is not True else (0,):
+        q = noise(r.g, 4, H, D) * 0.3
+        q[..., 0] = 4
+        k, v = noise(r.g, 4, 1, D) * 0.5, noise(r.g, 4, 1, D)
+        k[..., 0] = 0
+        r.ask([0, 1, 2, 3], q, k, v, scale, kernel, splits=splits)
+
+
+@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt, D, H", SHAPES)
+@pytest.mark.parametrize("nats", [12, 18, 24])
+def test_a_key_far_above_the_others_with_a_value_near_zero(kernel, dtype, fmt, D, H, nats):
+    """What a first token often is: all the weight, and nothing to say.  Its block's values are zeros, or those of its neighbours ordinary."""
+    n, scale = 4096 + 5, D ** -0.5
+    r = Apart(1, H, D, fmt, dtype, n_slots=3, width=65, seed=nats)
+    for slot, (at, alone) in enumerate([(0, True), (0, False), (2000, False)]):
+        k, v = noise(r.g, n, 1, D) * 0.5, noise(r.g, n, 1, D)
+        k[..., 0] = 0
+        v += 0.5                                    # (values that add up)
+        blk = slice(at // BLOCK * BLOCK, at // BLOCK * BLOCK + BLOCK)
+        if alone:
+            v[blk] = 0
+        k[blk] *= 0.01
+        k[at, :, 0] = nats / (4 * scale)
+        v[at] = 0
+        r.fill(slot, k, v)
+    for splits in (0, 1) if kernel is not True else (0,):
+        q = noise(r.g, 3, H, D) * 0.1
+        q[..., 0] = 4
+        k, v = noise(r.g, 3, 1, D) * 0.5, noise(r.g, 3, 1, D)
+        k[..., 0] = 0
+        r.ask([0, 1, 2], q, k, v, scale, kernel, splits=splits)
+
+
+@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fmt, D, H", SHAPES)
+def test_values_that_grow_and_shrink_from_block_to_block(kernel, dtype, fmt, D, H):
+    """Value sizes from 2^-40 to 2^40 in no order, keys alike: the largest block is what counts, wherever it stands.  And all values tiny, or large."""
+    n, scale = 1000, D ** -0.5
+    r = Apart(1, H, D, fmt, dtype, n_slots=4, width=17, seed=5)
+    for slot in range(4):
+        k, v = noise(r.g, n, 1, D) * 0.5, noise(r.g, n, 1, D)
+        if slot < 2:
+            powers = torch.randint(-40, 41, (-(-n // BLOCK),), generator=r.g).repeat_interleave(BLOCK)[:n].view(-1, 1, 1)
+            v = v * torch.exp2(powers.float())
+        else:
+            v = v * (2.0 ** -90 if slot == 2 else 2.0 ** 90)
+        r.fill(slot, k, v)
+    q, k, v = noise(r.g, 4, H, D) * 0.5, noise(r.g, 4, 1, D) * 0.5, noise(r.g, 4, 1, D)
+    v[2:] = 0
+    for splits in (0, 1) if kernel is not True else (0,):
+        r.ask([0, 1, 2, 3], q, k, v, scale, kernel, splits=splits)
