@@ -13,8 +13,10 @@
 //   * The order of dimensions inside a product is free as long as both operands agree: a lane takes 16 neighbouring bytes of a key
 //     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.  P^T gets into operand form by
 //     two 8 x 8 transpositions in registers (movmatrix).
-//   * A block's key scale multiplies its scores, its value scale (relative to the largest met so far) its probabilities: no level is
-//     ever multiplied.  The softmax reference moves only where a score passes it by 2^15, so a block costs no maximum across lanes.
+//   * A block's key scale multiplies its scores, its value scale its probabilities: no level is ever multiplied.  The products of probability and value scale
+//     are written as fp16 numbers in a unit, a power of two, that a warp keeps per head and that goes by these products alone: a block of large
+//     values that has no weight takes no digits from the others.  It moves where a block's heaviest product leaves [P_LEAST, 2^15], the softmax reference where a
+//     score passes it by 2^6, so most blocks cost no maximum across lanes.
 // The unfinished block, up to 16 rows in the run's type, is done in fp32 by the last CTA of the cluster, which also stores
 // the step's own key and value and turns the block into levels when it is full.
 #include <cooperative_groups.h>
@@ -29,8 +31,15 @@ using namespace iert;
 namespace {
 
 constexpr int NSTAGE = 2, GH = 8, MAX_SPLITS = 16, WARPS = 8;
-constexpr float HEADROOM = 15.f;          // probabilities stay below 2^15 (fp16's largest is just under 2^16)
-constexpr float BELOW = 4.f;              // where the reference moves it goes to 2^-4 of the largest: scores may grow 2^11-fold before the next time
+constexpr float HEADROOM = 6.f;           // probabilities stay below 2^6: their product with the largest scale there is still has a number
+// A block's heaviest product in its unit: where the unit moves, in [2^(P_TOP - 1), 2^(P_TOP + 1)); then below 2^15 (fp16's largest is just under 2^16) and at
+// least P_LEAST.  In two halves a product is off by at most 2^-23 of itself or half of fp16's smallest step, 2^-25: of a block's heaviest 2^-21 in
+// bfloat16 runs, 2^-25 in float32 runs.
+template <typename T> constexpr int P_TOP = sizeof(T) == 4 ? 8 : 5;
+constexpr float P_MOST = 0x1p15f;
+template <typename T> constexpr float P_LEAST = sizeof(T) == 4 ? 1.f : 0x1p-4f;
+// The output's sums stand in the same unit, so it comes down by no more than this from its highest (the products left out then are below 2^-80 of the heaviest).
+constexpr float DOWN = 0x1p40f;
 constexpr int TAIL_BLOCKS = 8;            // finished blocks that cost a CTA about as much time as the unfinished one
 
 struct BlockTcParams {
@@ -317,7 +326,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
 #pragma unroll
     for (int n = 0; n < DPL / 2; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
     float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // probabilities are relative to 2^ref
-    float v_top = 0.f, v_inv = INFINITY;                            // the largest value scale so far: o is in its units
+    float root[2] = {0.f, 0.f}, least[2] = {INFINITY, INFINITY};   // o's unit is root^-2 (0: none yet); the smallest root so far
     for (int i = 0; i < n_mine; ++i) {
       if ((i & 31) == 0 && i > 0) {                 // the next 32 blocks
         if ((i >> 5) & 1) look_up(i + 32, 0); else look_up(i + 32, 1);
@@ -370,7 +379,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
           float mx = fmaxf(v[h], v[h + 2]);
 #pragma unroll
           for (int w = 4; w < 32; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
-          const float to = fmaxf(ref[h], mx - BELOW);
+          const float to = fmaxf(ref[h], mx);
           const float alpha = to == ref[h] ? 1.f : ex2(ref[h] - to);
           ref[h] = to;
           l[h] *= alpha;
@@ -380,19 +389,42 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[e] = v[e] == -INFINITY ? v[e] : v[e] - ref[e & 1];
       }
-      if (v_scale > v_top) {                         // (the same for the whole warp)
-        const float f = v_top / v_scale;
-        v_top = v_scale;
-        v_inv = 1.f / v_scale;
-#pragma unroll
-        for (int n = 0; n < DPL / 2; ++n) { o[n][0] *= f; o[n][1] *= f; o[n][2] *= f; o[n][3] *= f; }
-      }
-      const float vr = v_scale * v_inv;
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = ex2(y[e]);
       const float s0 = y[0] + y[2], s1 = y[1] + y[3];
       l[0] += s0;
       l[1] += s1;
+      float w[4];
+      bool large = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = y[e] * v_scale * root[e & 1] * root[e & 1];
+        large |= !(w[e] <= P_MOST);
+      }
+      // lanes 4 g + tq: has any g a product of head 2 tq (2 tq + 1) that is not too small?
+      uint32_t some0 = __ballot_sync(0xffffffffu, fmaxf(w[0], w[2]) >= P_LEAST<T>), some1 = __ballot_sync(0xffffffffu, fmaxf(w[1], w[3]) >= P_LEAST<T>);
+      some0 |= some0 >> 16; some1 |= some1 >> 16;
+      some0 |= some0 >> 8; some1 |= some1 >> 8;
+      some0 |= some0 >> 4; some1 |= some1 >> 4;
+      if (__any_sync(0xffffffffu, large) || (some0 & some1 & 0xfu) != 0xfu) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float mx = fmaxf(y[h] * v_scale, y[h + 2] * v_scale);
+#pragma unroll
+          for (int x2 = 4; x2 < 32; x2 <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x2));
+          if (mx > 0.f) {                            // (a block without any leaves the unit as it is)
+            const int e = (int)(__float_as_uint(mx) >> 23);
+            const float to = fminf(__uint_as_float((uint32_t)(((P_TOP<T> + 127 - max(e, 1)) >> 1) + 127) << 23), least[h] * DOWN);
+            const float f = root[h] > 0.f ? to * __uint_as_float((254u << 23) - __float_as_uint(root[h])) : 0.f;      // to / root
+            root[h] = to;
+            least[h] = fminf(least[h], to);
+#pragma unroll
+            for (int n = 0; n < DPL / 2; ++n) { o[n][h] = o[n][h] * f * f; o[n][h + 2] = o[n][h + 2] * f * f; }
+          }
+          w[h] = y[h] * v_scale * root[h] * root[h];
+          w[h + 2] = y[h + 2] * v_scale * root[h] * root[h];
+        }
+      }
       if (part) {                                    // the block's sums: lanes of g < 4 end with head 2 tq, the others with 2 tq + 1
         float keep = g & 4 ? s1 : s0;
         keep += __shfl_xor_sync(0xffffffffu, g & 4 ? s0 : s1, 16);
@@ -400,11 +432,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
         keep += __shfl_xor_sync(0xffffffffu, keep, 4);
         if ((g & 3) == 0) part[(size_t)x * GH + 2 * tq + (g >> 2)] = (g & 4 ? ref[1] : ref[0]) + log2f(keep);
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] *= vr;
-      const uint32_t p0 = half2_bits(y[0], y[1]), p1 = half2_bits(y[2], y[3]);
+      const uint32_t p0 = half2_bits(w[0], w[1]), p1 = half2_bits(w[2], w[3]);
       const uint32_t b0 = transposed(p0), b1 = transposed(p1);
-      const uint32_t r0 = transposed(rest_bits(y[0], y[1], p0)), r1 = transposed(rest_bits(y[2], y[3], p1));
+      const uint32_t r0 = transposed(rest_bits(w[0], w[1], p0)), r1 = transposed(rest_bits(w[2], w[3], p1));
       // values of rows 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9, dimensions [DPL g, DPL (g + 1))
       uint32_t vw[4][DPL / 4];
 #pragma unroll
@@ -438,10 +468,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) block_attention_tc_kernel(Block
 #pragma unroll
       for (int w = 4; w < 32; w <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], w);
     float* mine = reinterpret_cast<float*>(&sm.ring[warp][0][0][0]);       // [GH][HD]
+    const float b0 = __uint_as_float((254u << 23) - __float_as_uint(root[0])), b1 = __uint_as_float((254u << 23) - __float_as_uint(root[1]));      // 1 / root
 #pragma unroll
     for (int n = 0; n < DPL / 2; ++n) {
-      *reinterpret_cast<float2*>(mine + (2 * tq) * HD + DPL * g + 2 * n) = make_float2(o[n][0] * v_top, o[n][2] * v_top);
-      *reinterpret_cast<float2*>(mine + (2 * tq + 1) * HD + DPL * g + 2 * n) = make_float2(o[n][1] * v_top, o[n][3] * v_top);
+      *reinterpret_cast<float2*>(mine + (2 * tq) * HD + DPL * g + 2 * n) = make_float2(o[n][0] * b0 * b0, o[n][2] * b0 * b0);
+      *reinterpret_cast<float2*>(mine + (2 * tq + 1) * HD + DPL * g + 2 * n) = make_float2(o[n][1] * b1 * b1, o[n][3] * b1 * b1);
     }
     if (g == 0) {
 #pragma unroll

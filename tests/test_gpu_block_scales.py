@@ -103,10 +103,10 @@ def test_bfloat16_outputs_are_rounded_once(kernel, fmt, D, H):
         r.ask([0, 1, 2, 3], noise(r.g, 4, 2 * H, D) * 0.05, noise(r.g, 4, 2, D), noise(r.g, 4, 2, D), D ** -0.5, kernel)
 
 
-SHAPES = [(torch.int8, 128, 8)]
+SHAPES = [(torch.int8, 128, 8), (torch.int8, 64, 5), (torch.float8_e4m3fn, 128, 4)]
 
 
-@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fmt, D, H", SHAPES)
 @pytest.mark.parametrize("power", [10, 20, 30, 60])
@@ -133,7 +133,7 @@ def test_large_values_that_have_next_to_no_weight(kernel, dtype, fmt, D, H, powe
         r.ask([0, 1, 2, 3], q, k, v, scale, kernel, splits=splits)
 
 
-@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fmt, D, H", SHAPES)
 @pytest.mark.parametrize("nats", [12, 18, 24])
@@ -160,7 +160,7 @@ def test_a_key_far_above_the_others_with_a_value_near_zero(kernel, dtype, fmt, D
         r.ask([0, 1, 2], q, k, v, scale, kernel, splits=splits)
 
 
-@pytest.mark.parametrize("kernel", [True, "digits"])
+@pytest.mark.parametrize("kernel", KERNELS)
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("fmt, D, H", SHAPES)
 def test_values_that_grow_and_shrink_from_block_to_block(kernel, dtype, fmt, D, H):
