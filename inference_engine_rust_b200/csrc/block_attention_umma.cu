@@ -94,7 +94,7 @@ template <typename T, int GROUPS, int NSTAGE> struct __align__(1024) Shared {
   __align__(16) float top[GROUPS][2][4][GH];     // of each warp: largest scores, heaviest products
   __align__(16) uint32_t seen[GROUPS][2][4];     // of each warp, tiles in turn: see `softmax`
   float sum[GROUPS][4][GH];
-  float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there: key scale NaN of its own kind (see NOWHERE)
+  float2 scale[SLOTS][TILE_BLOCKS];              // key and value scale; a block that is not there, or in front of the window: key scale NaN of its own kind (see NOWHERE)
   uint32_t red[GROUPS * 4 + 4];
   uint64_t k_full[NSTAGE], v_full[NSTAGE], k_empty[NSTAGE], v_empty[NSTAGE], s_full[2], s_empty[2], p_ready[2], pv_done[2], drained;
   uint32_t tmem;
@@ -238,9 +238,9 @@ block_attention_umma_kernel(const __grid_constant__ CUtensorMap map_k, const __g
       at_next = page >= 0 ? (page * c.kv_heads + kvh) * per_page + x % per_page : -1;
       if (V) return;
       ks_next = __uint_as_float(NOWHERE); vs_next = 0.f;
-      if (page >= 0) {
-        ks_next = c.k_scale[at_next];
-        vs_next = c.v_scale[at_next];
+      if (page >= 0 && x * BLK + BLK > j_min) {                // (a box may begin with blocks in front of the window: their levels are
+        ks_next = c.k_scale[at_next];                          // fetched, and may be written meanwhile where a ring's newest block takes their
+        vs_next = c.v_scale[at_next];                          // place, but count for nothing, whatever they are)
       }
     };
     const int page0 = page_at(lo + lane);

@@ -179,3 +179,26 @@ def test_values_that_grow_and_shrink_from_block_to_block(kernel, dtype, fmt, D, 
     v[2:] = 0
     for splits in (0, 1) if kernel is not True else (0,):
         r.ask([0, 1, 2, 3], q, k, v, scale, kernel, splits=splits)
+
+
+@pytest.mark.parametrize("kernel, splits", [(True, 0), (False, 0), ("digits", 0), ("digits", 1), ("digits", 8), ("digits", 9)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("odd", [float("inf"), float("nan"), 3e38, 2.0 ** 40])
+@pytest.mark.parametrize("ring", [None, 5])
+def test_blocks_in_front_of_a_window(kernel, splits, dtype, odd, ring):
+    """Scales of blocks that the window has left, in the page of its first one, change nothing, not a bit."""
+    window, n, D = 260, 700 + 16 * 3, 128
+    outs = []
+    for poison in (False, True):
+        r = Apart(1, 4, D, torch.int8, dtype, n_slots=3, width=17, window=window, ring=ring, seed=3)
+        for slot, m in enumerate((n, n - 16, n - 32)):            # the window's first block stands third, second and first in its page
+            r.fill(slot, noise(r.g, m, 1, D), noise(r.g, m, 1, D))
+            first = (m + 1 - window) // BLOCK
+            if poison:
+                for blk in range(first // 4 * 4, first):
+                    page = int(r.table_host[slot, blk // 4 % r.ring])
+                    r.v_scale[page, :, blk % 4] = odd
+                    r.k_scale[page, :, blk % 4] = odd
+        q, k, v = noise(r.g, 3, 4, D), noise(r.g, 3, 1, D), noise(r.g, 3, 1, D)
+        outs.append(r.ask([0, 1, 2], q, k, v, D ** -0.5, kernel, splits=splits))
+    assert torch.equal(*outs)
