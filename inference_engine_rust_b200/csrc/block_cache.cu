@@ -365,20 +365,19 @@ static int block_attention_plain(const void* qkv, void* out, const IertBatchView
   p.scale_log2e = scale * 1.44269504088896340736f;
   p.inv_freq = inv_freq; p.rope = inv_freq != nullptr; p.rotary_dim = rotary_dim; p.pairing = pairing; p.rot_mul = rot_mul; p.err = err;
   const int hd = view->head_dim;
-  const size_t smem = sizeof(float) * ((size_t)hd + GH * hd + 8 * GH * hd + 8 * GH * 2);
+  auto bytes = [](size_t d) { return sizeof(float) * (d + GH * d + 8 * GH * d + 8 * GH * 2); };
+  const size_t smem = bytes(hd);
   const dim3 grid(view->kv_heads, batch->n_seqs);
-  auto go = [&](auto kernel) {
-    if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto go = [&](auto fmt, auto* tail) {
+    constexpr auto kernel = block_attention_plain_kernel<decltype(fmt)::value, std::remove_pointer_t<decltype(tail)>>;
+    if (smem > 40 * 1024 && !shared_memory_up_to<kernel>(bytes(32 * MAXD))) return iert_check_launch("block_attention_plain (shared memory)");
     launch_dep(kernel, grid, dim3(256), smem, stream, p, *batch, *view);
+    return iert_check_launch("block_attention_plain");
   };
-  if (view->tail_dtype == IERT_F32) {
-    if (view->format == IERT_LEVEL_INT8) go(block_attention_plain_kernel<IERT_LEVEL_INT8, float>);
-    else go(block_attention_plain_kernel<IERT_LEVEL_E4M3, float>);
-  } else {
-    if (view->format == IERT_LEVEL_INT8) go(block_attention_plain_kernel<IERT_LEVEL_INT8, __nv_bfloat16>);
-    else go(block_attention_plain_kernel<IERT_LEVEL_E4M3, __nv_bfloat16>);
-  }
-  return iert_check_launch("block_attention_plain");
+  using I8 = std::integral_constant<int, IERT_LEVEL_INT8>;
+  using E4 = std::integral_constant<int, IERT_LEVEL_E4M3>;
+  if (view->tail_dtype == IERT_F32) return view->format == IERT_LEVEL_INT8 ? go(I8(), (float*)nullptr) : go(E4(), (float*)nullptr);
+  return view->format == IERT_LEVEL_INT8 ? go(I8(), (__nv_bfloat16*)nullptr) : go(E4(), (__nv_bfloat16*)nullptr);
 }
 
 // `plain`: the kernel above alone.  Else the first that takes the case: tcgen05 (`splits`, `groups`), mma.sync (`splits`), and with `splits` 0 the one above.

@@ -9,6 +9,7 @@ using namespace iert;
 namespace {
 
 constexpr int SELECT_THREADS = 256;
+constexpr int MOST_STAGED = 50 * 1024;       // blocks whose keys fit in shared memory
 
 struct EvictParams {
   const float* weight;      // [layers][n_pages][kv_heads][per_page]
@@ -215,13 +216,13 @@ IERT_API int iert_block_evict(void* k, void* v, float* k_scale, float* v_scale, 
   if (n_pages <= 0 || kv_heads <= 0 || page_tokens <= 0 || page_tokens % BLK || head_dim <= 0 || width <= 0 || rows <= 0 || keep <= 0 || recent < 0 ||
       recent > keep || max_blocks <= 0 || n > 65535 || layers > 65535 || (long long)new_width * page_tokens < (long long)keep * BLK)
     return IERT_BAD_ARGUMENT;
-  const bool staged = max_blocks <= 50 * 1024;
+  const bool staged = max_blocks <= MOST_STAGED;
   const size_t smem = staged ? (size_t)max_blocks * sizeof(uint32_t) : 0;
   EvictParams p = {};
   p.weight = weight; p.table = table; p.slots = slots; p.lengths = lengths; p.new_pages = new_pages; p.kept = kept; p.shift = shift;
   p.n = n; p.layers = layers; p.n_pages = n_pages; p.kv_heads = kv_heads; p.per_page = page_tokens / BLK; p.width = width; p.rows = rows;
   p.new_width = new_width; p.keep = keep; p.recent = recent; p.max_blocks = max_blocks; p.err = err;
-  if (smem > 40 * 1024) cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (smem > 40 * 1024 && !shared_memory_up_to<evict_select_kernel<true>>(MOST_STAGED * sizeof(uint32_t))) return iert_check_launch("block_evict (shared memory)");
   launch_dep(staged ? evict_select_kernel<true> : evict_select_kernel<false>, dim3(kv_heads, n, layers), dim3(SELECT_THREADS), smem, stream, p);
   const int status = iert_check_launch("block_evict (choice)");
   if (status) return status;

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #define IERT_API extern "C" __attribute__((visibility("default")))
 
 // Element type codes shared with the Python side.
@@ -373,4 +375,18 @@ inline void launch_dep(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t s
   cfg.attrs = attr;
   cfg.numAttrs = iert_pdl_enabled ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// Lets every launch of `Kernel` on the current device ask for up to `most` bytes of dynamic shared memory.  Set once, to the largest that any call takes: one
+// that set its own size could lower the limit between another thread's setting and launch.
+template <auto Kernel>
+inline bool shared_memory_up_to(size_t most) {
+  static std::atomic<unsigned long long> set{0};       // a bit per device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (set.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return false;
+  set.fetch_or(bit, std::memory_order_release);
+  return true;
 }

@@ -241,6 +241,14 @@ __global__ void __launch_bounds__(THREADS, 2) logit_rules_kernel(RulesParams p) 
   }
 }
 
+template <typename Count, bool VEC>
+int launch(cudaLaunchConfig_t& cfg, const RulesParams& p) {
+  if (cfg.dynamicSmemBytes > 40 * 1024 && !shared_memory_up_to<logit_rules_kernel<Count, VEC>>(COUNTED * sizeof(Count)))
+    return iert_check_launch("logit_rules (shared memory)");
+  cudaLaunchKernelEx(&cfg, logit_rules_kernel<Count, VEC>, p);
+  return iert_check_launch("logit_rules");
+}
+
 __global__ void history_append_kernel(int* history, int width, int hist_rows, int* lens, const int* rows, const int* tokens, int n, int* err) {
   pdl_launch_dependents();
   pdl_wait();
@@ -279,9 +287,6 @@ IERT_API int iert_logit_rules(const float* logits, int rows_n, int vocab, long l
                    (!bias || (ld_bias % 4 == 0 && (uintptr_t)bias % 16 == 0));
   const bool small = width < 32768;
   const size_t smem = penalties ? (small ? 2 : 4) * (size_t)(p.chunk < COUNTED ? p.chunk : COUNTED) : 0;
-  auto kernel = small ? (vec ? logit_rules_kernel<uint16_t, true> : logit_rules_kernel<uint16_t, false>)
-                      : (vec ? logit_rules_kernel<uint32_t, true> : logit_rules_kernel<uint32_t, false>);
-  if (smem > 40 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(cluster, rows_n);
   cfg.blockDim = dim3(THREADS);
@@ -294,8 +299,8 @@ IERT_API int iert_logit_rules(const float* logits, int rows_n, int vocab, long l
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = iert_pdl_enabled ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, kernel, p);
-  return iert_check_launch("logit_rules");
+  if (small) return vec ? launch<uint16_t, true>(cfg, p) : launch<uint16_t, false>(cfg, p);
+  return vec ? launch<uint32_t, true>(cfg, p) : launch<uint32_t, false>(cfg, p);
 }
 
 // tokens[r] joins the history of row rows[r] (null: r); the rows are distinct.
