@@ -1258,6 +1258,8 @@ def block_view(k, v, k_scale, v_scale, tail_k, tail_v, page_table, *, window: in
     page_table         int32 [n_slots, width]
     weight             fp32 like k_scale, or None: accumulated attention weight of each block (not together with a window)
     shift              int32 [n_slots] or None: positions a sequence has lost to eviction
+
+    All of them are on one device.
     """
     _need(k.dim() == 4 and k.dtype in LEVEL_TYPES and v.dtype == k.dtype and v.shape == k.shape, "k and v must be int8 or float8_e4m3fn of one shape "
           "[pages, kv_heads, page_tokens, head_dim]")
@@ -1275,6 +1277,9 @@ def block_view(k, v, k_scale, v_scale, tail_k, tail_v, page_table, *, window: in
         _need(t.is_contiguous(), f"{name} must be contiguous")
     _need(weight is None or not window, "block weights are kept for caches without a window")
     _need(shift is None or (shift.dtype == torch.int32 and shift.shape == (n_slots,) and shift.is_contiguous()), f"shift must be int32 [{n_slots}]")
+    for t, name in ((v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale"), (tail_k, "tail_k"), (tail_v, "tail_v"), (page_table, "page_table"),
+                    (weight, "weight"), (shift, "shift")):
+        _need(t is None or t.device == k.device, f"{name} is on another device than k")
     ring = width if ring_pages is None else ring_pages
     _need(0 < ring <= width and (ring == width or window), "a ring is part of a table row, and needs a window")
     _need(not window or ring * page_tokens >= min(window, width * page_tokens), "a ring must hold the window")
@@ -1322,7 +1327,7 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     projection's type (rows of padding sequences: 0).  The slots of a step are all different, and steps that may run at the same time
     need scratch of their own.  Batch and page table are read while the kernel in front may still run: it must not write them.
 
-    rope         (inv_freq, rotary_dim, pairing, factor): the kernel rotates queries and the new key by the position, evicted ones included
+    rope         (inv_freq fp32, rotary_dim, pairing, factor): the kernel rotates queries and the new key by the position, evicted ones included
     weight_out   where `view.weight` + this step's weights go (default: `view.weight`), of its shape; only the entries of the
                  sequences' own blocks are written
     plain        the kernel that computes as the equations say (head sizes other than 64 and 128 always run it)
@@ -1344,9 +1349,11 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
     if weight_out is not None and (weight is None or weight_out.dtype != torch.float32 or not weight_out.is_contiguous()
                                    or weight_out.shape != weight.shape):
         raise KernelError("weight_out must be laid out as the view's weight")
-    _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out)
-    weights = weight_out.data_ptr() if weight_out is not None else view.weight
     inv_freq, rotary_dim, pairing, factor = rope if rope is not None else (None, 0, 0, 1.0)
+    if inv_freq is not None and (inv_freq.dtype is not _F32 or not inv_freq.is_contiguous() or inv_freq.numel() < rotary_dim // 2):
+        raise KernelError("the rotation's frequencies must be contiguous float32, one per pair of rotary_dim")
+    _on_current_device(qkv, view.tensors[0], out, err, scratch, weight_out, inv_freq)
+    weights = weight_out.data_ptr() if weight_out is not None else view.weight
     check(core().iert_block_attention(qkv.data_ptr(), out.data_ptr(), byref(batch), byref(view), heads, scale, scratch.data_ptr(), weights, _ptr(inv_freq),
                                       rotary_dim, pairing, factor, plain, splits, groups, err.data_ptr(), stream), "block_attention")
 
