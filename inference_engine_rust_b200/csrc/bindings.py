@@ -1343,8 +1343,8 @@ def block_attention(qkv, out, batch: BatchView, view: BlockView, heads: int, sca
         raise KernelError(f"heads {heads} is not a multiple of kv_heads {view.kv_heads}")
     if out.dtype != qkv.dtype or not out.is_contiguous() or out.numel() < n * heads * view.head_dim:
         raise KernelError("out must be [sequences, heads * head_dim]")
-    if scratch.dtype != torch.float32 or scratch.numel() < block_attention_scratch_floats(n, heads, view):
-        raise KernelError("scratch is too small")
+    if scratch.dtype != torch.float32 or not scratch.is_contiguous() or scratch.numel() < block_attention_scratch_floats(n, heads, view):
+        raise KernelError("scratch is too small, or not contiguous float32")
     weight = view.tensors[7]
     if weight_out is not None and (weight is None or weight_out.dtype != torch.float32 or not weight_out.is_contiguous()
                                    or weight_out.shape != weight.shape):

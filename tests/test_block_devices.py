@@ -41,3 +41,12 @@ def test_every_tensor_of_a_step_is_looked_at(monkeypatch):
 def test_frequencies_that_do_not_fit_are_refused(inv_freq):
     with pytest.raises(B.KernelError, match="frequencies must be"):
         attention(inv_freq=inv_freq)
+
+
+def test_scratch_with_gaps_is_refused():
+    """Its count of numbers says nothing of the memory behind its first then."""
+    view = B.block_view(**pools())
+    with pytest.raises(B.KernelError, match="scratch"):
+        attention(scratch=torch.zeros(B.block_attention_scratch_floats(2, 4, view), 2)[:, 0])
+    with pytest.raises(B.KernelError, match="scratch"):
+        attention(scratch=torch.zeros(1).expand(B.block_attention_scratch_floats(2, 4, view)))
