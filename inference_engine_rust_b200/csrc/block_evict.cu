@@ -216,6 +216,8 @@ IERT_API int iert_block_evict(void* k, void* v, float* k_scale, float* v_scale, 
   if (n_pages <= 0 || kv_heads <= 0 || page_tokens <= 0 || page_tokens % BLK || head_dim <= 0 || width <= 0 || rows <= 0 || keep <= 0 || recent < 0 ||
       recent > keep || max_blocks <= 0 || n > 65535 || layers > 65535 || (long long)new_width * page_tokens < (long long)keep * BLK)
     return IERT_BAD_ARGUMENT;
+  const long long grid = (long long)layers * n * kv_heads * (keep / 8 + 1);          // of the copies; in front of both launches: the first one changes `shift`
+  if (grid > 0x7fffffffLL) return IERT_BAD_ARGUMENT;
   const bool staged = max_blocks <= MOST_STAGED;
   const size_t smem = staged ? (size_t)max_blocks * sizeof(uint32_t) : 0;
   EvictParams p = {};
@@ -227,8 +229,6 @@ IERT_API int iert_block_evict(void* k, void* v, float* k_scale, float* v_scale, 
   const int status = iert_check_launch("block_evict (choice)");
   if (status) return status;
   CopyParams q = {(uint8_t*)k, (uint8_t*)v, k_scale, v_scale, weight, BLK * head_dim};
-  const long long grid = (long long)layers * n * kv_heads * (keep / 8 + 1);
-  if (grid > 0x7fffffffLL) return IERT_BAD_ARGUMENT;
   const bool vec = ((uintptr_t)k | (uintptr_t)v) % 16 == 0;        // (a block is 16 x head_dim bytes)
   launch_dep(vec ? evict_copy_kernel<true> : evict_copy_kernel<false>, dim3((unsigned)grid), dim3(256), 0, stream, p, q);
   return iert_check_launch("block_evict (copy)");
