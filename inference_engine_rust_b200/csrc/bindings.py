@@ -1365,7 +1365,8 @@ def block_evict(k, v, k_scale, v_scale, weight, page_table, lengths, new_pages, 
 
     k, v, k_scale, v_scale, weight   the pools of all layers, as `block_view` takes them with an axis of layers in front
     page_table     int32 [rows, width]; sequence i is row slots[i] (slots int32 [n], all different; None: row i)
-    lengths        int32 [n]: positions that each sequence holds; one with at most `keep` finished blocks keeps them all
+    lengths        int32 [n]: positions that each sequence holds; one with at most `keep` finished blocks keeps them all, one longer than its row of the
+                   table sets the error word and is left as it is
     new_pages      int32 [n, >= keep * 16 / page_tokens, and room for the unfinished block (an error bit where it lacks)]: pages that no
                    sequence uses, all different
     kept           int32 [layers, n, kv_heads, keep]: the numbers of the kept blocks (-1 behind the last of a sequence with fewer)

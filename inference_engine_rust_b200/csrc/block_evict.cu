@@ -42,9 +42,10 @@ __device__ __forceinline__ int evict_page(const EvictParams& p, int row, int blk
   }
   return page;
 }
-// Finished blocks of sequence i that its table row can name.
+// Finished blocks of sequence i; -1 where it is longer than its row of the table.
 __device__ __forceinline__ int evict_blocks(const EvictParams& p, int i) {
-  return min(max(p.lengths[i], 0) / BLK, min(p.max_blocks, p.width * p.per_page));
+  const int length = max(p.lengths[i], 0);
+  return length > (long long)p.width * p.per_page * BLK || length / BLK > p.max_blocks ? -1 : length / BLK;
 }
 
 // Which blocks stay: one CTA per (kv head, sequence, layer).  The keys stand in shared memory (STAGED; where they do not fit, in memory
@@ -60,8 +61,8 @@ __global__ void __launch_bounds__(SELECT_THREADS) evict_select_kernel(EvictParam
   pdl_wait();
   const int row = evict_row(p, i);
   int* kept = p.kept + (((size_t)layer * p.n + i) * p.kv_heads + h) * p.keep;
-  const int nb = row < 0 ? 0 : evict_blocks(p, i);
-  if (row < 0 && tid == 0) atomicOr(p.err, IERT_ERR_PAGE_RANGE);
+  const int nb = row < 0 ? -1 : evict_blocks(p, i);
+  if (nb < 0 && tid == 0) atomicOr(p.err, IERT_ERR_PAGE_RANGE);      // (and the sequence is left as it is)
   if (nb <= p.keep) {                                    // nothing to choose
     for (int x = tid; x < p.keep; x += SELECT_THREADS) kept[x] = x < nb ? x : -1;
     return;
@@ -158,10 +159,11 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(EvictParams p, CopyPara
   const int row = evict_row(p, i);
   if (row < 0) return;
   const int nb = evict_blocks(p, i);
+  if (nb < 0) return;
   int from, to;
   const bool open = x == p.keep;
   if (open) {
-    if (p.lengths[i] % BLK == 0 || nb * BLK + BLK <= p.lengths[i] || nb >= p.width * p.per_page) return;
+    if (max(p.lengths[i], 0) % BLK == 0) return;
     from = nb;
     to = min(nb, p.keep);
   } else {
