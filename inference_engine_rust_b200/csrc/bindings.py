@@ -461,8 +461,9 @@ def logit_rules(logits, out, history, lens, prompt_lens, rows, err, stream, *, p
                  and how many of them are the prompt's; rows int32 [R]: the history of each logits row, all different (None: row r has
                  history r).  Tokens outside the vocabulary count for nothing.  history None: no row has one
     penalties    fp32 [H, 3]: repetition r > 0 (a seen id: x / r if x > 0 else x * r), presence a, frequency f (an id with c > 0
-                 occurrences in the answer: x - f c - a)
-    bias         fp32 [vocab] or [R, vocab], added after the penalties; -infinity rules an id out
+                 occurrences in the answer: x - f c - a), all finite, f times the history's length too (else the error word is set)
+    bias         fp32 [vocab] or [R, vocab], added after the penalties; -infinity rules an id out.  A result of +infinity or NaN sets the
+                 error word
     mask         int32 [R, ceil(vocab / 32)] or [1, ...]: bit i % 32 of word i // 32 set = id i is allowed
     chosen       int32 [R]: the id of the largest result, the lowest of equal ones; 0 and an error bit where nothing is left
     lens_out     int32 [H] (may be `lens`): the choice is appended to its history and the length plus one is written here

@@ -123,7 +123,8 @@ __global__ void __launch_bounds__(THREADS, 2) logit_rules_kernel(RulesParams p) 
 
   float bv = -INFINITY;
   int bi = 0x7fffffff;
-  bool bad = false;
+  // A row's penalties are asked once, not each result: with these no NaN comes of them, and an infinity is the best of its thread.
+  bool bad = counted && !(rep > 0.f && rep < INFINITY && fabsf(pres) < INFINITY && fabsf(freq) * (float)len < INFINITY);
   // Four logits at a time, most of which nothing happens to: what is common to the four is asked once (61 instructions a logit with each
   // rule asked of each, 64 rows of 131,072 then 32 us).  c: counts; m: a bit per allowed id; i, step: their ids.
   auto rules = [&](float (&y)[4], const uint32_t (&c)[4], const float (&b)[4], uint32_t m, int i, int step, int n) {
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(THREADS, 2) logit_rules_kernel(RulesParams p) 
       }
     }
   }
-  if (bad) atomicOr(p.err, IERT_ERR_NONFINITE_LOGIT);
+  if (bad || bv == INFINITY) atomicOr(p.err, IERT_ERR_NONFINITE_LOGIT);
   if (!p.chosen) return;                      // (the same for the whole cluster)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {

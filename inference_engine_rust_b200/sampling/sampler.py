@@ -24,6 +24,9 @@ class SamplingError(ValueError):
     pass
 
 
+_F32_MOST, _F32_LEAST = float(np.finfo(np.float32).max), 2.0 ** -149       # the largest and the smallest positive number of 32 bits
+
+
 @dataclass(frozen=True)
 class SamplingParams:
     """temperature 0 = greedy; > 0 = temperature sampling with `seed`.  The penalties and biases are the rules above; `logit_bias` maps
@@ -43,8 +46,9 @@ class SamplingParams:
             raise SamplingError(f"seed must be an integer in [0, 2^64), got {self.seed!r}")
         for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
             v = getattr(self, name)
-            if isinstance(v, bool) or not isinstance(v, (int, float)) or not math.isfinite(v) or (name == "repetition_penalty" and v <= 0):
-                raise SamplingError(f"{name} must be finite{' and positive' if name == 'repetition_penalty' else ''}, got {v!r}")
+            if (isinstance(v, bool) or not isinstance(v, (int, float)) or not -_F32_MOST <= v <= _F32_MOST
+                    or (name == "repetition_penalty" and v < _F32_LEAST)):
+                raise SamplingError(f"{name} must be finite{' and positive' if name == 'repetition_penalty' else ''} in 32 bits, got {v!r}")
         bias = self.logit_bias
         if bias is None:
             bias = ()
@@ -53,10 +57,10 @@ class SamplingParams:
             try:
                 i, b = pair
                 i, b = operator.index(i), float(b)
-            except (TypeError, ValueError):
+            except (TypeError, ValueError, OverflowError):
                 raise SamplingError(f"logit_bias maps token ids to numbers, got {pair!r}") from None
-            if i < 0 or math.isnan(b) or b == math.inf:
-                raise SamplingError(f"logit_bias: id {i} must be >= 0 and its bias finite or -infinity, got {b!r}")
+            if i < 0 or not b <= _F32_MOST:
+                raise SamplingError(f"logit_bias: id {i} must be >= 0 and its bias finite or -infinity in 32 bits, got {b!r}")
             pairs.append((i, b))
         if len({i for i, _ in pairs}) != len(pairs):
             raise SamplingError("logit_bias: an id appears twice")
