@@ -213,7 +213,8 @@ def generate(engine, sampler: Callable, prompts: Sequence[Sequence[int]], max_ne
     out: List[Optional[GenerationResult]] = [None] * len(prompts)
     for batch in batches:
         if hasattr(sampler, "begin"):
-            sampler.begin([request_ids[i] for i in batch], [prompts[i] for i in batch], max_new_tokens)
+            # (a sequence never chooses more than the longest one holds and one; "until it stops" may be any number)
+            sampler.begin([request_ids[i] for i in batch], [prompts[i] for i in batch], min(max_new_tokens, max_seq_len + 1))
         args = (engine, sampler, [prompts[i] for i in batch], [request_ids[i] for i in batch], max_new_tokens, stop, max_seq_len, on_token)
         if allowed_tokens is not None:
             res = run_batch(*args, allowed_tokens=allowed_tokens)
