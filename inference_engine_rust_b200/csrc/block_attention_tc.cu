@@ -3,13 +3,15 @@
 // The sequences' keys and values in 8 bits are all that has to come from memory, so everything is arranged around that stream:
 //   * A cluster of up to 16 CTAs shares one (sequence, kv head): each takes a run of its blocks, and each adds up a share of the
 //     outputs from what the others have put into its shared memory.  One launch, no scratch memory for partial outputs.
-//     (Two CTAs of eight warps an SM: in fours, two to a pair, 64 sequences of 4,096 positions take as long in bfloat16 runs, 69 us, and 83 for 74 in
+//     (Two CTAs of eight warps an SM; in fours, two to a pair, 64 sequences of 4,096 positions took as long in bfloat16 runs and an eighth longer in
 //     float32 runs.)
 //   * A warp owns a block (16 positions) at a time, with a ring of its own that cp.async fills: no barrier inside the loop.
 //   * Levels become fp16 in registers, exactly (int8: 1024 + (q + 128) by a byte permutation, minus 1152; e4m3: a conversion
 //     instruction), and are the 16-row operand of mma.m16n8k16: S^T = K Q^T has 16 positions x 8 heads, O^T = V^T P^T 16 dimensions x 8
 //     heads, so that a group of up to 8 query heads fills the narrow side.  Queries are scaled by a power of two of their row; bf16
-//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`).  Probabilities go in twice in every run.
+//     numbers are then exact in fp16, fp32 numbers go in twice, the upper 11 bits and the next 11 (`LO`).  Probabilities go in twice in
+//     every run: one half alone is off by 2^-12, which moves bfloat16 outputs past the border of their own rounding (64 sequences of up to 4,096
+//     positions, e4m3, took 62.0 us so, 64.6 with both).
 //   * The order of dimensions inside a product is free as long as both operands agree: a lane takes 16 neighbouring bytes of a key
 //     row for four steps (one 16-byte load), and 16 (8) neighbouring dimensions of four value rows.  P^T gets into operand form by
 //     two 8 x 8 transpositions in registers (movmatrix).
@@ -574,15 +576,15 @@ int launch(BlockTcParams p, const IertBatchView& b, const IertBlockView& c, int 
   const long long pairs = (long long)c.kv_heads * b.n_seqs;
   const int sms = iert_sm_count_cached();
   if (splits == 0) {
-    // The largest clusters that all run at once (8 sequences of 2,048 positions with 8 key heads: 22.8, 16.7, 13.7, 23.8 us with 1, 2, 4, 8 CTAs
-    // to a pair; two of 3,000: 18.8 us in clusters of 16, of which the device holds 14, and 11.9 of 8), those of 16 for sequences that may be long
-    // (one sequence of 700 positions: 7.9 us, 6.8 in clusters of 8; of 3,000: 8.9 and 9.3; of 6,000: 10.5 and 11.4).  Between one and two pairs an SM a second CTA evens
-    // out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 36.7 us for 44.3, of 1,024: 22.8 for 20.0).
+    // The largest clusters that all run at once (8 sequences of 2,048 positions with 8 key heads: 22.8, 17.8, 14.6, 24.0 us with 1, 2, 4, 8 CTAs
+    // to a pair; two of 3,000: 19.1 us in clusters of 16, of which the device holds 14, and 12.3 of 8), those of 16 for sequences that may be long
+    // (one sequence of 700 positions: 8.1 us, 7.2 in clusters of 8; of 3,000: 9.4 and 9.3; of 6,000: 11.3 and 11.8).  Between one and two pairs an SM a second CTA evens
+    // out what the SMs have to do, which is worth its start for long sequences (24 of 4,096: 38.4 us for 50.8, of 1,024: 23.3 for 21.2).
     const long long reach = (long long)c.ring_pages * c.page_tokens;       // the most that a sequence holds
     for (splits = reach >= 4096 ? MAX_SPLITS : 8; splits > 1 && pairs > clusters_at_once(kernel, splits, WARPS * 32, smem, known);) splits >>= 1;
     if (splits == 1 && pairs <= 2LL * sms && reach >= 4096) splits = 2;
   }
-  p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 71.5 us as they stand, 69.5 so)
+  p.by_length = pairs * splits > 2LL * sms;      // (64 sequences of up to 4,096 positions, e4m3: 85 us as they stand, 74 so)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(splits, c.kv_heads, b.n_seqs);
   cfg.blockDim = dim3(WARPS * 32);
@@ -601,7 +603,7 @@ int launch(BlockTcParams p, const IertBatchView& b, const IertBlockView& c, int 
 
 }  // namespace
 
-// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule below.
+// `splits` (1, 2, 4, 8, 16): CTAs that share a sequence's kv head; 0: by the rule above.
 int block_attention_tc(const void* qkv, void* out, const IertBatchView* batch, const IertBlockView* view, int heads, float scale,
                        float* scratch, float* weight_out, const float* inv_freq, int rotary_dim, int pairing, float rot_mul, int splits,
                        int* err, cudaStream_t stream) {

@@ -6,8 +6,8 @@
 //   S [128 positions x 32] = K [128 x 128] Q^T     Q: a head's query as fixed-point numbers, DIG signed digits of 7 bits (base 128)
 //   O [128 dimensions x 32] += V^T [128 x 128] P   P: a head's probabilities times value scales as 32-bit fixed-point numbers, four unsigned digits of 8 bits
 // A tile is eight blocks of 16 positions of a (sequence, kv head), keys row by row (K-major), the values' tile read with its columns as
-// rows (MN-major).  Every position is one thread of the softmax, which needs about 210 instructions a warp and tile (mma.sync with
-// its conversions: 3,100 for the same 128 positions): what remains is the stream of levels.
+// rows (MN-major).  Every position is one thread of the softmax, which needs about 265 instructions a warp and tile (mma.sync with
+// its conversions: 3,400 for the same 128 positions): what remains is the stream of levels.
 //   warps 0-3  softmax, a position per thread: a head's score from its digits, times the block's key scale; the probability times the
 //              block's value scale, as digits, into (swizzled) shared memory.  A head's unit is a power of two of its own and goes by these
 //              products alone, so that a block of large values that has no weight takes no digits from the others.  It moves where a tile's heaviest
@@ -162,7 +162,7 @@ __device__ __forceinline__ float head_value(const T* src, int d, const UmmaParam
 }
 
 // GROUPS: of four softmax warps each, which take the tiles in turn and keep an O, references and sums of their own.  One group and two CTAs
-// an SM where there are CTAs enough, else two groups and a deeper ring in one CTA an SM: a tile takes a group about 1.1 us, an SM's share of the
+// an SM where there are CTAs enough, else two groups and a deeper ring in one CTA an SM: a tile takes a group more than 1.1 us, an SM's share of the
 // memory's rate brings one in 0.75 us.
 template <typename T, int GROUPS, int NSTAGE, bool WIDE>
 __global__ void __launch_bounds__(GROUPS * SOFT + 128, 3 - GROUPS)
@@ -814,24 +814,24 @@ int launch(UmmaParams p, const IertBatchView& b, const IertBlockView& c, int spl
   const long long pairs = (long long)c.kv_heads * b.n_seqs, reach = (long long)c.ring_pages * c.page_tokens;         // the most that a sequence holds
   const int sms = iert_sm_count_cached();
   if (splits == 0) {
-    // The largest clusters, up to eight, that all run at once with a CTA an SM (8 sequences of 2,048 positions with 8 key heads: 15.9, 13.0, 21.0 us
-    // with 1, 2, 4 CTAs to a pair; two of 3,500: 17.4 us in clusters of eight, of which the device holds 15, and 10.7 of four).  Pairs that leave more
-    // than eight SMs each, and may be long, take them all without a cluster (one sequence of 8,192 positions: 11.4 us, 10.9 as a cluster; 16,384: 13.9
-    // and 15.2; 32,768: 19.6 and 24.0; 131,071: 54 and 86; two of 32,768: 25.4 and 26.9).
+    // The largest clusters, up to eight, that all run at once with a CTA an SM (8 sequences of 2,048 positions with 8 key heads: 15.4, 12.9, 20.8 us
+    // with 1, 2, 4 CTAs to a pair; two of 3,500: 17.3 us in clusters of eight, of which the device holds 15, and 10.8 of four).  Pairs that leave more
+    // than eight SMs each, and may be long, take them all without a cluster (one sequence of 8,192 positions: 11.8 us, 10.6 as a cluster; 16,384: 14.3
+    // and 15.1; 32,768: 20.1 and 23.6; 131,071: 53 and 78; two of 32,768: 26.0 and 26.4).
     if (pairs * (MAX_SPLITS + 1) <= sms && reach >= WIDE_FROM) splits = (int)(std::min(sms, MAX_PIECES) / pairs);
     else
       for (splits = MAX_SPLITS; splits > 1 && pairs > at_once<T, 2, 5>(splits);) splits >>= 1;
-    // Twice the CTAs, two an SM with one group each, where they all run at once and sequences may be long enough for a second start (16 of 4,096, 128
-    // pairs: 26.6 us, 24.3 so, of 1,024: 13.7 and 13.8; 56 pairs of 14,000: 37.7 and 31.8, of 3,500: 15.0 and 15.0; 24 pairs of 14,000: 20.9 and 19.5,
-    // of 7,000: 13.7 and 13.9; inside a model a start costs more: four layers, 8 sequences of 2,048 of at most 4,096: 448 us a step, 460 so).
+    // Twice the CTAs, two an SM with one group each, where they all run at once and sequences may be long enough for a second start (16 of 8,192, 128
+    // pairs: 42.8 us, 38.5 so, of 4,096: 25.8 and 25.6, of 1,024: 13.5 and 14.4; 56 pairs of 14,000: 36.8 and 32.9, of 8,192: 24.1 and 22.9, of 3,500: 14.6 and
+    // 15.5; 24 pairs of 30,000: 37.8 and 33.4, of 14,000: 21.8 and 22.0, of 7,000: 13.7 and 15.2; inside a model a start costs more: four layers, 8 sequences of 2,048 of at most 4,096: 448 us a step, 460 so).
     if (splits < MAX_SPLITS && groups != 2 && reach >= 4096 * splits && pairs <= at_once<T, 1, 2>(2 * splits)) splits *= 2;
   }
   const bool wide = splits > MAX_SPLITS;
-  // Two groups where a CTA has an SM to itself, one where two share it (64 sequences of 4,096 positions: 84 us and 72).  Between one and two pairs an SM,
-  // long sequences one after the other even out what the SMs have to do (24 of 4,096: 35.2 us for 37.2; 36 of 4,096: 45.7 and 43.1, of 8,192: 68.6 and
-  // 72.6; 20 of 2,048: 25.4 and 22.9).
+  // Two groups where a CTA has an SM to itself, one where two share it (64 sequences of 4,096 positions: 82 us and 74).  Between one and two pairs an SM,
+  // long sequences one after the other even out what the SMs have to do (24 of 4,096: 34.5 us for 39.0; 36 of 4,096: 45.2 and 44.7, of 8,192: 66.9 and
+  // 74.7; 20 of 2,048: 24.9 and 24.5).
   if (groups == 0) groups = wide || pairs <= at_once<T, 2, 5>(splits) || (splits == 1 && pairs <= 2LL * sms && pairs * 3000 <= reach * sms) ? 2 : 1;
-  p.by_length = pairs * splits > (groups == 2 ? sms : 2 * sms);      // (64 sequences of up to 4,096 positions: 80 us as they stand, 73 so)
+  p.by_length = pairs * splits > (groups == 2 ? sms : 2 * sms);      // (64 sequences of up to 4,096 positions: 83 us as they stand, 74 so)
   CUtensorMap mk, mv;
   const long long rows = (long long)c.n_pages * c.kv_heads * c.page_tokens;
   if (!level_map(c.k, rows, p.run, &mk) || !level_map(c.v, rows, p.run, &mv)) return IERT_BAD_ARGUMENT;
@@ -860,8 +860,8 @@ int block_attention_umma(const void* qkv, void* out, const IertBatchView* batch,
   const long long pairs = (long long)c.kv_heads * batch->n_seqs;
   if (splits < 0 || groups < 0 || groups > 2 || (splits > MAX_SPLITS ? pairs * splits > MAX_PIECES : (splits & (splits - 1)) != 0)) return IERT_BAD_ARGUMENT;
   // Few and short sequences are left to block_attention_tc.cu: its start overlaps the kernel in front and its end the one behind, which this one's shared and
-  // tensor memory do not allow (four layers of a model with 8 key heads: one sequence of 700 positions 408 us a step, 416 here; of 12,000 443 and 451;
-  // two of 7,000 448 and 464, of 12,000 498 and 488; three of 2,048 423 and 432, four 455 and 437; alone this kernel is the faster one by up to 1 us).
+  // tensor memory do not allow (four layers of a model with 8 key heads: one sequence of 700 positions 408 us a step, 418 here; of 12,000 445 and 451;
+  // two of 7,000 452 and 465, of 12,000 507 and 503; three of 2,048 425 and 433, four 465 and 437; alone this kernel is the faster one by up to 1 us).
   if (splits == 0 && groups == 0 && pairs <= 24 && pairs * c.ring_pages * c.page_tokens < 120000) return IERT_BAD_ARGUMENT;
   UmmaParams p = {};
   p.run = TILE_BLOCKS;

@@ -1,6 +1,5 @@
 // The cache in 8 bits (block_cache.cuh): writing a step's keys and values, one-token attention over it as the equations say (any
-// head size up to 256; block_attention_tc.cu has the tensor-core form of the usual sizes), and eviction of the blocks
-// that attention has weighed least.
+// head size up to 256; block_attention_tc.cu and block_attention_umma.cu have the tensor-core forms of the usual sizes).
 #include <type_traits>
 
 #include "block_cache.cuh"
@@ -12,10 +11,11 @@ namespace {
 // ---------------------------------------------------------------------------------------
 // Store: the keys and values of a step's tokens, positions [pos0, pos0 + q) of each sequence.  One CTA per (block of 16
 // positions, kv head), half of it for the keys and half for the values.  The blocks of sequence s are the units [cu_q[s] / 16 + 2 s, ...): q
-// tokens touch at most q / 16 + 2 blocks.  A step reads and writes each number once, and its time is that of one chain of loads: so a
+// tokens touch at most q / 16 + 2 blocks.  A step reads and writes each number once, and few tokens take the time of one chain of loads: so a
 // thread asks for all its numbers (eight at a time, `RUNS` runs of them), keeps them in registers over the search for the
 // largest, and writes their levels; the page is looked up while they are on their way.  2,048 tokens of 8 heads of 128 take 6 us (38 with two
-// passes of single numbers), 16,001 of 4 heads of 64, 25 MB, 12; two heads of 64 a CTA, with half the overhead, took 15.
+// passes of single numbers), 16,001 of 4 heads of 64, 25 MB, 12, which is the time to issue 9.4 M warp instructions (2.5 of 4 a cycle): about 36 a
+// number, most of them a CTA's own setup and the levels' two roundings; two heads of 64 a CTA, with half the setup, took 15.
 constexpr int STORE_THREADS = 128, HALF = STORE_THREADS / 2;
 
 __device__ __forceinline__ void load8(const float* p, float (&x)[8]) {

@@ -121,7 +121,7 @@ template <int FMT> __device__ __forceinline__ uint8_t to_level(float x, float sc
 }
 // Levels of four numbers, the first in the lowest byte, to the bit what `to_level` gives, at a fifth of its instructions: x / scale, rounded,
 // lies within three roundings of q = x * (1 / scale), so where q (1 - 2^-21) and q (1 + 2^-21) have the same level it is that one, and
-// only where a border lies between them (int8: at most 6 numbers in 100,000) is the division carried out.  `inv`: see below.
+// only where a border lies between them (int8: 3 of 100,000 normal numbers, at most 12) is the division carried out.  `inv`: see below.
 template <int FMT> __device__ __forceinline__ uint32_t to_levels4(const float* x, float scale, float inv) {
   constexpr float DOWN = 1.f - 0x1p-21f, UP = 1.f + 0x1p-21f;
   uint32_t w[2];

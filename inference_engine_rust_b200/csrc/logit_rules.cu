@@ -44,7 +44,7 @@ struct RulesParams {
 
 __device__ __forceinline__ bool better(float v, int i, float bv, int bi) { return v > bv || (v == bv && i < bi); }
 
-// Count: 16-bit words serve histories of up to 32,767 tokens (32 KB a window), 32-bit words longer ones.  The highest bit: seen at all.
+// Count: 16-bit words serve histories of up to 32,767 tokens (64 KB for the COUNTED ids), 32-bit words longer ones.  The highest bit: seen at all.
 // VEC: rows, biases and results in 16-byte runs.
 template <typename Count, bool VEC>
 __global__ void __launch_bounds__(THREADS, 2) logit_rules_kernel(RulesParams p) {

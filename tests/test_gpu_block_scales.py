@@ -95,7 +95,7 @@ def noise(g, *shape):
 @pytest.mark.parametrize("fmt, D, H", [(torch.int8, 128, 8), (torch.int8, 64, 5), (torch.int8, 128, 12), (torch.float8_e4m3fn, 128, 4), (torch.float8_e4m3fn, 64, 8)])
 def test_bfloat16_outputs_are_rounded_once(kernel, fmt, D, H):
     """Weights that differ little over few positions, so that all that may be seen beside the output's own rounding is a few 2^-20: a
-    weight rounded to 11 bits where it multiplies values moves one output in fifty past a border."""
+    weight rounded to 11 bits where it multiplies values moves outputs past a border."""
     r = Apart(2, 2 * H, D, fmt, torch.bfloat16, n_slots=4, width=2, seed=H)
     for slot, n in enumerate((16, 35, 64, 100)):
         r.fill(slot, noise(r.g, n, 2, D), noise(r.g, n, 2, D))
